@@ -1,0 +1,471 @@
+"""Serving several sequences at once: a paged KV cache held in 4 bits, and the attention around it, as timed cases.
+
+Four operators that one serving step strings together:
+
+  append  a step's new tokens: per-head q/k RMSNorm, rotary position, and K/V quantized into the pages. The
+          outputs are the rotated q (and, for prompts, the rotated k) and the new rows as the cache now holds them,
+          which is the append and a read of those rows.
+  read    the cached K and V of packed sequences, back as binary16 rows.
+  attend  one query token per sequence over its cached context.
+  prompt  causal attention of packed prompts (or of the last part of each) over binary16 K and V.
+
+Cache format. A page holds `page` tokens of every KV head. Values are symmetric INT4, q in [-7, 7], one binary16
+scale per token, head and group of `group` dimensions: s = fp16(max|x| / 7), q = clamp(round_half_even(x / s)),
+value q * s. Eight values share a 32-bit word, nibble i holding value AWQ[i].
+  k_pages [P, NKV, page, hd / 2]: a token's hd / 8 words, word w * g + i holding dimensions 8 (4 i + g) .. + 7
+          (w = hd / 32, g = 0 .. 3);
+  v_pages [P, NKV, page, hd / 2]: the words of four tokens interleaved, [page / 4][hd / 8][4 tokens];
+  k_scale, v_scale [P, NKV, hd / group, page].
+Sequence b's token t is in slot t % page of page block_table[b, t // page].
+"""
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+_PKG = str(Path(__file__).resolve().parent.parent / "sparse-offload-infer_amd")
+if _PKG not in sys.path:
+    sys.path.insert(0, _PKG)
+
+own = False
+
+AWQ = (0, 2, 4, 6, 1, 3, 5, 7)
+EPS = 1e-6
+THETA = 1e6
+
+
+# ---------------------------------------------------------------------------
+# the cases
+# ---------------------------------------------------------------------------
+
+def listed():
+    return [
+        # one token of one conversation enters the cache: a call's fixed cost
+        dict(name="append_1", kind="append", NQ=16, NKV=8, hd=128, group=64, page=64, B=1, new=1, old=1998,
+             mix=1, keep_k=False, norm=True),
+        # a decode step of a busy server: one token each of 200 sequences
+        dict(name="append_200", kind="append", NQ=32, NKV=8, hd=128, group=32, page=16, B=200, new=1, old=8000,
+             mix=2, keep_k=False, norm=True),
+        # a batch of prompts enters the cache; the prompt attention wants the rotated k too
+        dict(name="append_prompts", kind="append", NQ=16, NKV=8, hd=128, group=64, page=64, B=24, new=1024, old=0,
+             mix=3, keep_k=True, norm=True),
+        # one conversation's context read back, narrow heads
+        dict(name="read_300", kind="read", NQ=14, NKV=2, hd=64, group=32, page=32, B=1, old=300, mix=4),
+        # the cached context of a batch read back for a prompt that continues it
+        dict(name="read_16", kind="read", NQ=16, NKV=8, hd=128, group=64, page=64, B=16, old=8192, mix=5),
+        # a single conversation late in a 2048-token context
+        dict(name="attend_1", kind="attend", NQ=16, NKV=8, hd=128, group=128, page=64, B=1, old=1999, mix=6),
+        # a decode step of a busy server, contexts of all lengths
+        dict(name="attend_48", kind="attend", NQ=32, NKV=8, hd=128, group=32, page=16, B=48, old=4095, mix=7),
+        # a few very long documents
+        dict(name="attend_long", kind="attend", NQ=64, NKV=8, hd=128, group=64, page=256, B=4, old=131072, mix=8),
+        # one short question
+        dict(name="prompt_37", kind="prompt", NQ=16, NKV=8, hd=128, B=1, new=37, old=0, mix=9),
+        # a batch of ordinary prompts of different lengths
+        dict(name="prompt_20", kind="prompt", NQ=32, NKV=8, hd=128, B=20, new=1000, old=0, mix=10),
+        # the next part of prompts whose beginning is cached, narrow heads
+        dict(name="prompt_part", kind="prompt", NQ=14, NKV=2, hd=64, B=5, new=513, old=4000, mix=11),
+        # one long document
+        dict(name="prompt_16k", kind="prompt", NQ=16, NKV=8, hd=128, B=1, new=16384, old=0, mix=12),
+    ]
+
+
+HEADS = ((16, 8), (32, 8), (8, 8), (64, 8), (14, 2), (40, 8), (12, 1))
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """Any head layout, width, group, page and batch of the ranges above, no more work than the largest listed."""
+    kind = rng.choice(("append", "read", "attend", "prompt"))
+    NQ, NKV = rng.choice(HEADS)
+    hd = rng.choice((64, 128, 128, 256))
+    group = rng.choice([g for g in (32, 64, 128) if g <= hd])
+    c = dict(kind=kind, NQ=NQ, NKV=NKV, hd=hd, group=group, page=rng.choice((16, 32, 64, 128, 256)),
+             mix=rng.randrange(1 << 30))
+    if kind == "append":
+        B = _log(rng, 1, 256)
+        new = 1 if rng.random() < 0.4 else _log(rng, 2, 16384)
+        while B * new * (NQ + 2 * NKV) * hd > 24 * 1024 * 32 * 128:
+            B, new = max(1, B // 2), max(1, new * 3 // 4)
+        c.update(B=B, new=new, old=_log(rng, 1, 16000) - 1, keep_k=rng.random() < 0.5, norm=rng.random() < 0.7)
+    elif kind == "read":
+        B, old = _log(rng, 1, 64), _log(rng, 1, 32768)
+        while B * old * NKV * hd > 16 * 8192 * 8 * 128:
+            B, old = max(1, B // 2), max(1, old * 3 // 4)
+        c.update(B=B, old=old)
+    elif kind == "attend":
+        B, old = _log(rng, 1, 256), _log(rng, 1, 131072)
+        while B * old * NKV * hd > 4 * 131072 * 8 * 128 // 4:
+            B, old = max(1, B // 2), max(1, old * 3 // 4)
+        c.update(B=B, old=old)
+    else:
+        B, new = _log(rng, 1, 48), _log(rng, 1, 16384)
+        old = 0 if rng.random() < 0.6 else _log(rng, 1, 8192)
+        while B * new * (new + 2 * old) * NQ * hd > 16384 * 16384 * 16 * 128 // 2:
+            B, new, old = max(1, B * 3 // 4), max(1, new * 3 // 4), old * 3 // 4
+        c.update(B=B, new=new, old=old)
+        del c["group"], c["page"]
+    return c
+
+
+def _lengths(case):
+    """(tokens in the cache before the call, new tokens) of each sequence: the last has both maxima, the others any
+    length up to them (decode steps: one new token each)."""
+    r = random.Random(case["mix"])
+    B, old, new = case["B"], case["old"], case.get("new", 0)
+    olds = [r.randint(0, old) for _ in range(B - 1)] + [old]
+    news = [new if new <= 1 else r.randint(0, new) for _ in range(B - 1)] + [new]
+    return olds, news
+
+
+# ---------------------------------------------------------------------------
+# inputs
+# ---------------------------------------------------------------------------
+
+def _offsets(ns, dev):
+    out = [0]
+    for n in ns:
+        out.append(out[-1] + n)
+    return torch.tensor(out, dtype=torch.int32, device=dev)
+
+
+def _kv_order(hd):
+    w = hd // 32
+    return [4 * (p % w) + p // w for p in range(hd // 8)]
+
+
+def _quantized_words(x, group):
+    """x [..., hd] fp16 -> (int32 words [..., hd / 8] in dimension order, fp16 scales [..., hd / group])."""
+    g = x.float().unflatten(-1, (-1, group))
+    s = (g.abs().amax(-1) / 7).half()
+    q = torch.where(s[..., None] > 0, torch.round(g / s.float()[..., None]), 0).clamp(-7, 7).to(torch.int32)
+    q = q.flatten(-2).unflatten(-1, (-1, 8)) & 15
+    words = torch.zeros(q.shape[:-1], dtype=torch.int32, device=x.device)
+    for i in range(8):
+        words |= q[..., AWQ[i]] << (4 * i)
+    return words, s
+
+
+def _cache(case, gen, total, table_len, dev, fill):
+    """Pages with the K and V of earlier tokens: K with a few strong channels, as projections have them, V near normal."""
+    NKV, hd, group, page = case["NKV"], case["hd"], case["group"], case["page"]
+    P = max(1, total) + 3
+    shape = (P, NKV, page, hd)
+    if fill:
+        ch = torch.exp(0.6 * torch.randn(1, NKV, 1, hd, generator=gen, device=dev))
+        kw, ks = _quantized_words((torch.randn(shape, generator=gen, device=dev) * ch).half(), group)
+        vw, vs = _quantized_words((torch.randn(shape, generator=gen, device=dev) * 0.7).half(), group)
+    else:
+        kw = torch.zeros((P, NKV, page, hd // 8), dtype=torch.int32, device=dev)
+        ks = torch.zeros((P, NKV, page, hd // group), dtype=torch.float16, device=dev)
+        vw, vs = kw.clone(), ks.clone()
+    kw = kw[..., _kv_order(hd)].contiguous()
+    vw = vw.unflatten(2, (page // 4, 4)).transpose(3, 4).contiguous()
+    return dict(k_pages=kw.view(torch.uint8).view(P, NKV, page, hd // 2), k_scale=ks.transpose(2, 3).contiguous(),
+                v_pages=vw.view(torch.uint8).view(P, NKV, page, hd // 2), v_scale=vs.transpose(2, 3).contiguous())
+
+
+def _table(lens, page, P, gen, dev):
+    """Block table: the sequences' pages in any order; entries behind a sequence's last page are 0."""
+    counts = [-(-n // page) for n in lens]
+    order = torch.randperm(P, generator=gen, device=dev).to(torch.int32)
+    table = torch.zeros((len(lens), max(1, max(counts))), dtype=torch.int32, device=dev)
+    at = 0
+    for b, n in enumerate(counts):
+        table[b, :n] = order[at:at + n]
+        at += n
+    return table
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    gen = torch.Generator(device=dev).manual_seed(seed)
+    kind, NQ, NKV, hd, B = case["kind"], case["NQ"], case["NKV"], case["hd"], case["B"]
+    olds, news = _lengths(case)
+    s = dict(case=case, kind=kind)
+
+    def randn(*shape, scale=1.0):
+        return (torch.randn(shape, generator=gen, device=dev) * scale).half()
+
+    if kind == "prompt":
+        # q, k, v as the attention gets them: q rotated and contiguous, k likewise, v a view of the projection's rows
+        T, Tk = sum(news), sum(olds) + sum(news)
+        s.update(q=randn(T, NQ, hd), k=randn(Tk, NKV, hd), v=randn(Tk, 2 * NKV, hd)[:, NKV:],
+                 cu_q=_offsets(news, dev), cu_k=_offsets([o + n for o, n in zip(olds, news)], dev),
+                 max_q=max(news), max_k=max(o + n for o, n in zip(olds, news)))
+        return s
+    lens = [o + n for o, n in zip(olds, news)]
+    page = case["page"]
+    pages = sum(-(-n // page) for n in lens)
+    s.update(_cache(case, gen, pages, 0, dev, kind != "append"))
+    s.update(table=_table(lens, page, s["k_pages"].shape[0], gen, dev), max_len=max(lens),
+             lens=torch.tensor(lens, dtype=torch.int32, device=dev))
+    if kind == "append":
+        T = sum(news)
+        angle = torch.arange(max(lens), dtype=torch.float64, device=dev)[:, None] * \
+            THETA ** (-torch.arange(0, hd, 2, dtype=torch.float64, device=dev) / hd)
+        s.update(qkv=randn(T, (NQ + 2 * NKV) * hd), cos=angle.cos().float(), sin=angle.sin().float(),
+                 cu=_offsets(news, dev), tokens=T, q_norm=None, k_norm=None)
+        if case["norm"]:
+            s.update(q_norm=1 + randn(hd, scale=0.2), k_norm=1 + randn(hd, scale=0.2))
+        if case["keep_k"]:
+            s["k_out"] = torch.empty((T, NKV, hd), dtype=torch.float16, device=dev)
+    elif kind == "read":
+        s.update(cu=_offsets(lens, dev), tokens=sum(lens))
+    else:
+        s["q"] = randn(B, NQ, hd, scale=1.5)
+    return s
+
+
+# ---------------------------------------------------------------------------
+# the plain form
+# ---------------------------------------------------------------------------
+
+def _values(words, scale):
+    """int32 words [..., n] in dimension order, scales [..., G] -> fp32 values [..., 8 n]."""
+    shift = torch.tensor([4 * AWQ.index(j) for j in range(8)], dtype=torch.int32, device=words.device)
+    q = (words[..., None] >> shift) & 15
+    q = (q - ((q & 8) << 1)).flatten(-2).float()
+    return (q.unflatten(-1, (scale.shape[-1], -1)) * scale.float()[..., None]).flatten(-2)
+
+
+def _unpaged(s):
+    """The pages as fp32 values [P, NKV, page, hd]."""
+    P, NKV, page, half = s["k_pages"].shape
+    back = torch.tensor(_kv_order(2 * half), device=s["k_pages"].device).argsort()
+    kw = s["k_pages"].view(torch.int32)[..., back]
+    vw = s["v_pages"].view(torch.int32).view(P, NKV, page // 4, half // 4, 4).transpose(3, 4).flatten(2, 3)
+    return _values(kw, s["k_scale"].transpose(2, 3)), _values(vw, s["v_scale"].transpose(2, 3))
+
+
+def _token_slots(s):
+    """For each packed token: its position, and its page and slot."""
+    cu, lens, page = s["cu"].long(), s["lens"].long(), s["k_pages"].shape[2]
+    t = torch.arange(s["tokens"], device=cu.device)
+    b = torch.bucketize(t, cu[1:], right=True)
+    pos = lens[b] - cu[b + 1] + t
+    return pos, s["table"].long()[b, pos // page], pos % page
+
+
+def _plain_append(s):
+    NQ, NKV, hd, group = (s["case"][n] for n in ("NQ", "NKV", "hd", "group"))
+    x = s["qkv"].view(-1, NQ + 2 * NKV, hd).double()  # 64 bits: values next to a rounding border of the 4-bit codes
+    qk, v = x[:, :NQ + NKV], x[:, NQ + NKV:]
+    if s["q_norm"] is not None:
+        w = torch.cat([s["q_norm"].expand(NQ, hd), s["k_norm"].expand(NKV, hd)]).double()
+        qk = qk * (1 / torch.sqrt(qk.square().mean(-1, keepdim=True) + EPS)) * w
+        qk = qk.half().double()
+    pos, _, _ = _token_slots(s)
+    c, sn = s["cos"][pos].double()[:, None], s["sin"][pos].double()[:, None]
+    a, b = qk.chunk(2, -1)
+    qk = torch.cat([a * c - b * sn, b * c + a * sn], -1).half()
+    kv = torch.cat([qk[:, NQ:], v.half()], 1).float().unflatten(-1, (-1, group))
+    scale = (kv.abs().amax(-1, keepdim=True) / 7).half().float()
+    code = torch.where(scale > 0, torch.round(kv / scale), 0).clamp(-7, 7)
+    kv = (code * scale).flatten(-2).half()
+    out = dict(q=qk[:, :NQ].contiguous(), cached_k=kv[:, :NKV].contiguous(), cached_v=kv[:, NKV:].contiguous())
+    if "k_out" in s:
+        out["k"] = qk[:, NQ:].contiguous()
+    return out
+
+
+def _plain_read(s):
+    k, v = _unpaged(s)
+    _, pg, slot = _token_slots(s)
+    return dict(k=k[pg, :, slot].half(), v=v[pg, :, slot].half())
+
+
+def _softmax_product(scores, mask, v):
+    """softmax(scores where mask) @ v, zeros in rows without a key."""
+    scores = torch.where(mask, scores, -math.inf)
+    top = scores.amax(-1, keepdim=True)
+    p = torch.exp(scores - torch.where(torch.isfinite(top), top, 0))
+    total = p.sum(-1, keepdim=True)
+    return torch.matmul(p, v) / torch.where(total > 0, total, 1)
+
+
+def _plain_attend(s):
+    q = s["q"]
+    B, NQ, hd = q.shape
+    NKV, L = s["k_pages"].shape[1], s["max_len"]
+    k, v = (x[s["table"].long()].transpose(1, 2).flatten(2, 3)[:, :, :L] for x in _unpaged(s))  # [B, NKV, L, hd]
+    q = q.float().view(B, NKV, NQ // NKV, hd)
+    live = torch.arange(L, device=q.device) < s["lens"][:, None]
+    out = _softmax_product(torch.matmul(q, k.transpose(2, 3)) / math.sqrt(hd), live[:, None, None], v)
+    return out.reshape(B, NQ, hd).half()
+
+
+def _padded(x, cu, most):
+    """x [T, heads, hd] of packed sequences -> fp32 [B, heads, most, hd], the rows' places, and which are real."""
+    i = torch.arange(most, device=x.device)
+    real = i < (cu[1:] - cu[:-1])[:, None]
+    at = torch.where(real, cu[:-1, None] + i, 0).long()
+    return x[at].transpose(1, 2).float(), at, real
+
+
+def _plain_prompt(s):
+    T, NQ, hd = s["q"].shape
+    NKV, rep = s["k"].shape[1], NQ // s["k"].shape[1]
+    q, at, real = _padded(s["q"], s["cu_q"], s["max_q"])
+    k, _, _ = _padded(s["k"], s["cu_k"], s["max_k"])
+    v, _, _ = _padded(s["v"], s["cu_k"], s["max_k"])
+    B, _, Sq, _ = q.shape
+    nq, nk = (s[c][1:] - s[c][:-1] for c in ("cu_q", "cu_k"))
+    last = torch.arange(Sq, device=q.device) + (nk - nq)[:, None]  # the last key that query i sees
+    mask = torch.arange(s["max_k"], device=q.device) <= last[..., None]  # [B, Sq, Sk]
+    mask = mask[:, None, None].expand(-1, -1, rep, -1, -1).reshape(B, 1, rep * Sq, -1)
+    q = q.reshape(B, NKV, rep * Sq, hd)
+    out = _softmax_product(torch.matmul(q, k.transpose(2, 3)) / math.sqrt(hd), mask, v)
+    out = out.view(B, NQ, Sq, hd).transpose(1, 2)[real]
+    return out.half()
+
+
+# ---------------------------------------------------------------------------
+# one pass
+# ---------------------------------------------------------------------------
+
+def _pages(s):
+    return s["k_pages"], s["k_scale"], s["v_pages"], s["v_scale"]
+
+
+def run(s):
+    kind = s["kind"]
+    if own:
+        from soinfer import ops
+
+        if kind == "append":
+            q = ops.kv4_append(s["qkv"], s["q_norm"], s["k_norm"], s["cos"], s["sin"], *_pages(s), s["table"],
+                               s["lens"], s["cu"], s["case"]["NQ"], EPS, k_out=s.get("k_out"))
+            k, v = ops.kv4_read(*_pages(s), s["table"], s["lens"], s["cu"], s["tokens"])
+            out = dict(q=q, cached_k=k, cached_v=v)
+            if "k_out" in s:
+                out["k"] = s["k_out"]
+            return out
+        if kind == "read":
+            k, v = ops.kv4_read(*_pages(s), s["table"], s["lens"], s["cu"], s["tokens"])
+            return dict(k=k, v=v)
+        if kind == "attend":
+            return ops.kv4_decode_attention(s["q"], *_pages(s), s["table"], s["lens"], max_len=s["max_len"])
+        return ops.prompt_attention(s["q"], s["k"], s["v"], s["cu_q"], s["cu_k"], s["max_q"])
+    if kind == "append":
+        return _plain_append(s)
+    if kind == "read":
+        return _plain_read(s)
+    if kind == "attend":
+        return _plain_attend(s)
+    return _plain_prompt(s)
+
+
+def work(case):
+    """Inputs once, outputs once; of the cache only the tokens that the call concerns."""
+    NQ, NKV, hd = case["NQ"], case["NKV"], case["hd"]
+    olds, news = _lengths(case)
+    if case["kind"] == "prompt":
+        pairs = sum(n * o + n * (n + 1) // 2 for o, n in zip(olds, news))
+        rows = 2 * NQ * sum(news) + 2 * NKV * (sum(olds) + sum(news))
+        return dict(bytes=2 * hd * rows, flops=4 * pairs * NQ * hd)
+    token = 2 * NKV * (hd // 2 + 2 * (hd // case["group"]))  # a token's cached bytes
+    if case["kind"] == "append":
+        T = sum(news)
+        values = (NQ + 2 * NKV) * hd * T
+        kept = NKV * hd * T if case["keep_k"] else 0
+        # the projection, the rotations, q (k), the pages written, and the new rows read back and returned
+        return dict(bytes=2 * values + 4 * hd * T + 2 * NQ * hd * T + 2 * kept + 2 * token * T + 4 * NKV * hd * T,
+                    flops=12 * values)
+    L = sum(olds)
+    if case["kind"] == "read":
+        return dict(bytes=(token + 4 * NKV * hd) * L, flops=2 * NKV * hd * L)
+    return dict(bytes=token * L + 4 * case["B"] * NQ * hd, flops=4 * L * NQ * hd)
+
+
+# ---------------------------------------------------------------------------
+# in 64 bits
+# ---------------------------------------------------------------------------
+
+def _exact_page_rows(s, b, first, last):
+    """K and V [last - first, NKV, hd] of sequence b's positions first .. last - 1, in 64 bits, nibble by nibble."""
+    page, dev = s["k_pages"].shape[2], s["k_pages"].device
+    hd = 2 * s["k_pages"].shape[3]
+    pos = torch.arange(first, last, device=dev)
+    pg, slot = s["table"][b][pos // page].long(), pos % page
+    d = torch.arange(hd, device=dev)
+    octet, nibble = d // 8, torch.tensor([AWQ.index(j) for j in range(8)], device=dev)[d % 8]
+    w = hd // 32
+    k_byte = ((octet % 4) * w + octet // 4) * 4 + nibble // 2
+    v_byte = ((slot[:, None] // 4 * (hd // 8) + octet) * 4 + slot[:, None] % 4) * 4 + nibble // 2  # in the head's page
+
+    def signed(byte):
+        q = torch.where(nibble % 2 == 1, byte >> 4, byte & 15).double()
+        return torch.where(q >= 8, q - 16, q)
+
+    k = signed(s["k_pages"][pg, :, slot][..., k_byte])
+    head = torch.arange(s["k_pages"].shape[1], device=dev)
+    v = signed(s["v_pages"].flatten(2)[pg[:, None, None], head[:, None], v_byte[:, None]])
+    G = s["k_scale"].shape[2]
+    spread = d // (hd // G)
+    return k * s["k_scale"][pg, :, :, slot].double()[..., spread], v * s["v_scale"][pg, :, :, slot].double()[..., spread]
+
+
+def _exact_attention(q, k, v, last):
+    """q [n, NQ, hd] over k, v [m, NKV, hd]; query i sees keys 0 .. last[i]."""
+    rep = q.shape[1] // k.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    key = torch.arange(k.shape[0], device=q.device)
+    for h in range(q.shape[1]):
+        kh, vh = k[:, h // rep].contiguous(), v[:, h // rep].contiguous()
+        for i in range(0, q.shape[0], 4096):
+            z = q[i:i + 4096, h] @ kh.T / q.shape[2] ** 0.5
+            z.masked_fill_(key > last[i:i + 4096, None], -math.inf)
+            out[i:i + 4096, h] = torch.softmax(z, -1).nan_to_num(0.0) @ vh if k.shape[0] else 0.0
+    return out
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    kind, NQ, NKV, hd = case["kind"], case["NQ"], case["NKV"], case["hd"]
+    dev = torch.device("cuda")
+    olds, news = _lengths(case)
+    if kind == "prompt":
+        out, q0, k0 = [], 0, 0
+        for o, n in zip(olds, news):
+            q = s["q"][q0:q0 + n].double()
+            k, v = (s[x][k0:k0 + o + n].double() for x in "kv")
+            out.append(_exact_attention(q, k, v, torch.arange(n, device=dev) + o))
+            q0, k0 = q0 + n, k0 + o + n
+        return torch.cat(out)
+    if kind == "attend":
+        return torch.cat([_exact_attention(s["q"][b:b + 1].double(), *_exact_page_rows(s, b, 0, n),
+                                           torch.tensor([n - 1], device=dev)) for b, n in enumerate(olds)])
+    if kind == "read":
+        rows = [_exact_page_rows(s, b, 0, n) for b, n in enumerate(olds)]
+        return dict(k=torch.cat([r[0] for r in rows]), v=torch.cat([r[1] for r in rows]))
+    # append: the definition rounds to binary16 after the norm, and once more where k enters the cache
+    x = s["qkv"].double().unflatten(-1, (NQ + 2 * NKV, hd))
+    q, k, v = x[:, :NQ], x[:, NQ:NQ + NKV], x[:, NQ + NKV:]
+    pos = torch.cat([torch.arange(o, o + n, device=dev) for o, n in zip(olds, news)])
+
+    def turned(x, w):
+        if w is not None:
+            x = (x / torch.sqrt((x * x).sum(-1, keepdim=True) / hd + EPS) * w.double()).to(torch.float16).double()
+        lo, hi = x[..., :hd // 2], x[..., hd // 2:]
+        c, sn = s["cos"].double()[pos].unsqueeze(1), s["sin"].double()[pos].unsqueeze(1)
+        return torch.cat((lo * c - hi * sn, hi * c + lo * sn), -1)
+
+    def held(x):
+        g = x.to(torch.float16).double().reshape(*x.shape[:2], -1, case["group"])
+        step = (g.abs().max(-1, keepdim=True).values / 7).to(torch.float16).double()
+        code = torch.round(g / step.clamp_min(2.0 ** -24)).clamp(-7, 7)
+        return (code * step).reshape(x.shape)
+
+    q, k = turned(q, s["q_norm"]), turned(k, s["k_norm"])
+    out = dict(q=q, cached_k=held(k), cached_v=held(v))
+    if case["keep_k"]:
+        out["k"] = k
+    return out
