@@ -11,10 +11,11 @@ Four operators that one serving step strings together:
 
 Cache format. A page holds `page` tokens of every KV head. Values are symmetric INT4, q in [-7, 7], one binary16
 scale per token, head and group of `group` dimensions: s = fp16(max|x| / 7), q = clamp(round_half_even(x / s)),
-value q * s. Eight values share a 32-bit word, nibble i holding value AWQ[i].
-  k_pages [P, NKV, page, hd / 2]: a token's hd / 8 words, word w * g + i holding dimensions 8 (4 i + g) .. + 7
-          (w = hd / 32, g = 0 .. 3);
-  v_pages [P, NKV, page, hd / 2]: the words of four tokens interleaved, [page / 4][hd / 8][4 tokens];
+value q * s.
+  k_pages [P, NKV, page, hd / 2]: a token's hd / 8 words of 32 bits, word w * g + i holding dimensions
+          8 (4 i + g) .. + 7 (w = hd / 32, g = 0 .. 3), nibble n of a word its dimension AWQ[n];
+  v_pages [P, NKV, page, hd / 2]: units of 16 bits, [page / 4][16][hd / 64][4 tokens], nibble n of unit (m, u) the
+          dimension 64 u + 16 n + m;
   k_scale, v_scale [P, NKV, hd / group, page].
 Sequence b's token t is in slot t % page of page block_table[b, t // page].
 """
@@ -141,35 +142,46 @@ def _kv_order(hd):
     return [4 * (p % w) + p // w for p in range(hd // 8)]
 
 
-def _quantized_words(x, group):
-    """x [..., hd] fp16 -> (int32 words [..., hd / 8] in dimension order, fp16 scales [..., hd / group])."""
+def _quantized(x, group):
+    """x [..., hd] fp16 -> (codes int32 [..., hd] in 0 .. 15, fp16 scales [..., hd / group])."""
     g = x.float().unflatten(-1, (-1, group))
     s = (g.abs().amax(-1) / 7).half()
     q = torch.where(s[..., None] > 0, torch.round(g / s.float()[..., None]), 0).clamp(-7, 7).to(torch.int32)
-    q = q.flatten(-2).unflatten(-1, (-1, 8)) & 15
-    words = torch.zeros(q.shape[:-1], dtype=torch.int32, device=x.device)
-    for i in range(8):
-        words |= q[..., AWQ[i]] << (4 * i)
-    return words, s
+    return q.flatten(-2) & 15, s
 
 
-def _cache(case, gen, total, table_len, dev, fill):
+def _k_bytes(q):
+    """Codes [P, NKV, page, hd] -> k_pages."""
+    P, NKV, page, hd = q.shape
+    q = q.unflatten(-1, (-1, 8))
+    words = sum(q[..., AWQ[i]] << (4 * i) for i in range(8))
+    return words[..., _kv_order(hd)].contiguous().view(torch.uint8).view(P, NKV, page, hd // 2)
+
+
+def _v_bytes(q):
+    """Codes [P, NKV, page, hd] -> v_pages."""
+    P, NKV, page, hd = q.shape
+    q = q.view(P, NKV, page // 4, 4, hd // 64, 4, 16)  # ..., token, u, nibble, m
+    units = sum(q[..., n, :] << (4 * n) for n in range(4)).permute(0, 1, 2, 5, 4, 3)
+    return units.to(torch.int16).contiguous().view(torch.uint8).view(P, NKV, page, hd // 2)
+
+
+def _cache(case, gen, total, dev, fill):
     """Pages with the K and V of earlier tokens: K with a few strong channels, as projections have them, V near normal."""
     NKV, hd, group, page = case["NKV"], case["hd"], case["group"], case["page"]
     P = max(1, total) + 3
     shape = (P, NKV, page, hd)
     if fill:
         ch = torch.exp(0.6 * torch.randn(1, NKV, 1, hd, generator=gen, device=dev))
-        kw, ks = _quantized_words((torch.randn(shape, generator=gen, device=dev) * ch).half(), group)
-        vw, vs = _quantized_words((torch.randn(shape, generator=gen, device=dev) * 0.7).half(), group)
+        kq, ks = _quantized((torch.randn(shape, generator=gen, device=dev) * ch).half(), group)
+        vq, vs = _quantized((torch.randn(shape, generator=gen, device=dev) * 0.7).half(), group)
+        kb, vb = _k_bytes(kq), _v_bytes(vq)
     else:
-        kw = torch.zeros((P, NKV, page, hd // 8), dtype=torch.int32, device=dev)
+        kb = torch.zeros((P, NKV, page, hd // 2), dtype=torch.uint8, device=dev)
         ks = torch.zeros((P, NKV, page, hd // group), dtype=torch.float16, device=dev)
-        vw, vs = kw.clone(), ks.clone()
-    kw = kw[..., _kv_order(hd)].contiguous()
-    vw = vw.unflatten(2, (page // 4, 4)).transpose(3, 4).contiguous()
-    return dict(k_pages=kw.view(torch.uint8).view(P, NKV, page, hd // 2), k_scale=ks.transpose(2, 3).contiguous(),
-                v_pages=vw.view(torch.uint8).view(P, NKV, page, hd // 2), v_scale=vs.transpose(2, 3).contiguous())
+        vb, vs = kb.clone(), ks.clone()
+    return dict(k_pages=kb, k_scale=ks.transpose(2, 3).contiguous(), v_pages=vb,
+                v_scale=vs.transpose(2, 3).contiguous())
 
 
 def _table(lens, page, P, gen, dev):
@@ -204,7 +216,7 @@ def prepare(case, seed):
     lens = [o + n for o, n in zip(olds, news)]
     page = case["page"]
     pages = sum(-(-n // page) for n in lens)
-    s.update(_cache(case, gen, pages, 0, dev, kind != "append"))
+    s.update(_cache(case, gen, pages, dev, kind != "append"))
     s.update(table=_table(lens, page, s["k_pages"].shape[0], gen, dev), max_len=max(lens),
              lens=torch.tensor(lens, dtype=torch.int32, device=dev))
     if kind == "append":
@@ -228,21 +240,21 @@ def prepare(case, seed):
 # the plain form
 # ---------------------------------------------------------------------------
 
-def _values(words, scale):
-    """int32 words [..., n] in dimension order, scales [..., G] -> fp32 values [..., 8 n]."""
-    shift = torch.tensor([4 * AWQ.index(j) for j in range(8)], dtype=torch.int32, device=words.device)
-    q = (words[..., None] >> shift) & 15
-    q = (q - ((q & 8) << 1)).flatten(-2).float()
-    return (q.unflatten(-1, (scale.shape[-1], -1)) * scale.float()[..., None]).flatten(-2)
-
-
 def _unpaged(s):
     """The pages as fp32 values [P, NKV, page, hd]."""
     P, NKV, page, half = s["k_pages"].shape
-    back = torch.tensor(_kv_order(2 * half), device=s["k_pages"].device).argsort()
-    kw = s["k_pages"].view(torch.int32)[..., back]
-    vw = s["v_pages"].view(torch.int32).view(P, NKV, page // 4, half // 4, 4).transpose(3, 4).flatten(2, 3)
-    return _values(kw, s["k_scale"].transpose(2, 3)), _values(vw, s["v_scale"].transpose(2, 3))
+    hd, dev = 2 * half, s["k_pages"].device
+    back = torch.tensor(_kv_order(hd), device=dev).argsort()
+    kq = s["k_pages"].view(torch.int32)[..., back, None] >> torch.tensor([4 * AWQ.index(j) for j in range(8)], device=dev)
+    vq = s["v_pages"].view(torch.int16).view(P, NKV, page // 4, 16, hd // 64, 4).permute(0, 1, 2, 5, 4, 3)
+    vq = vq[..., None, :].to(torch.int32) >> torch.tensor([0, 4, 8, 12], device=dev)[:, None]
+
+    def values(q, scale):
+        q = q.reshape(P, NKV, page, hd) & 15
+        q = (q - ((q & 8) << 1)).float()
+        return (q.unflatten(-1, (scale.shape[2], -1)) * scale.float().transpose(2, 3)[..., None]).flatten(-2)
+
+    return values(kq, s["k_scale"]), values(vq, s["v_scale"])
 
 
 def _token_slots(s):
@@ -399,15 +411,17 @@ def _exact_page_rows(s, b, first, last):
     octet, nibble = d // 8, torch.tensor([AWQ.index(j) for j in range(8)], device=dev)[d % 8]
     w = hd // 32
     k_byte = ((octet % 4) * w + octet // 4) * 4 + nibble // 2
-    v_byte = ((slot[:, None] // 4 * (hd // 8) + octet) * 4 + slot[:, None] % 4) * 4 + nibble // 2  # in the head's page
+    v_nibble = d // 16 % 4
+    v_unit = ((slot[:, None] // 4 * 16 + d % 16) * (hd // 64) + d // 64) * 4 + slot[:, None] % 4  # in the head's page
+    v_byte = 2 * v_unit + v_nibble // 2
 
-    def signed(byte):
+    def signed(byte, nibble):
         q = torch.where(nibble % 2 == 1, byte >> 4, byte & 15).double()
         return torch.where(q >= 8, q - 16, q)
 
-    k = signed(s["k_pages"][pg, :, slot][..., k_byte])
+    k = signed(s["k_pages"][pg, :, slot][..., k_byte], nibble)
     head = torch.arange(s["k_pages"].shape[1], device=dev)
-    v = signed(s["v_pages"].flatten(2)[pg[:, None, None], head[:, None], v_byte[:, None]])
+    v = signed(s["v_pages"].flatten(2)[pg[:, None, None], head[:, None], v_byte[:, None]], v_nibble)
     G = s["k_scale"].shape[2]
     spread = d // (hd // G)
     return k * s["k_scale"][pg, :, :, slot].double()[..., spread], v * s["v_scale"][pg, :, :, slot].double()[..., spread]
