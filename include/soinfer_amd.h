@@ -734,6 +734,79 @@ int64_t soi_sparse_accumulate_counter_words(int64_t H);
 /* Row chunks of the sparse accumulate's partition of k rows of H columns. */
 int64_t soi_sparse_accumulate_row_chunks(int64_t H, int64_t k);
 
+/* --------------------------------------------------------------------------
+ * Several sequences at once: a paged KV cache held in 4 bits, and the
+ * attention around it. No reference counterpart as one call: the reference
+ * serves one sequence from a contiguous binary16 cache (qk_norm, apply_rope,
+ * kv_cache_append, decode_attention, python/soinfer/ops.py:222-260).
+ *
+ * Packed tokens: sequence b's rows are cu_seqlens[b] .. cu_seqlens[b+1] - 1
+ * (int32 [batch + 1], ascending from 0) of T; rows behind the last sequence
+ * are left as they are. The last of a sequence's n rows is position
+ * seq_lens[b] - 1, so its first is seq_lens[b] - n: seq_lens counts the rows
+ * of an append. A decode step is n = 1.
+ *
+ * Cache: position t of sequence b is slot t % page_size of page
+ * block_table[b * max_blocks + t / page_size]. Values are symmetric INT4,
+ * one binary16 scale per (token, KV head, group of group_size dimensions):
+ * s = fp16(max|x| / 7), q = clamp(round_half_even(x / s), -7, 7), value q s;
+ * a group with an infinity or NaN reads back as NaN.
+ *   k_pages uint8 [num_pages, num_kv_heads, page_size, head_dim / 2]: a
+ *     token's head_dim / 8 little-endian 32-bit words; word w g + i
+ *     (w = head_dim / 32, g < 4, i < w) holds dimensions 8 (4 i + g) .. + 7 in
+ *     AWQ nibble order.
+ *   v_pages uint8, same shape: 16-bit units [page_size / 4][16][head_dim / 64]
+ *     [4 tokens]; nibble n of unit (m, u) is dimension 64 u + 16 n + m.
+ *   k_scale, v_scale binary16 [num_pages, num_kv_heads,
+ *     head_dim / group_size, page_size].
+ * head_dim 64, 128 or 256; group_size 32, 64 or 128, at most head_dim;
+ * page_size a power of two from 16 up; pages and scales 16-byte aligned.
+ * Positions outside [0, max_blocks * page_size) and table entries outside
+ * [0, num_pages) name no page: nothing is written there, they read as zeros
+ * and the attention leaves their tokens out. Sequences may share pages that
+ * are only read; an append needs its slots to itself.
+ * ------------------------------------------------------------------------ */
+typedef struct soi_kv4_cache {
+    uint8_t* k_pages;
+    uint16_t* k_scale;
+    uint8_t* v_pages;
+    uint16_t* v_scale;
+    const int32_t* block_table; /* [batch, max_blocks] */
+    const int32_t* seq_lens;    /* [batch] */
+    int64_t batch, max_blocks, num_pages, num_kv_heads, page_size, head_dim, group_size;
+} soi_kv4_cache;
+
+/* qkv [T, (NQ + 2 NKV) * head_dim] (rows qkv_stride elements apart) -> per-head RMSNorm of q and k (both weights, or
+ * none for no norm), RoPE from tables [table_rows, head_dim / 2], each rounded to binary32 and then binary16; q to q_out
+ * [T, NQ, head_dim], k also to k_out [T, NKV, head_dim] if given, k and v quantized into the cache. Norm and rotation
+ * are evaluated in binary64, so the codes follow from the inputs alone. A position past the tables or the cache
+ * appends nothing and rotates by the last table row. */
+int soi_kv4_append(const soi_kv4_cache* cache, const uint16_t* qkv, int64_t qkv_stride, const uint16_t* q_norm,
+                   const uint16_t* k_norm, const float* cos_table, const float* sin_table, int64_t table_rows,
+                   const int32_t* cu_seqlens, int64_t T, int64_t num_q_heads, uint16_t* q_out, uint16_t* k_out, float eps,
+                   void* stream);
+/* k_out, v_out [T, NKV, head_dim]: the cached rows of packed tokens, each value q s rounded once to binary16. */
+int soi_kv4_read(const soi_kv4_cache* cache, const int32_t* cu_seqlens, int64_t T, uint16_t* k_out, uint16_t* v_out,
+                 void* stream);
+/* out [batch, NQ, head_dim]: attention of one query token per sequence (q rows q_stride elements apart) over its
+ * min(seq_lens[b], max_len) cached tokens; query head h reads KV head h / (NQ / NKV); zeros for an empty context; scale positive. The
+ * workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
+ * stream; calls that overlap need one each. */
+size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t max_len);
+int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,
+                             int64_t max_len, uint16_t* out, float scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
+/* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
+ * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
+ * one that sees none gives zeros. head_dim a multiple of 8 up to 256; k, v 16-byte aligned with strides of whole 16
+ * bytes, out 8-byte; scale positive. */
+int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
+                         int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
+                         int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t Tq,
+                         int64_t Tk, int64_t max_q, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                         uint16_t* out, int64_t out_token_stride, int64_t out_head_stride, float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1918,6 +1918,204 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> dip_gate_select(torch::T
     return {gate, idx.narrow(0, 0, k), ws.buf};
 }
 
+// ---------------------------------------------------------------------------
+// several sequences at once: the paged 4-bit KV cache, and packed prompts
+// ---------------------------------------------------------------------------
+
+namespace {
+
+using OptTensor = c10::optional<torch::Tensor>;
+
+// [first, last) bytes of a tensor with non-negative strides
+std::pair<uintptr_t, uintptr_t> span_of(const torch::Tensor& t) {
+    const auto p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    int64_t n = t.numel() ? 1 : 0;
+    for (int64_t d = 0; n && d < t.dim(); ++d) n += (t.size(d) - 1) * t.stride(d);
+    return {p, p + n * t.element_size()};
+}
+
+void no_overlap(const torch::Tensor& out, const torch::Tensor& in, const char* name, const char* what) {
+    const auto a = span_of(out), b = span_of(in);
+    TORCH_CHECK(a.first >= b.second || b.first >= a.second, name, ": ", what, " must not overlap");
+}
+
+soi_kv4_cache kv4_cache_of(const torch::Tensor& k_pages, const torch::Tensor& k_scale, const torch::Tensor& v_pages,
+                           const torch::Tensor& v_scale, const torch::Tensor& block_table, const torch::Tensor& seq_lens,
+                           const torch::Tensor& dev, const char* n) {
+    need(k_pages, torch::kUInt8, dev, n, "k_pages");
+    need(k_scale, torch::kFloat16, dev, n, "k_scale");
+    need(v_pages, torch::kUInt8, dev, n, "v_pages");
+    need(v_scale, torch::kFloat16, dev, n, "v_scale");
+    need(block_table, torch::kInt32, dev, n, "block_table");
+    need(seq_lens, torch::kInt32, dev, n, "seq_lens");
+    TORCH_CHECK(k_pages.dim() == 4 && v_pages.sizes() == k_pages.sizes(), n,
+                ": pages must be 4D [num_pages, num_kv_heads, page_size, head_dim / 2] of one shape");
+    TORCH_CHECK(k_scale.dim() == 4 && v_scale.sizes() == k_scale.sizes() && k_scale.size(0) == k_pages.size(0) &&
+                    k_scale.size(1) == k_pages.size(1) && k_scale.size(3) == k_pages.size(2),
+                n, ": scales must be 4D [num_pages, num_kv_heads, head_dim / group_size, page_size] of one shape");
+    const int64_t hd = 2 * k_pages.size(3), G = k_scale.size(2);
+    TORCH_CHECK(G >= 1 && hd % G == 0, n, ": scale groups must divide head_dim");
+    TORCH_CHECK(block_table.dim() == 2 && seq_lens.dim() == 1 && block_table.size(0) == seq_lens.size(0), n,
+                ": block_table must be 2D [batch, max_blocks] and seq_lens 1D [batch]");
+    soi_kv4_cache c;
+    c.k_pages = k_pages.data_ptr<uint8_t>();
+    c.k_scale = reinterpret_cast<uint16_t*>(k_scale.data_ptr<at::Half>());
+    c.v_pages = v_pages.data_ptr<uint8_t>();
+    c.v_scale = reinterpret_cast<uint16_t*>(v_scale.data_ptr<at::Half>());
+    c.block_table = block_table.data_ptr<int32_t>();
+    c.seq_lens = seq_lens.data_ptr<int32_t>();
+    c.batch = block_table.size(0);
+    c.max_blocks = block_table.size(1);
+    c.num_pages = k_pages.size(0);
+    c.num_kv_heads = k_pages.size(1);
+    c.page_size = k_pages.size(2);
+    c.head_dim = hd;
+    c.group_size = hd / G;
+    return c;
+}
+
+torch::Tensor out_or_empty(const OptTensor& given, c10::IntArrayRef sizes, const torch::Tensor& like, const char* n,
+                           const char* arg) {
+    if (!given) return torch::empty(sizes, like.options().dtype(torch::kFloat16));
+    need(*given, torch::kFloat16, like, n, arg);
+    TORCH_CHECK(given->sizes() == sizes, n, "(", arg, "): must have shape ", sizes, ", got ", given->sizes());
+    return *given;
+}
+
+void need_cu(const torch::Tensor& cu, int64_t B, const torch::Tensor& dev, const char* n, const char* arg) {
+    need(cu, torch::kInt32, dev, n, arg);
+    TORCH_CHECK(cu.dim() == 1 && cu.size(0) == B + 1, n, "(", arg, "): must be 1D [batch + 1]");
+}
+
+}  // namespace
+
+torch::Tensor kv4_append(torch::Tensor qkv, OptTensor q_norm, OptTensor k_norm, torch::Tensor cos_table,
+                         torch::Tensor sin_table, torch::Tensor k_pages, torch::Tensor k_scale, torch::Tensor v_pages,
+                         torch::Tensor v_scale, torch::Tensor block_table, torch::Tensor seq_lens, torch::Tensor cu_seqlens,
+                         int64_t num_q_heads, double eps, OptTensor k_out, OptTensor q_out) {
+    const char* n = "kv4_append";
+    TORCH_CHECK(qkv.is_cuda() && qkv.scalar_type() == torch::kFloat16 && qkv.dim() == 2 && qkv.stride(1) == 1, n,
+                "(qkv): must be a 2D float16 CUDA tensor with contiguous rows");
+    const soi_kv4_cache c = kv4_cache_of(k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, qkv, n);
+    const int64_t T = qkv.size(0), hd = c.head_dim;
+    TORCH_CHECK(num_q_heads >= 1 && qkv.size(1) == (num_q_heads + 2 * c.num_kv_heads) * hd, n,
+                "(qkv): rows must hold (num_q_heads + 2 * num_kv_heads) * head_dim values");
+    TORCH_CHECK(q_norm.has_value() == k_norm.has_value(), n, ": q_norm and k_norm come together");
+    if (q_norm) {
+        need(*q_norm, torch::kFloat16, qkv, n, "q_norm");
+        need(*k_norm, torch::kFloat16, qkv, n, "k_norm");
+        TORCH_CHECK(q_norm->numel() == hd && k_norm->numel() == hd, n, ": norm weights must be [head_dim]");
+    }
+    need(cos_table, torch::kFloat32, qkv, n, "cos_table");
+    need(sin_table, torch::kFloat32, qkv, n, "sin_table");
+    TORCH_CHECK(cos_table.dim() == 2 && cos_table.size(1) == hd / 2 && sin_table.sizes() == cos_table.sizes(), n,
+                ": RoPE tables must be [positions, head_dim / 2]");
+    need_cu(cu_seqlens, c.batch, qkv, n, "cu_seqlens");
+    const at::DeviceGuard guard(qkv.device());
+    torch::Tensor q = out_or_empty(q_out, {T, num_q_heads, hd}, qkv, n, "q_out");
+    if (q_out) no_overlap(q, qkv, n, "q_out and qkv");
+    if (k_out) {
+        out_or_empty(k_out, {T, c.num_kv_heads, hd}, qkv, n, "k_out");
+        no_overlap(*k_out, qkv, n, "k_out and qkv");
+        no_overlap(*k_out, q, n, "k_out and q_out");
+    }
+    check_status(soi_kv4_append(&c, h16(qkv), qkv.stride(0), q_norm ? h16(*q_norm) : nullptr,
+                                k_norm ? h16(*k_norm) : nullptr, cos_table.data_ptr<float>(),
+                                sin_table.data_ptr<float>(), cos_table.size(0), cu_seqlens.data_ptr<int32_t>(), T,
+                                num_q_heads, h16m(q), k_out ? h16m(*k_out) : nullptr, static_cast<float>(eps),
+                                cur_stream(qkv)),
+                 n);
+    return q;
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor k_pages, torch::Tensor k_scale, torch::Tensor v_pages,
+                                                  torch::Tensor v_scale, torch::Tensor block_table,
+                                                  torch::Tensor seq_lens, torch::Tensor cu_seqlens, int64_t num_tokens,
+                                                  OptTensor k_out, OptTensor v_out) {
+    const char* n = "kv4_read";
+    const soi_kv4_cache c = kv4_cache_of(k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, k_pages, n);
+    TORCH_CHECK(num_tokens >= 0, n, ": num_tokens must not be negative");
+    need_cu(cu_seqlens, c.batch, k_pages, n, "cu_seqlens");
+    const at::DeviceGuard guard(k_pages.device());
+    torch::Tensor k = out_or_empty(k_out, {num_tokens, c.num_kv_heads, c.head_dim}, k_pages, n, "k_out");
+    torch::Tensor v = out_or_empty(v_out, {num_tokens, c.num_kv_heads, c.head_dim}, k_pages, n, "v_out");
+    if (k_out && v_out) no_overlap(k, v, n, "k_out and v_out");
+    check_status(soi_kv4_read(&c, cu_seqlens.data_ptr<int32_t>(), num_tokens, h16m(k), h16m(v), cur_stream(k_pages)), n);
+    return {k, v};
+}
+
+int64_t kv4_decode_attention_workspace_bytes(int64_t B, int64_t NQ, int64_t NKV, int64_t head_dim, int64_t max_len) {
+    return static_cast<int64_t>(soi_kv4_decode_attention_workspace_bytes(B, NQ, NKV, head_dim, max_len));
+}
+
+torch::Tensor kv4_decode_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor k_scale, torch::Tensor v_pages,
+                                   torch::Tensor v_scale, torch::Tensor block_table, torch::Tensor seq_lens,
+                                   c10::optional<int64_t> max_len, c10::optional<double> scale, OptTensor out,
+                                   OptTensor workspace) {
+    const char* n = "kv4_decode_attention";
+    TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kFloat16 && q.dim() == 3, n,
+                "(q): must be a 3D [batch, num_q_heads, head_dim] float16 CUDA tensor");
+    const soi_kv4_cache c = kv4_cache_of(k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, q, n);
+    const int64_t B = q.size(0), NQ = q.size(1), hd = q.size(2);
+    TORCH_CHECK(B == c.batch && hd == c.head_dim, n, "(q): must be [batch, num_q_heads, head_dim] of the cache's batch and head_dim");
+    TORCH_CHECK(q.stride(2) == 1 && (NQ == 1 || q.stride(1) == hd), n, "(q): the heads of a token must be contiguous");
+    const int64_t cap = c.max_blocks * c.page_size, ml = max_len.value_or(cap);
+    TORCH_CHECK(ml >= 0 && ml <= cap, n, ": max_len must be in [0, ", cap, "], got ", ml);
+    const double sc = scale.value_or(1.0 / std::sqrt(static_cast<double>(hd)));
+    const at::DeviceGuard guard(q.device());
+    torch::Tensor o = out_or_empty(out, {B, NQ, hd}, q, n, "out");
+    if (out) no_overlap(o, q, n, "out and q");
+    if (B == 0) return o;
+    const int64_t bytes = kv4_decode_attention_workspace_bytes(B, NQ, c.num_kv_heads, hd, ml);
+    torch::Tensor ws;
+    if (workspace) {
+        need(*workspace, torch::kUInt8, q, n, "workspace");
+        ws = *workspace;
+    } else if (bytes > 0) {
+        ws = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+    }
+    check_status(soi_kv4_decode_attention(&c, h16(q), q.stride(0), NQ, ml, h16m(o), static_cast<float>(sc),
+                                          ws.defined() ? ws.data_ptr<uint8_t>() : nullptr,
+                                          ws.defined() ? ws.numel() : 0, cur_stream(q)),
+                 n);
+    return o;
+}
+
+torch::Tensor prompt_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
+                               int64_t max_q, c10::optional<double> scale, OptTensor out) {
+    const char* n = "prompt_attention";
+    for (const auto* t : {&q, &k, &v})
+        TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat16 && t->dim() == 3 && t->stride(2) == 1 &&
+                        t->device() == q.device(),
+                    n, ": q, k and v must be 3D [tokens, heads, head_dim] float16 tensors on one CUDA device, each head's "
+                    "dimensions contiguous");
+    const int64_t Tq = q.size(0), NQ = q.size(1), hd = q.size(2), Tk = k.size(0), NKV = k.size(1);
+    TORCH_CHECK(k.size(2) == hd && v.sizes() == k.sizes(), n, ": k and v must be [key tokens, num_kv_heads, head_dim]");
+    need(cu_q, torch::kInt32, q, n, "cu_q");
+    TORCH_CHECK(cu_q.dim() == 1 && cu_q.size(0) >= 1, n, "(cu_q): must be 1D [batch + 1]");
+    const int64_t B = cu_q.size(0) - 1;
+    need_cu(cu_k, B, q, n, "cu_k");
+    TORCH_CHECK(max_q >= 0, n, ": max_q must not be negative");
+    const double sc = scale.value_or(1.0 / std::sqrt(static_cast<double>(hd)));
+    const at::DeviceGuard guard(q.device());
+    torch::Tensor o = out ? *out : torch::empty({Tq, NQ, hd}, q.options());
+    if (out) {
+        TORCH_CHECK(o.device() == q.device() && o.scalar_type() == torch::kFloat16 && o.sizes() == q.sizes() &&
+                        o.stride(2) == 1,
+                    n, "(out): must be a float16 tensor of q's shape and device, each head's dimensions contiguous");
+        no_overlap(o, q, n, "out and q");
+        no_overlap(o, k, n, "out and k");
+        no_overlap(o, v, n, "out and v");
+    }
+    if (B == 0) return o;
+    check_status(soi_prompt_attention(h16(q), q.stride(0), q.stride(1), h16(k), k.stride(0), k.stride(1), h16(v),
+                                      v.stride(0), v.stride(1), cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), B, Tq,
+                                      Tk, max_q, NQ, NKV, hd, h16m(o), o.stride(0), o.stride(1), static_cast<float>(sc),
+                                      cur_stream(q)),
+                 n);
+    return o;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "soinfer MI355X (gfx950) quantized decode hot path";
     m.def("gemv_w8a16", &gemv_w8a16, "INT8 GEMV");
@@ -2053,4 +2251,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("gate_Wq"), py::arg("gate_scale"), py::arg("x"), py::arg("k"), py::arg("K"), py::arg("group_size"),
           py::arg("slot_of") = py::none(), py::arg("miss_count") = py::none());
     m.def("version", []() { return std::string(soi_version()); });
+    m.def("kv4_append", &kv4_append, "q/k norm, RoPE and append of packed tokens to a paged 4-bit KV cache", py::arg("qkv"),
+          py::arg("q_norm"), py::arg("k_norm"), py::arg("cos_table"), py::arg("sin_table"), py::arg("k_pages"),
+          py::arg("k_scale"), py::arg("v_pages"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"),
+          py::arg("cu_seqlens"), py::arg("num_q_heads"), py::arg("eps") = 1e-6, py::arg("k_out") = py::none(),
+          py::arg("q_out") = py::none());
+    m.def("kv4_read", &kv4_read, "cached K and V of packed tokens as binary16", py::arg("k_pages"), py::arg("k_scale"),
+          py::arg("v_pages"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"), py::arg("cu_seqlens"),
+          py::arg("num_tokens"), py::arg("k_out") = py::none(), py::arg("v_out") = py::none());
+    m.def("kv4_decode_attention_workspace_bytes", &kv4_decode_attention_workspace_bytes);
+    m.def("kv4_decode_attention", &kv4_decode_attention, "one query token per sequence over a paged 4-bit KV cache",
+          py::arg("q"), py::arg("k_pages"), py::arg("k_scale"), py::arg("v_pages"), py::arg("v_scale"),
+          py::arg("block_table"), py::arg("seq_lens"), py::arg("max_len") = py::none(), py::arg("scale") = py::none(),
+          py::arg("out") = py::none(), py::arg("workspace") = py::none());
+    m.def("prompt_attention", &prompt_attention, "causal attention of packed prompts", py::arg("q"), py::arg("k"),
+          py::arg("v"), py::arg("cu_q"), py::arg("cu_k"), py::arg("max_q"), py::arg("scale") = py::none(),
+          py::arg("out") = py::none());
 }

@@ -401,3 +401,56 @@ def kv_cache_append(k_cache: torch.Tensor, v_cache: torch.Tensor, k_new: torch.T
                     pos: int) -> None:
     """Write k_new / v_new [NKV, hd] into the caches [NKV, max_seq, hd] at position pos, in place."""
     _C.kv_cache_append(k_cache, v_cache, k_new, v_new, pos)
+
+
+# ---------------------------------------------------------------------------
+# several sequences at once: a paged KV cache in 4 bits, and packed prompts
+# ---------------------------------------------------------------------------
+
+def kv4_append(qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Tensor | None, cos_table: torch.Tensor,
+               sin_table: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor,
+               v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: torch.Tensor,
+               num_q_heads: int, eps: float = 1e-6, k_out: torch.Tensor | None = None,
+               q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """New tokens of several sequences into a paged 4-bit KV cache (soinfer.runtime.paged_kv.PagedKV4 keeps one).
+    qkv [T, (num_q_heads + 2 NKV) * hd] fp16: sequence b's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32
+    [B + 1]), the last of them at position seq_lens[b] - 1 (int32 [B], the new tokens included). Per head: RMSNorm of q
+    and k by q_norm / k_norm [hd] (None, None: no norm), RoPE by the fp32 tables [positions, hd / 2]; k and v are
+    quantized (symmetric INT4, one fp16 scale per group) into the pages block_table [B, max_blocks] names. Returns the
+    rotated q [T, num_q_heads, hd] (q_out if given); the rotated k also goes to k_out [T, NKV, hd] if given. Rows behind
+    the last sequence are left as they are; a position without a page, or past the tables, is not appended."""
+    return _C.kv4_append(qkv, q_norm, k_norm, cos_table, sin_table, k_pages, k_scale, v_pages, v_scale, block_table,
+                         seq_lens, cu_seqlens, num_q_heads, eps, k_out, q_out)
+
+
+def kv4_read(k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor, v_scale: torch.Tensor,
+             block_table: torch.Tensor, seq_lens: torch.Tensor, cu_seqlens: torch.Tensor, num_tokens: int,
+             k_out: torch.Tensor | None = None,
+             v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached K and V of packed tokens, fp16 [num_tokens, NKV, hd] each: rows cu_seqlens[b] .. cu_seqlens[b + 1] - 1
+    are the last positions before seq_lens[b] (all of them where the row count is seq_lens[b]). Positions without a page
+    read as zeros. What prompt_attention takes for prompts that continue a cached context."""
+    return _C.kv4_read(k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, cu_seqlens, num_tokens, k_out, v_out)
+
+
+def kv4_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor,
+                         v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         max_len: int | None = None, scale: float | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """out [B, NQ, hd]: attention of one query token per sequence, q [B, NQ, hd] fp16 (rotated), over its seq_lens[b]
+    cached tokens (at most max_len, which sets the split of long contexts: pass the longest length the host knows;
+    default: all the block table holds). Query head h reads KV head h // (NQ // NKV); scale 1/sqrt(hd) by default; an
+    empty context gives zeros. workspace (uint8, _C.kv4_decode_attention_workspace_bytes) and out are allocated unless
+    given; a workspace needs no initial value, and calls that overlap need one each."""
+    return _C.kv4_decode_attention(q, k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, max_len, scale, out,
+                                   workspace)
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                     max_q: int, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts on the matrix cores: q [Tq, NQ, hd], k and v [Tk, NKV, hd] fp16 (any token and
+    head strides with contiguous dimensions: views of a fused projection work), hd a multiple of 8 up to 256. Sequence
+    b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 (at most max_q), its keys rows cu_k[b] .. cu_k[b + 1] - 1; query i of
+    nq sees keys j <= i + nk - nq, so more keys than queries continue a context. A query without a key gives zeros; rows
+    behind the last sequence are left as they are. k and v start on 16 bytes, their strides are multiples of 8."""
+    return _C.prompt_attention(q, k, v, cu_q, cu_k, max_q, scale, out)

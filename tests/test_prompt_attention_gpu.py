@@ -1,0 +1,139 @@
+"""Causal attention of packed prompts (ops.prompt_attention) against the formula in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import kv4_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def problem(dev, nq, nk, NQ, NKV, hd, seed, scale=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    mk = lambda n, h: (torch.randn((n, h, hd), generator=g, device=dev) * scale).half()  # noqa: E731
+    cu = [torch.from_numpy(R.offsets(x)).to(dev) for x in (nq, nk)]
+    return mk(sum(nq), NQ), mk(sum(nk), NKV), mk(sum(nk), NKV), *cu
+
+
+def check(got, q, k, v, nq, nk, label, scale=None):
+    q0 = k0 = 0
+    scale = scale or 1 / math.sqrt(q.shape[2])
+    for i, (a, b) in enumerate(zip(nq, nk)):
+        last = torch.arange(a, device=q.device) + b - a
+        ref, bound = R.attention(q[q0:q0 + a].double(), k[k0:k0 + b].double(), v[k0:k0 + b].double(), last, scale)
+        R.assert_within(got[q0:q0 + a], ref, bound, f"{label} sequence {i}")
+        q0, k0 = q0 + a, k0 + b
+
+
+@pytest.mark.parametrize("hd", [8, 40, 64, 72, 128, 136, 256])
+@pytest.mark.parametrize("NQ,NKV", [(4, 4), (6, 2), (8, 1)])
+def test_head_layouts(cuda, hd, NQ, NKV):
+    import soinfer.ops as ops
+
+    n = [1, 31, 32, 33, 63, 64, 65, 129, 200]
+    q, k, v, cu, _ = problem(cuda, n, n, NQ, NKV, hd, hd + NQ)
+    check(ops.prompt_attention(q, k, v, cu, cu, max(n)), q, k, v, n, n, f"hd {hd}")
+
+
+@pytest.mark.parametrize("nq,nk", [([1], [1]), ([1], [700]), ([5, 0, 3], [5, 4, 900]), ([127, 128, 257], [300, 128, 1000]),
+                                   ([600], [601]), ([0, 2], [0, 2]), ([2000], [2000])])
+def test_lengths(cuda, nq, nk):
+    import soinfer.ops as ops
+
+    q, k, v, cu_q, cu_k = problem(cuda, nq, nk, 4, 2, 128, 5, 1.5)
+    check(ops.prompt_attention(q, k, v, cu_q, cu_k, max(nq)), q, k, v, nq, nk, f"{nq} {nk}")
+
+
+def test_queries_without_keys_give_zeros(cuda):
+    import soinfer.ops as ops
+
+    nq, nk = [40, 70, 3], [10, 0, 3]
+    q, k, v, cu_q, cu_k = problem(cuda, nq, nk, 4, 2, 64, 6)
+    got = ops.prompt_attention(q, k, v, cu_q, cu_k, 70)
+    check(got, q, k, v, nq, nk, "short keys")
+    assert (got[:30] == 0).all() and (got[40:110] == 0).all()
+
+
+def test_strided_views_and_output(cuda):
+    """q, k, v as views of one fused projection, the output into every other head of a wider tensor."""
+    import soinfer.ops as ops
+
+    NQ, NKV, hd, n = 6, 2, 64, [50, 77]
+    g = torch.Generator(device=cuda).manual_seed(7)
+    rows = torch.randn((sum(n), NQ + 2 * NKV, hd), generator=g, device=cuda).half()
+    q, k, v = rows.split([NQ, NKV, NKV], 1)
+    cu = torch.from_numpy(R.offsets(n)).to(cuda)
+    out = torch.full((sum(n), 2 * NQ, hd), 7.0, dtype=torch.float16, device=cuda)
+    got = ops.prompt_attention(q, k, v, cu, cu, 77, out=out[:, ::2])
+    assert got.data_ptr() == out.data_ptr()
+    check(out[:, ::2], q, k, v, n, n, "views")
+    assert (out[:, 1::2] == 7).all()
+
+
+def test_rows_behind_the_last_sequence_stay(cuda):
+    import soinfer.ops as ops
+
+    n = [33, 20]
+    q, k, v, cu, _ = problem(cuda, [33, 20, 90], [33, 20, 90], 4, 2, 128, 8)
+    cu = cu[:3].contiguous()
+    out = torch.full_like(q, 3.0)
+    ops.prompt_attention(q, k, v, cu, cu, 33, out=out)
+    check(out, q, k, v, n, n, "padded")
+    assert (out[53:] == 3).all()
+
+
+def test_large_scores_and_scale(cuda):
+    import soinfer.ops as ops
+
+    n = [150]
+    q, k, v, cu, _ = problem(cuda, n, n, 2, 1, 128, 9, 12.0)
+    check(ops.prompt_attention(q, k, v, cu, cu, 150), q, k, v, n, n, "large")
+    check(ops.prompt_attention(q, k, v, cu, cu, 150, scale=0.01), q, k, v, n, n, "scale", 0.01)
+
+
+def test_same_bits_again_and_in_a_graph(cuda):
+    import soinfer.ops as ops
+
+    n = [100, 300]
+    q, k, v, cu, _ = problem(cuda, n, n, 8, 2, 128, 10)
+    want = ops.prompt_attention(q, k, v, cu, cu, 300)
+    assert torch.equal(want, ops.prompt_attention(q, k, v, cu, cu, 300))
+    out = torch.empty_like(q)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.prompt_attention(q, k, v, cu, cu, 300, out=out)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.prompt_attention(q, k, v, cu, cu, 300, out=out)
+    for seed in range(3):
+        q.copy_(problem(cuda, n, n, 8, 2, 128, 20 + seed)[0])
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.prompt_attention(q, k, v, cu, cu, 300))
+
+
+def test_refusals(cuda):
+    import soinfer.ops as ops
+
+    n = [16]
+    q, k, v, cu, _ = problem(cuda, n, n, 4, 2, 64, 11)
+    bad = [
+        dict(q=q.float()), dict(q=q.cpu()), dict(q=q[0]), dict(k=k[:, :1]), dict(k=k.transpose(1, 2)), dict(cu_q=cu.long()),
+        dict(cu_k=cu[:1]), dict(max_q=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(out=q),
+        dict(out=torch.empty_like(q)[:8]), dict(out=torch.empty_like(q).float()), dict(v=v[:8]),
+    ]
+    for change in bad:
+        args = dict(q=q, k=k, v=v, cu_q=cu, cu_k=cu, max_q=16) | change
+        with pytest.raises(RuntimeError):
+            ops.prompt_attention(**args)
+    flat = torch.zeros(16 * 2 * 64 + 4, dtype=torch.float16, device=cuda)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        ops.prompt_attention(q, flat[4:].view(16, 2, 64), v, cu, cu, 16)
+    with pytest.raises(RuntimeError, match="multiple of 8"):
+        ops.prompt_attention(q[..., :60], k[..., :60], v[..., :60], cu, cu, 16)
+    with pytest.raises(RuntimeError, match="multiple of num_kv_heads"):
+        ops.prompt_attention(q[:, :3], k, v, cu, cu, 16)
