@@ -49,22 +49,39 @@ __device__ __forceinline__ int pa_swz_v(int row) {
     return HD == 64 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 3) : (row & 3) << 2 | ((row >> 2) & 3);
 }
 
+// A wave's 1 KB pieces of a tile into LDS: lane offsets `off` from `base`, zeros from `bytes` on. The load is written in
+// asm because the compiler, which cannot tell the two buffers apart, would let every LDS read wait for the loads in
+// flight (the kernel waits for them itself, at the barrier; no register is written). m0 holds the LDS address.
+template <int LOADS>
+__device__ __forceinline__ void pa_load(const uint16_t* base, int64_t bytes, const uint32_t (&off)[LOADS], uint32_t lds) {
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    const u32x4 r = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p))),
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32))) & 0xffffu,
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00027000u};
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + i * 1024),
+                     "v"(off[i]), "s"(r)
+                     : "memory", "m0");
+}
+
 template <int HD, int NW>
-__global__ __launch_bounds__(NW * kWave) void prompt_attention_kernel(const PaArgs a) {
+__global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attention_kernel(const PaArgs a) {
     constexpr int CPR = HD / 8, ROWB = HD * 2, TILEB = kPaKeys * ROWB;  // chunks and bytes of a row, bytes of a tile
     constexpr int KK = HD / 16, DT = HD / 32, NT = kPaKeys / 32, NJ = kPaKeys / 16;
     constexpr int LOADS = TILEB / 1024 / NW;  // 1 KB loads per wave and tile
     static_assert(TILEB % (1024 * NW) == 0, "whole loads per wave");
     __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][TILEB];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hh = lane >> 5;
     // heads of one KV head lie NKV apart in x: with NKV a multiple of 8 they run on one XCD and share its L2
     const int kvh = static_cast<int>(blockIdx.x) % a.NKV, rep = a.NQ / a.NKV;
     const int head = kvh * rep + static_cast<int>(blockIdx.x) / a.NKV;
     const int b = blockIdx.z;
     auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
-    const int q_lo = clamp(ldg(a.cu_q + b), 0, a.Tq), q_hi = clamp(ldg(a.cu_q + b + 1), q_lo, a.Tq);
-    const int k_lo = clamp(ldg(a.cu_k + b), 0, a.Tk), k_hi = clamp(ldg(a.cu_k + b + 1), k_lo, a.Tk);
+    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+    const int q_lo = clamp(uniform(ldg(a.cu_q + b)), 0, a.Tq), q_hi = clamp(uniform(ldg(a.cu_q + b + 1)), q_lo, a.Tq);
+    const int k_lo = clamp(uniform(ldg(a.cu_k + b)), 0, a.Tk), k_hi = clamp(uniform(ldg(a.cu_k + b + 1)), k_lo, a.Tk);
     const int nq = q_hi - q_lo, nk = k_hi - k_lo, off = nk - nq;
     const int qt = static_cast<int>(gridDim.y - 1 - blockIdx.y);  // the longest rows first
     const int q0 = qt * (32 * NW);
@@ -86,24 +103,25 @@ __global__ __launch_bounds__(NW * kWave) void prompt_attention_kernel(const PaAr
             qf[i] = __builtin_bit_cast(f16x8, ldg_any(d < a.hd ? static_cast<const void*>(qr + d) : g_zero16));
         }
     }
+    // Tile loads: the buffer descriptor starts at the tile's first key and ends with the sequence's last one, so rows past
+    // the end arrive as zeros, and so do the chunks between hd and HD (their offset is past any end). The lanes' offsets
+    // are the same for every tile.
+    uint32_t ko[LOADS], vof[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int id = (wave * LOADS + i) * 64 + lane, r = id / CPR, p = id % CPR;
+        const int ck = p ^ pa_swz_k<HD>(r), cv = p ^ pa_swz_v<HD>(r);
+        ko[i] = 8 * ck < a.hd ? static_cast<uint32_t>(r * a.k_ts + 8 * ck) * 2 : 0xfffffff0u;
+        vof[i] = 8 * cv < a.hd ? static_cast<uint32_t>(r * a.v_ts + 8 * cv) * 2 : 0xfffffff0u;
+    }
     const uint16_t* kb = a.k + k_lo * a.k_ts + kvh * a.k_hs;
     const uint16_t* vb = a.v + k_lo * a.v_ts + kvh * a.v_hs;
-
+    const uint32_t lds = __builtin_amdgcn_readfirstlane(
+        static_cast<int>(reinterpret_cast<uintptr_t>((lds_u8*)&s_kv[0][0][0])) + wave * LOADS * 1024);
     auto load = [&](int tile, int buf) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int id = (wave * LOADS + i) * 64 + lane, r = id / CPR, p = id % CPR;
-            const int key = min(tile * kPaKeys + r, nk - 1);  // rows past the end read the last one; they are masked
-            const int ck = p ^ pa_swz_k<HD>(r), cv = p ^ pa_swz_v<HD>(r);
-            const void* ks = 8 * ck < a.hd ? static_cast<const void*>(kb + key * a.k_ts + 8 * ck) : g_zero16;
-            const void* vs = 8 * cv < a.hd ? static_cast<const void*>(vb + key * a.v_ts + 8 * cv) : g_zero16;
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)ks,
-                (__attribute__((address_space(3))) void*)&s_kv[buf][0][(wave * LOADS + i) * 1024], 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)vs,
-                (__attribute__((address_space(3))) void*)&s_kv[buf][1][(wave * LOADS + i) * 1024], 16, 0, 0);
-        }
+        const int key = tile * kPaKeys, rows = min(nk - key, kPaKeys);
+        pa_load<LOADS>(kb + key * a.k_ts, ((rows - 1) * a.k_ts + a.hd) * 2, ko, lds + (2 * buf) * TILEB);
+        pa_load<LOADS>(vb + key * a.v_ts, ((rows - 1) * a.v_ts + a.hd) * 2, vof, lds + (2 * buf + 1) * TILEB);
     };
 
     f32x16 acc[DT];
@@ -120,7 +138,8 @@ __global__ __launch_bounds__(NW * kWave) void prompt_attention_kernel(const PaAr
     if (tiles > 0) load(0, 0);
     for (int t = 0; t < tiles; ++t) {
         // this wave's part of tile t has landed and its reads of tile t - 1 are done; after the barrier everyone's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const int buf = t & 1;
@@ -172,9 +191,13 @@ __global__ __launch_bounds__(NW * kWave) void prompt_attention_kernel(const PaAr
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 const float p = fast_exp2(fmaf(s[j >> 1][8 * (j & 1) + e], a.scale_log2, -m));
-                l += p;
                 pb[j][e] = static_cast<f16>(p);
             }
+        // the sum is that of the weights the products use: rounded p, added in binary32
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) l = dot2(f16x2{pb[j][e], pb[j][e + 1]}, f16x2{(f16)1.0f, (f16)1.0f}, l);
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -229,6 +252,9 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
     SOI_REQUIRE(scale > 0.0f && scale < __builtin_inff(), "%s: scale must be positive and finite", what);
     if (Tq == 0 || max_q == 0) return SOI_OK;
     SOI_REQUIRE(q && out && cu_q && cu_k && (Tk == 0 || (k && v)), "%s: null pointer", what);
+    SOI_REQUIRE(k_token_stride >= 0 && k_token_stride < (int64_t(1) << 24) && v_token_stride >= 0 &&
+                    v_token_stride < (int64_t(1) << 24),
+                "%s: key and value rows must be less than 2^24 elements apart", what);
     SOI_REQUIRE(aligned16(k) && aligned16(v) && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
                     v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
                 "%s: k and v must be 16-byte aligned with strides of whole 16 bytes", what);
