@@ -29,6 +29,9 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int kPaKeys = 64;  // keys per LDS tile
+// m is the base of the exponents, raised only where a score would pass it by more than this (in powers of two): weights
+// then reach 2^kPaSlack, well inside binary16, and most tiles of a row rescale nothing
+constexpr float kPaSlack = 8.0f;
 
 struct PaArgs {
     const uint16_t *q, *k, *v;
@@ -62,7 +65,7 @@ __device__ __forceinline__ void pa_load(const uint16_t* base, int64_t bytes, con
     for (int i = 0; i < LOADS; ++i)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + i * 1024),
                      "v"(off[i]), "s"(r)
-                     : "memory", "m0");
+                     : "memory");
 }
 
 template <int HD, int NW>
@@ -176,7 +179,7 @@ __global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attentio
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
         top = fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
-        if (ballot(top > m)) {
+        if (ballot(top > m + kPaSlack)) {
             const float mn = fmaxf(m, top), w = fast_exp2(m - mn);
             m = mn;
             l *= w;
