@@ -80,13 +80,13 @@ __global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attentio
     // heads of one KV head lie NKV apart in x: with NKV a multiple of 8 they run on one XCD and share its L2
     const int kvh = static_cast<int>(blockIdx.x) % a.NKV, rep = a.NQ / a.NKV;
     const int head = kvh * rep + static_cast<int>(blockIdx.x) / a.NKV;
-    const int b = blockIdx.z;
+    const int b = blockIdx.y;
     auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
     auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
     const int q_lo = clamp(uniform(ldg(a.cu_q + b)), 0, a.Tq), q_hi = clamp(uniform(ldg(a.cu_q + b + 1)), q_lo, a.Tq);
     const int k_lo = clamp(uniform(ldg(a.cu_k + b)), 0, a.Tk), k_hi = clamp(uniform(ldg(a.cu_k + b + 1)), k_lo, a.Tk);
     const int nq = q_hi - q_lo, nk = k_hi - k_lo, off = nk - nq;
-    const int qt = static_cast<int>(gridDim.y - 1 - blockIdx.y);  // the longest rows first
+    const int qt = static_cast<int>(gridDim.z - 1 - blockIdx.z);  // the longest rows of all sequences first
     const int q0 = qt * (32 * NW);
     if (q0 >= nq) return;
     const int wq0 = q0 + 32 * wave;
@@ -268,8 +268,8 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
                    static_cast<int>(Tk), static_cast<int>(num_q_heads), static_cast<int>(num_kv_heads),
                    static_cast<int>(head_dim), scale * kLog2e};
     constexpr int NW = 4;
-    const dim3 grid(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(ceil_div64(max_q, 32 * NW)),
-                    static_cast<unsigned>(batch));
+    const dim3 grid(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(batch),
+                    static_cast<unsigned>(ceil_div64(max_q, 32 * NW)));
 #define SOI_P(H) hipLaunchKernelGGL((prompt_attention_kernel<H, NW>), grid, dim3(NW * kWave), 0, as_stream(stream), a)
     if (head_dim <= 64) SOI_P(64);
     else if (head_dim <= 128) SOI_P(128);
