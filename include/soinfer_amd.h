@@ -799,13 +799,16 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
                              void* stream);
 /* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
  * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
- * one that sees none gives zeros. head_dim a multiple of 8 up to 256; k, v 16-byte aligned with strides of whole 16
- * bytes, out 8-byte; scale positive. */
+ * one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
+ * bytes, out 8-byte; scale positive. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
+ * aligned, needs no initial value and may be reused by the next call on the stream; calls that overlap need one each. */
+size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim);
 int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                          int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v, int64_t v_token_stride,
                          int64_t v_head_stride, const int32_t* cu_q, const int32_t* cu_k, int64_t batch, int64_t Tq,
                          int64_t Tk, int64_t max_q, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
-                         uint16_t* out, int64_t out_token_stride, int64_t out_head_stride, float scale, void* stream);
+                         uint16_t* out, int64_t out_token_stride, int64_t out_head_stride, float scale, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

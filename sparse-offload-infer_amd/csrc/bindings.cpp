@@ -2081,8 +2081,12 @@ torch::Tensor kv4_decode_attention(torch::Tensor q, torch::Tensor k_pages, torch
     return o;
 }
 
+int64_t prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t NQ, int64_t head_dim) {
+    return static_cast<int64_t>(soi_prompt_attention_workspace_bytes(Tq, Tk, NQ, head_dim));
+}
+
 torch::Tensor prompt_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor cu_q, torch::Tensor cu_k,
-                               int64_t max_q, c10::optional<double> scale, OptTensor out) {
+                               int64_t max_q, c10::optional<double> scale, OptTensor out, OptTensor workspace) {
     const char* n = "prompt_attention";
     for (const auto* t : {&q, &k, &v})
         TORCH_CHECK(t->is_cuda() && t->scalar_type() == torch::kFloat16 && t->dim() == 3 && t->stride(2) == 1 &&
@@ -2108,9 +2112,18 @@ torch::Tensor prompt_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v
         no_overlap(o, v, n, "out and v");
     }
     if (B == 0) return o;
+    const int64_t bytes = prompt_attention_workspace_bytes(Tq, Tk, NQ, hd);
+    torch::Tensor ws;
+    if (workspace) {
+        need(*workspace, torch::kUInt8, q, n, "workspace");
+        ws = *workspace;
+    } else if (bytes > 0) {
+        ws = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+    }
     check_status(soi_prompt_attention(h16(q), q.stride(0), q.stride(1), h16(k), k.stride(0), k.stride(1), h16(v),
                                       v.stride(0), v.stride(1), cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), B, Tq,
                                       Tk, max_q, NQ, NKV, hd, h16m(o), o.stride(0), o.stride(1), static_cast<float>(sc),
+                                      ws.defined() ? ws.data_ptr<uint8_t>() : nullptr, ws.defined() ? ws.numel() : 0,
                                       cur_stream(q)),
                  n);
     return o;
@@ -2266,5 +2279,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("out") = py::none(), py::arg("workspace") = py::none());
     m.def("prompt_attention", &prompt_attention, "causal attention of packed prompts", py::arg("q"), py::arg("k"),
           py::arg("v"), py::arg("cu_q"), py::arg("cu_k"), py::arg("max_q"), py::arg("scale") = py::none(),
-          py::arg("out") = py::none());
+          py::arg("out") = py::none(), py::arg("workspace") = py::none());
+    m.def("prompt_attention_workspace_bytes", &prompt_attention_workspace_bytes);
 }

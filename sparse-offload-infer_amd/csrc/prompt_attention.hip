@@ -21,16 +21,17 @@
 #include "soi_device.h"
 #include "soi_attn.h"
 
+#include <type_traits>
+
 namespace soi {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr int kPaKeys = 64;  // keys per LDS tile
-// m is the base of the exponents, raised only where a score would pass it by more than this (in powers of two): weights
-// then reach 2^kPaSlack, well inside binary16, and most tiles of a row rescale nothing
 constexpr float kPaSlack = 8.0f;
 
 struct PaArgs {
@@ -38,9 +39,34 @@ struct PaArgs {
     uint16_t* out;
     int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;  // token and head strides, in elements
     const int32_t *cu_q, *cu_k;
-    int Tq, Tk, NQ, NKV, hd;
+    float* part;  // split rows: acc [nsplit][Tq][NQ][hd], then (m, l) [nsplit][Tq][NQ][2]
+    int Tq, Tk, NQ, NKV, hd, nsplit;
     float scale_log2;
 };
+
+// The rows and keys of one workgroup: `rows` queries from q0 of sequence b.
+struct PaRows {
+    int q_lo, nq, k_lo, nk, off, q0, tiles;
+    __device__ __forceinline__ PaRows(const PaArgs& a, int b, int qtile, int rows, int keys_per_tile) {
+        auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
+        auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
+        q_lo = clamp(uniform(ldg(a.cu_q + b)), 0, a.Tq);
+        nq = clamp(uniform(ldg(a.cu_q + b + 1)), q_lo, a.Tq) - q_lo;
+        k_lo = clamp(uniform(ldg(a.cu_k + b)), 0, a.Tk);
+        nk = clamp(uniform(ldg(a.cu_k + b + 1)), k_lo, a.Tk) - k_lo;
+        off = nk - nq;
+        q0 = qtile * rows;
+        const int keys = clamp(min(q0 + rows, nq) + off, 0, nk);  // seen by the last query
+        tiles = (keys + keys_per_tile - 1) / keys_per_tile;
+    }
+};
+
+// Key tiles per split, for at most nsplit splits of at least kPaSplitTiles tiles.
+constexpr int kPaSplitTiles = 4;
+__device__ __forceinline__ int pa_split_tiles(int tiles, int nsplit) {
+    const int most = (tiles + kPaSplitTiles - 1) / kPaSplitTiles, ns = most < nsplit ? most : nsplit;
+    return ns <= 1 ? (tiles < 1 ? 1 : tiles) : (tiles + ns - 1) / ns;
+}
 
 // physical 16-byte chunk of logical chunk c: c ^ swizzle(row)
 template <int HD>
@@ -68,44 +94,35 @@ __device__ __forceinline__ void pa_load(const uint16_t* base, int64_t bytes, con
                      : "memory");
 }
 
-template <int HD, int NW>
-__global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attention_kernel(const PaArgs a) {
+// 16 bytes to any address
+__device__ __forceinline__ void stg_any(void* p, const u32x4& v) {
+    typedef __attribute__((address_space(1))) u32x4_any gT;
+    *(gT*)(p) = v;
+}
+
+template <int HD, int NW, int KT, int NBUF, int OCC>
+__global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const PaArgs a) {
+    constexpr int kPaKeys = KT;
     constexpr int CPR = HD / 8, ROWB = HD * 2, TILEB = kPaKeys * ROWB;  // chunks and bytes of a row, bytes of a tile
     constexpr int KK = HD / 16, DT = HD / 32, NT = kPaKeys / 32, NJ = kPaKeys / 16;
     constexpr int LOADS = TILEB / 1024 / NW;  // 1 KB loads per wave and tile
     static_assert(TILEB % (1024 * NW) == 0, "whole loads per wave");
-    __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][TILEB];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_kv[NBUF][2][TILEB];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int n = lane & 31, hh = lane >> 5;
     // heads of one KV head lie NKV apart in x: with NKV a multiple of 8 they run on one XCD and share its L2
-    const int kvh = static_cast<int>(blockIdx.x) % a.NKV, rep = a.NQ / a.NKV;
-    const int head = kvh * rep + static_cast<int>(blockIdx.x) / a.NKV;
-    const int b = blockIdx.y;
-    auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
-    auto uniform = [](int x) { return __builtin_amdgcn_readfirstlane(x); };
-    const int q_lo = clamp(uniform(ldg(a.cu_q + b)), 0, a.Tq), q_hi = clamp(uniform(ldg(a.cu_q + b + 1)), q_lo, a.Tq);
-    const int k_lo = clamp(uniform(ldg(a.cu_k + b)), 0, a.Tk), k_hi = clamp(uniform(ldg(a.cu_k + b + 1)), k_lo, a.Tk);
-    const int nq = q_hi - q_lo, nk = k_hi - k_lo, off = nk - nq;
-    const int qt = static_cast<int>(gridDim.z - 1 - blockIdx.z);  // the longest rows of all sequences first
-    const int q0 = qt * (32 * NW);
+    const int split = static_cast<int>(blockIdx.x) / a.NQ, hx = static_cast<int>(blockIdx.x) % a.NQ;
+    const int kvh = hx % a.NKV, rep = a.NQ / a.NKV;
+    const int head = kvh * rep + hx / a.NKV;
+    const PaRows w(a, blockIdx.y, static_cast<int>(gridDim.z - 1 - blockIdx.z), 32 * NW, KT);  // the longest rows first
+    const int q_lo = w.q_lo, nq = w.nq, k_lo = w.k_lo, nk = w.nk, off = w.off, q0 = w.q0;
     if (q0 >= nq) return;
+    auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
+    const int per = pa_split_tiles(w.tiles, a.nsplit), t0 = split * per, tiles = min(w.tiles, t0 + per);
+    if (split > 0 && t0 >= w.tiles) return;
     const int wq0 = q0 + 32 * wave;
-    // keys seen by the workgroup's and by the wave's last query
-    const int keys = clamp(min(q0 + 32 * NW, nq) + off, 0, nk);
-    const int wkeys = wq0 < nq ? clamp(min(wq0 + 32, nq) + off, 0, nk) : 0;
-    const int tiles = (keys + kPaKeys - 1) / kPaKeys;
-    const int row = wq0 + n;  // the lane's query
-    const int last = row + off;  // the last key it sees
+    const int last = wq0 + n + off;  // the last key that the lane's query sees
 
-    f16x8 qf[KK];
-    {
-        const uint16_t* qr = a.q + static_cast<int64_t>(q_lo + min(row, nq - 1)) * a.q_ts + head * a.q_hs;
-#pragma unroll
-        for (int i = 0; i < KK; ++i) {
-            const int d = 16 * i + 8 * hh;
-            qf[i] = __builtin_bit_cast(f16x8, ldg_any(d < a.hd ? static_cast<const void*>(qr + d) : g_zero16));
-        }
-    }
     // Tile loads: the buffer descriptor starts at the tile's first key and ends with the sequence's last one, so rows past
     // the end arrive as zeros, and so do the chunks between hd and HD (their offset is past any end). The lanes' offsets
     // are the same for every tile.
@@ -117,14 +134,24 @@ __global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attentio
         ko[i] = 8 * ck < a.hd ? static_cast<uint32_t>(r * a.k_ts + 8 * ck) * 2 : 0xfffffff0u;
         vof[i] = 8 * cv < a.hd ? static_cast<uint32_t>(r * a.v_ts + 8 * cv) * 2 : 0xfffffff0u;
     }
+    // the workgroup's queries, loaded like a tile into the buffers that no key tile needs yet
+    constexpr int QROWS = 32 * NW, QLOADS = QROWS * ROWB / 1024 / NW;
+    static_assert((NBUF - 1) * 2 * KT >= QROWS, "room for the queries");
+    uint32_t qo[QLOADS];
+#pragma unroll
+    for (int i = 0; i < QLOADS; ++i) {
+        const int id = (wave * QLOADS + i) * 64 + lane, r = id / CPR, c = (id % CPR) ^ pa_swz_k<HD>(r);
+        qo[i] = 8 * c < a.hd ? static_cast<uint32_t>(r * a.q_ts + 8 * c) * 2 : 0xfffffff0u;
+    }
     const uint16_t* kb = a.k + k_lo * a.k_ts + kvh * a.k_hs;
     const uint16_t* vb = a.v + k_lo * a.v_ts + kvh * a.v_hs;
-    const uint32_t lds = __builtin_amdgcn_readfirstlane(
-        static_cast<int>(reinterpret_cast<uintptr_t>((lds_u8*)&s_kv[0][0][0])) + wave * LOADS * 1024);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)&s_kv[0][0][0]));
+    const uint32_t lds = lds0 + wave * LOADS * 1024;
     auto load = [&](int tile, int buf) {
         const int key = tile * kPaKeys, rows = min(nk - key, kPaKeys);
-        pa_load<LOADS>(kb + key * a.k_ts, ((rows - 1) * a.k_ts + a.hd) * 2, ko, lds + (2 * buf) * TILEB);
-        pa_load<LOADS>(vb + key * a.v_ts, ((rows - 1) * a.v_ts + a.hd) * 2, vof, lds + (2 * buf + 1) * TILEB);
+        const int64_t kn = rows > 0 ? ((rows - 1) * a.k_ts + a.hd) * 2 : 0, vn = rows > 0 ? ((rows - 1) * a.v_ts + a.hd) * 2 : 0;
+        pa_load<LOADS>(kb + key * a.k_ts, kn, ko, lds + 2 * buf * TILEB);
+        pa_load<LOADS>(vb + key * a.v_ts, vn, vof, lds + (2 * buf + 1) * TILEB);
     };
 
     f32x16 acc[DT];
@@ -134,51 +161,38 @@ __global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attentio
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
     float m = kNegBig, l = 0.0f;
 
-    const int krow = n * ROWB, kx = hh ^ pa_swz_k<HD>(n);  // K operand: key n of a 32-key tile, chunk 2 kk + hh
-    const int vr = 4 * hh + ((lane & 15) >> 2);             // V operand: token vr (+ 8 s + 16 j)
-    const int vc = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), vo = 8 * (lane & 1);
+    // Operand addresses: the lane's part below with bits flipped for the chunk, the row and the buffer added. (They stay
+    // out of loop-invariant registers that way: one XOR a read is cheaper than the registers.)
+    // K: key n of 32, chunk 2 kk + hh
+    const uint32_t k_at = lds0 + n * ROWB + ((hh ^ pa_swz_k<HD>(n)) << 4);
+    // V: token vr + 8 x + 16 j, four dimensions of chunk 4 d + ...; 8 x flips bit 1 of the swizzle
+    const int vr = 4 * hh + ((lane & 15) >> 2);
+    const uint32_t v_at = lds0 + TILEB + vr * ROWB +
+                          (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ pa_swz_v<HD>(vr)) << 4) + 8 * (lane & 1);
 
-    if (tiles > 0) load(0, 0);
-    for (int t = 0; t < tiles; ++t) {
-        // this wave's part of tile t has landed and its reads of tile t - 1 are done; after the barrier everyone's
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const int buf = t & 1;
-        if (t + 1 < tiles) load(t + 1, buf ^ 1);
-        const int k0 = t * kPaKeys;
-        if (k0 >= wkeys) continue;  // wave-uniform: nothing of this tile is seen here
-        const lds_u8* kt = (const lds_u8*)&s_kv[buf][0][0];
-        const lds_u8* vt = (const lds_u8*)&s_kv[buf][1][0];
-
-        f32x16 s[NT];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[i][r] = 0.0f;
-#pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                const f16x8 ka = *(const __attribute__((address_space(3))) f16x8*)(kt + i * 32 * ROWB + krow +
-                                                                                   (((2 * kk) ^ kx) << 4));
-                s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[kk], s[i], 0, 0, 0);
-            }
-        }
-        if (k0 + kPaKeys - 1 > wq0 + off) {  // some query of the wave does not see some key of the tile
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = k0 + 32 * i + 8 * (r >> 2) + 4 * hh + (r & 3);
-                    s[i][r] = key <= last ? s[i][r] : -__builtin_inff();
-                }
-        }
-        float top = s[0][0];
+    // the tiles that all queries of the wave see in full
+    const int wtiles = (clamp(min(wq0 + 32, nq) + off, 0, nk) + kPaKeys - 1) / kPaKeys;
+    const int whole = wq0 + off + 1 < 0 ? 0 : (wq0 + off + 1) / kPaKeys;
+    auto mask = [&](f32x16 (&z)[NT], int tile) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[i][r]);
-        top = fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
+            for (int r = 0; r < 16; ++r) {
+                const int key = tile * kPaKeys + 32 * i + 8 * (r >> 2) + 4 * hh + (r & 3);
+                z[i][r] = key <= last ? z[i][r] : -__builtin_inff();
+            }
+    };
+    auto highest = [&](const f32x16 (&z)[NT]) {
+        float top = z[0][0];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, z[i][r]);
+        return fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
+    };
+    // m is the base of the exponents, raised only where a score would pass it by more than 2^kPaSlack: weights then reach
+    // 2^kPaSlack, well inside binary16, and most tiles of a long row rescale nothing
+    auto raise = [&](float top) {
         if (ballot(top > m + kPaSlack)) {
             const float mn = fmaxf(m, top), w = fast_exp2(m - mn);
             m = mn;
@@ -188,62 +202,183 @@ __global__ __launch_bounds__(NW * kWave, HD == 256 ? 1 : 2) void prompt_attentio
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= w;
         }
-        f16x8 pb[NJ];
+    };
+    // this wave's LDS reads are done, and its loads but for the last `flight`; after the barrier everyone's
+    auto meet = [](auto flight) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (flight & 15) | (flight >> 4) << 14);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    if (t0 < tiles) {  // (workgroup-uniform)
+        pa_load<QLOADS>(a.q + (q_lo + q0) * a.q_ts + head * a.q_hs, ((min(nq - q0, QROWS) - 1) * a.q_ts + a.hd) * 2, qo,
+                        lds0 + 2 * TILEB + wave * QLOADS * 1024);
+        load(t0, 0);
+        meet(std::integral_constant<int, 0>{});
+        f16x8 qf[KK];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+        for (int kk = 0; kk < KK; ++kk)
+            qf[kk] = *(const lds_f16x8*)((lds_u8*)((k_at + 2 * TILEB + 32 * wave * ROWB) ^ (kk << 5)));
+        meet(std::integral_constant<int, 0>{});
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float p = fast_exp2(fmaf(s[j >> 1][8 * (j & 1) + e], a.scale_log2, -m));
-                pb[j][e] = static_cast<f16>(p);
+        for (int i = 1; i < NBUF - 1; ++i) load(t0 + i, i);
+        int buf = 0, nbuf = NBUF - 1;
+        for (int t = t0; t < tiles; ++t) {
+            if (t > t0) meet(std::integral_constant<int, (NBUF - 2) * 2 * LOADS>{});
+            load(t + NBUF - 1, nbuf);
+            const int cur = buf;
+            buf = buf + 1 == NBUF ? 0 : buf + 1;
+            nbuf = nbuf + 1 == NBUF ? 0 : nbuf + 1;
+            if (t >= wtiles) continue;  // wave-uniform: nothing of this tile is seen here
+            f32x16 z[NT];
+            const uint32_t ka = k_at + cur * 2 * TILEB;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z[i][r] = 0.0f;
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk)
+                    z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const lds_f16x8*)((lds_u8*)(ka ^ (kk << 5)) + i * 32 * ROWB),
+                                                                  qf[kk], z[i], 0, 0, 0);
             }
-        // the sum is that of the weights the products use: rounded p, added in binary32
+            if (t >= whole) mask(z, t);
+            raise(highest(z));
+            f16x8 pb[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) l = dot2(f16x2{pb[j][e], pb[j][e + 1]}, f16x2{(f16)1.0f, (f16)1.0f}, l);
+                for (int e = 0; e < 8; ++e)
+                    pb[j][e] = static_cast<f16>(fast_exp2(fmaf(z[j >> 1][8 * (j & 1) + e], a.scale_log2, -m)));
+            // the sum is that of the weights the products use: rounded p, added in binary32
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
+            for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                s16x4 w[2];
+                for (int e = 0; e < 8; e += 2)
+                    l = dot2(f16x2{pb[j][e], pb[j][e + 1]}, f16x2{(f16)1.0f, (f16)1.0f}, l);
+            const uint32_t va = v_at + cur * 2 * TILEB;
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int r = vr + 8 * x;  // + 16 j, which leaves the swizzle alone
-                    w[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (__attribute__((address_space(3))) s16x4*)(vt + (16 * j + r) * ROWB +
-                                                                   (((4 * d + vc) ^ pa_swz_v<HD>(r)) << 4) + vo));
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    s16x4 w[2];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x)
+                        w[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4*)((lds_u8*)(va ^ (d << 6 | x << 5)) + (16 * j + 8 * x) * ROWB));
+                    const f16x8 v8 = __builtin_bit_cast(
+                        f16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pb[j], acc[d], 0, 0, 0);
                 }
-                const f16x8 va = __builtin_bit_cast(
-                    f16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[j], acc[d], 0, 0, 0);
-            }
+        }
     }
     l += xor_lanes<32>(l);
+    if (w.tiles > per) {  // a split row: its state as it is, 64 dimensions at a time through LDS
+        lds_u8* so = (lds_u8*)(lds0 + wave * 32 * 256);
+        float* pb = a.part + (static_cast<int64_t>(split) * a.Tq + q_lo + wq0) * a.NQ * a.hd + head * a.hd;
+#pragma unroll
+        for (int d = 0; d < DT; d += 2) {
+            meet(std::integral_constant<int, 0>{});
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const f32x16& v = acc[d + (x >> 2)];
+                const int r = 4 * (x & 3);
+                *(__attribute__((address_space(3))) f32x4*)(so + n * 256 + (((2 * x + hh) ^ (n & 15)) << 4)) =
+                    f32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 4), c = lane & 15;
+                const f32x4 o = *(const __attribute__((address_space(3))) f32x4*)(so + r * 256 + ((c ^ (r & 15)) << 4));
+                if (wq0 + r < nq && 32 * d + 4 * c < a.hd)
+                    stg(reinterpret_cast<f32x4*>(pb + static_cast<int64_t>(r) * a.NQ * a.hd + 32 * d + 4 * c), o);
+            }
+        }
+        if (hh == 0 && wq0 + n < nq) {
+            float* ml = a.part + static_cast<int64_t>(a.nsplit) * a.Tq * a.NQ * a.hd +
+                        2 * ((static_cast<int64_t>(split) * a.Tq + q_lo + wq0 + n) * a.NQ + head);
+            stg(reinterpret_cast<f32x2*>(ml), f32x2{m, l});
+        }
+        return;
+    }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    if (row >= nq) return;
-    uint16_t* orow = a.out + static_cast<int64_t>(q_lo + row) * a.o_ts + head * a.o_hs;
+    // out rows leave through LDS, so that a store covers whole rows: 8 bytes of 32 rows at a time otherwise
+    meet(std::integral_constant<int, 0>{});
+    lds_u8* so = (lds_u8*)(lds0 + wave * 32 * ROWB);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int dim = 32 * d + 8 * x + 4 * hh;
-            if (dim >= a.hd) continue;
-            const u32x2 o = {pack_f16x2(acc[d][4 * x] * inv, acc[d][4 * x + 1] * inv),
-                             pack_f16x2(acc[d][4 * x + 2] * inv, acc[d][4 * x + 3] * inv)};
-            stg(reinterpret_cast<u32x2*>(orow + dim), o);
-        }
+        for (int x = 0; x < 4; ++x)
+            *(__attribute__((address_space(3))) u32x2*)(so + n * ROWB + (((4 * d + x) ^ pa_swz_k<HD>(n)) << 4) + 8 * hh) =
+                u32x2{pack_f16x2(acc[d][4 * x] * inv, acc[d][4 * x + 1] * inv),
+                      pack_f16x2(acc[d][4 * x + 2] * inv, acc[d][4 * x + 3] * inv)};
+    uint16_t* ob = a.out + head * a.o_hs;
+#pragma unroll
+    for (int i = 0; i < 32 * ROWB / 1024; ++i) {
+        const int id = i * 64 + lane, r = id / CPR, c = id % CPR;  // (a wave's LDS writes and reads are in order)
+        const u32x4 o = *(const __attribute__((address_space(3))) u32x4*)(so + r * ROWB + ((c ^ pa_swz_k<HD>(r)) << 4));
+        if (wq0 + r < nq && 8 * c < a.hd) stg_any(ob + (q_lo + wq0 + r) * a.o_ts + 8 * c, o);
+    }
 }
+
+// The split rows' states, in split order: four dimensions of one query and head a thread, kPaCombineRows queries of one
+// attention workgroup's `rows` a workgroup (many small workgroups: a thread's loads are two round trips, whatever they move).
+constexpr int kPaCombineRows = 8;
+__global__ __launch_bounds__(256) void prompt_combine_kernel(const PaArgs a, int rows, int keys_per_tile) {
+    const int head = blockIdx.x, r0 = static_cast<int>(blockIdx.z) * kPaCombineRows;
+    const PaRows w(a, blockIdx.y, r0 / rows, rows, keys_per_tile);
+    const int per = pa_split_tiles(w.tiles, a.nsplit);
+    if (r0 >= w.nq || w.tiles <= per) return;  // written by its one split
+    const int ns = (w.tiles + per - 1) / per, quads = a.hd >> 2;
+    const int64_t stride = static_cast<int64_t>(a.Tq) * a.NQ;
+    const float* ml = a.part + a.nsplit * stride * a.hd;
+    const int n = min(kPaCombineRows, w.nq - r0) * quads;
+    for (int i = threadIdx.x; i < n; i += 256) {
+        const int r = r0 + i / quads, d = 4 * (i % quads);
+        const int64_t at = static_cast<int64_t>(w.q_lo + r) * a.NQ + head;
+        float M = kNegBig, lsum = 0.0f;
+        f32x4 v = {0, 0, 0, 0};
+        for (int s = 0; s < ns; ++s) M = fmaxf(M, ldg(ml + 2 * (s * stride + at)));
+        for (int s = 0; s < ns; ++s) {
+            const float e = fast_exp2(ldg(ml + 2 * (s * stride + at)) - M);
+            lsum = fmaf(ldg(ml + 2 * (s * stride + at) + 1), e, lsum);
+            v += ldg(reinterpret_cast<const f32x4*>(a.part + (s * stride + at) * a.hd + d)) * e;
+        }
+        const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
+        const u32x2 o = {pack_f16x2(v.x * inv, v.y * inv), pack_f16x2(v.z * inv, v.w * inv)};
+        stg(reinterpret_cast<u32x2*>(a.out + (w.q_lo + r) * a.o_ts + head * a.o_hs + d), o);
+    }
+}
+
+constexpr int kPaWaves = 4;
+
+// Splits of a row's keys: where the queries alone make fewer workgroups than two to a CU, enough for that. (Every split
+// writes and reads hd + 2 floats a query.)
+static int64_t pa_nsplit(int64_t Tq, int64_t Tk, int64_t NQ, int64_t KT) {
+    const int64_t groups = NQ * ceil_div64(Tq, 32 * kPaWaves), most = ceil_div64(ceil_div64(Tk, KT), kPaSplitTiles);
+    int64_t n = 512 / groups;
+    n = n < most ? n : most;
+    return n < 1 ? 1 : n > 64 ? 64 : n;
+}
+
+static int64_t pa_keys(int64_t hd) { return hd > 64 && hd <= 128 ? 32 : 64; }
 
 }  // namespace soi
 
 using namespace soi;
+
+extern "C" size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim) {
+    if (Tq < 1 || Tk < 1 || num_q_heads < 1 || head_dim < 1 || head_dim > 256) return 0;
+    const int64_t n = pa_nsplit(Tq, Tk, num_q_heads, pa_keys(head_dim));
+    return n == 1 ? 0 : static_cast<size_t>(n) * Tq * num_q_heads * (head_dim + 2) * sizeof(float);
+}
 
 extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,
                                     int64_t k_token_stride, int64_t k_head_stride, const uint16_t* v,
                                     int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_q,
                                     const int32_t* cu_k, int64_t batch, int64_t Tq, int64_t Tk, int64_t max_q,
                                     int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, uint16_t* out,
-                                    int64_t out_token_stride, int64_t out_head_stride, float scale, void* stream) {
+                                    int64_t out_token_stride, int64_t out_head_stride, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
     const char* what = "soi_prompt_attention";
     SOI_REQUIRE(head_dim >= 8 && head_dim % 8 == 0 && head_dim <= 256, "%s: head_dim must be a multiple of 8 up to 256, got %lld",
                 what, (long long)head_dim);
@@ -251,29 +386,45 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
                 "%s: num_q_heads must be a multiple of num_kv_heads", what);
     SOI_REQUIRE(batch >= 1 && batch <= 65535, "%s: the number of sequences must be in [1, 65535]", what);
     SOI_REQUIRE(Tq >= 0 && Tk >= 0 && Tq < (int64_t(1) << 30) && Tk < (int64_t(1) << 30), "%s: token counts out of range", what);
-    SOI_REQUIRE(max_q >= 0 && max_q <= 8 * 65535, "%s: max_q must be in [0, 524280]", what);
+    SOI_REQUIRE(max_q >= 0 && max_q <= 65535 * kPaCombineRows, "%s: max_q must be in [0, 524280]", what);
     SOI_REQUIRE(scale > 0.0f && scale < __builtin_inff(), "%s: scale must be positive and finite", what);
     if (Tq == 0 || max_q == 0) return SOI_OK;
     SOI_REQUIRE(q && out && cu_q && cu_k && (Tk == 0 || (k && v)), "%s: null pointer", what);
     SOI_REQUIRE(k_token_stride >= 0 && k_token_stride < (int64_t(1) << 24) && v_token_stride >= 0 &&
                     v_token_stride < (int64_t(1) << 24),
                 "%s: key and value rows must be less than 2^24 elements apart", what);
-    SOI_REQUIRE(aligned16(k) && aligned16(v) && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
+    SOI_REQUIRE(q_token_stride >= 0 && q_token_stride < (int64_t(1) << 24), "%s: query rows must be less than 2^24 elements apart",
+                what);
+    SOI_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && q_token_stride % 8 == 0 &&
+                    q_head_stride % 8 == 0 && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
                     v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
-                "%s: k and v must be 16-byte aligned with strides of whole 16 bytes", what);
+                "%s: q, k and v must be 16-byte aligned with strides of whole 16 bytes", what);
     SOI_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_token_stride % 4 == 0 && out_head_stride % 4 == 0,
                 "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
+    const size_t need = soi_prompt_attention_workspace_bytes(Tq, Tk, num_q_heads, head_dim);
+    if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
+        set_last_error("%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", what, need, workspace_bytes);
+        return SOI_ERR_WORKSPACE;
+    }
+    const int64_t kt = pa_keys(head_dim), nsplit = pa_nsplit(Tq, Tk, num_q_heads, kt);
     const PaArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
-                   v_head_stride, out_token_stride, out_head_stride, cu_q, cu_k, static_cast<int>(Tq),
-                   static_cast<int>(Tk), static_cast<int>(num_q_heads), static_cast<int>(num_kv_heads),
-                   static_cast<int>(head_dim), scale * kLog2e};
-    constexpr int NW = 4;
-    const dim3 grid(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(batch),
-                    static_cast<unsigned>(ceil_div64(max_q, 32 * NW)));
-#define SOI_P(H) hipLaunchKernelGGL((prompt_attention_kernel<H, NW>), grid, dim3(NW * kWave), 0, as_stream(stream), a)
-    if (head_dim <= 64) SOI_P(64);
-    else if (head_dim <= 128) SOI_P(128);
-    else SOI_P(256);
+                   v_head_stride, out_token_stride, out_head_stride, cu_q, cu_k, static_cast<float*>(workspace),
+                   static_cast<int>(Tq), static_cast<int>(Tk), static_cast<int>(num_q_heads),
+                   static_cast<int>(num_kv_heads), static_cast<int>(head_dim), static_cast<int>(nsplit), scale * kLog2e};
+    constexpr int NW = kPaWaves;
+    const unsigned qtiles = static_cast<unsigned>(ceil_div64(max_q, 32 * NW));
+    const dim3 grid(static_cast<unsigned>(num_q_heads * nsplit), static_cast<unsigned>(batch), qtiles);
+    hipStream_t st = as_stream(stream);
+#define SOI_P(H, KT, NB, OCC) \
+    hipLaunchKernelGGL((prompt_attention_kernel<H, NW, KT, NB, OCC>), grid, dim3(NW * kWave), 0, st, a)
+    if (head_dim <= 64) SOI_P(64, 64, 2, 4);
+    else if (head_dim <= 128) SOI_P(128, 32, 3, 3);
+    else SOI_P(256, 64, 2, 1);
 #undef SOI_P
+    const int status = launch_status(what);
+    if (status || nsplit == 1) return status;
+    hipLaunchKernelGGL(prompt_combine_kernel, dim3(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(batch),
+                            static_cast<unsigned>(ceil_div64(max_q, kPaCombineRows))),
+                       dim3(256), 0, st, a, 32 * NW, static_cast<int>(kt));
     return launch_status(what);
 }

@@ -447,10 +447,13 @@ def kv4_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.
 
 
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
-                     max_q: int, scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+                     max_q: int, scale: float | None = None, out: torch.Tensor | None = None,
+                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed prompts on the matrix cores: q [Tq, NQ, hd], k and v [Tk, NKV, hd] fp16 (any token and
     head strides with contiguous dimensions: views of a fused projection work), hd a multiple of 8 up to 256. Sequence
     b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 (at most max_q), its keys rows cu_k[b] .. cu_k[b + 1] - 1; query i of
     nq sees keys j <= i + nk - nq, so more keys than queries continue a context. A query without a key gives zeros; rows
-    behind the last sequence are left as they are. k and v start on 16 bytes, their strides are multiples of 8."""
-    return _C.prompt_attention(q, k, v, cu_q, cu_k, max_q, scale, out)
+    behind the last sequence are left as they are. q, k and v start on 16 bytes, their strides are multiples of 8. out and
+    workspace (uint8, _C.prompt_attention_workspace_bytes; where few queries have their keys split over workgroups) are
+    allocated unless given; a workspace needs no initial value, and calls that overlap need one each."""
+    return _C.prompt_attention(q, k, v, cu_q, cu_k, max_q, scale, out, workspace)

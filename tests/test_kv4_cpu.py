@@ -28,7 +28,9 @@ def lib():
     lib.soi_kv4_decode_attention.argtypes = [p, p, i, i, i, p, f, p, C.c_size_t, p]
     lib.soi_kv4_decode_attention_workspace_bytes.argtypes = [i] * 5
     lib.soi_kv4_decode_attention_workspace_bytes.restype = C.c_size_t
-    lib.soi_prompt_attention.argtypes = [p, i, i, p, i, i, p, i, i, p, p, i, i, i, i, i, i, i, p, i, i, f, p]
+    lib.soi_prompt_attention.argtypes = [p, i, i, p, i, i, p, i, i, p, p, i, i, i, i, i, i, i, p, i, i, f, p, C.c_size_t, p]
+    lib.soi_prompt_attention_workspace_bytes.argtypes = [i] * 4
+    lib.soi_prompt_attention_workspace_bytes.restype = C.c_size_t
     return lib
 
 
@@ -89,8 +91,8 @@ def test_workspace_query(lib):
 
 
 def test_prompt_attention_checks(lib):
-    # q, 3 x (pointer, token stride, head stride), cu_q, cu_k, batch, Tq, Tk, max_q, NQ, NKV, hd, out, strides, scale, stream
-    ok = [16, 512, 128, 32, 256, 128, 48, 256, 128, 64, 64, 1, 8, 8, 8, 4, 2, 128, 1024, 512, 128, 1.0, None]
+    # q, 3 x (pointer, token stride, head stride), cu_q, cu_k, batch, Tq, Tk, max_q, NQ, NKV, hd, out, strides, scale, workspace, its bytes, stream
+    ok = [16, 512, 128, 32, 256, 128, 48, 256, 128, 64, 64, 1, 8, 8, 8, 4, 2, 128, 1024, 512, 128, 1.0, None, 0, None]
     for at, bad, text in ((17, 100, "multiple of 8"), (17, 264, "up to 256"), (17, 0, "head_dim"), (15, 3, "multiple of num_kv"),
                           (15, 0, "multiple"), (11, 0, "sequences"), (11, 65536, "sequences"), (12, -1, "token"),
                           (13, 1 << 30, "token"), (14, -1, "max_q"), (21, 0.0, "scale"), (21, float("inf"), "scale"),
@@ -99,8 +101,22 @@ def test_prompt_attention_checks(lib):
         args = list(ok)
         args[at] = bad
         assert text in error(lib, lib.soi_prompt_attention(*args)), (at, bad)
+    args = list(ok)
+    args[13] = 8192  # 8 queries over 8192 keys: split
+    st = lib.soi_prompt_attention(*args)
+    assert st == 2 and "workspace" in error(lib, st)
     assert lib.soi_prompt_attention(*ok[:12], 0, *ok[13:]) == 0
     assert lib.soi_prompt_attention(*ok[:14], 0, *ok[15:]) == 0
+
+
+def test_prompt_workspace_query(lib):
+    q = lib.soi_prompt_attention_workspace_bytes
+    assert q(8, 100, 4, 128) == 0 and q(0, 4096, 4, 128) == 0 and q(1 << 16, 1 << 16, 16, 128) == 0
+    n = q(8, 8192, 4, 128)
+    assert n > 0 and n % (8 * 4 * 130 * 4) == 0
+    for rows in (1, 100, 1000, 8000):  # bounded whatever the rows: at most about 2^16 of them with the splits counted
+        for heads in (1, 8, 64):
+            assert q(rows, 1 << 20, heads, 256) <= 2 * 65536 * 258 * 4
 
 
 @pytest.mark.parametrize("hd", [64, 128, 256])

@@ -45,6 +45,27 @@ def test_lengths(cuda, nq, nk):
     check(ops.prompt_attention(q, k, v, cu_q, cu_k, max(nq)), q, k, v, nq, nk, f"{nq} {nk}")
 
 
+@pytest.mark.parametrize("hd", [40, 64, 128, 200])
+@pytest.mark.parametrize("nq,nk", [([1, 40, 0], [1500, 3000, 9]), ([130], [1100]), ([700, 5], [700, 5000]), ([3], [129])])
+def test_split_keys(cuda, hd, nq, nk):
+    """Few queries: their keys are split over workgroups, some rows' more than others'."""
+    import soinfer._C as _C
+    import soinfer.ops as ops
+
+    q, k, v, cu_q, cu_k = problem(cuda, nq, nk, 4, 2, hd, 12)
+    n = _C.prompt_attention_workspace_bytes(sum(nq), sum(nk), 4, hd)
+    # 129 keys are fewer than two splits of four tiles where a tile has 64 keys (head_dim up to 64, or over 128)
+    assert n > 0 or (nk == [129] and not 64 < hd <= 128)
+    ws = torch.full((n,), 0xFF, dtype=torch.uint8, device=cuda)  # NaN floats: what it held before does not matter
+    out = torch.full_like(q, 2.0)
+    ops.prompt_attention(q, k, v, cu_q, cu_k, max(nq), out=out, workspace=ws)
+    check(out, q, k, v, nq, nk, f"split {hd}")
+    assert torch.equal(out, ops.prompt_attention(q, k, v, cu_q, cu_k, max(nq) + 500))
+    if n:
+        with pytest.raises(RuntimeError, match="workspace"):
+            ops.prompt_attention(q, k, v, cu_q, cu_k, max(nq), workspace=ws[:n - 16])
+
+
 def test_queries_without_keys_give_zeros(cuda):
     import soinfer.ops as ops
 
