@@ -323,6 +323,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
 // The split rows' states, in split order: four dimensions of one query and head a thread, kPaCombineRows queries of one
 // attention workgroup's `rows` a workgroup (many small workgroups: a thread's loads are two round trips, whatever they move).
 constexpr int kPaCombineRows = 8;
+constexpr int kPaMaxSplits = 64;
 __global__ __launch_bounds__(256) void prompt_combine_kernel(const PaArgs a, int rows, int keys_per_tile) {
     const int head = blockIdx.x, r0 = static_cast<int>(blockIdx.z) * kPaCombineRows;
     const PaRows w(a, blockIdx.y, r0 / rows, rows, keys_per_tile);
@@ -331,33 +332,61 @@ __global__ __launch_bounds__(256) void prompt_combine_kernel(const PaArgs a, int
     const int ns = (w.tiles + per - 1) / per, quads = a.hd >> 2;
     const int64_t stride = static_cast<int64_t>(a.Tq) * a.NQ;
     const float* ml = a.part + a.nsplit * stride * a.hd;
-    const int n = min(kPaCombineRows, w.nq - r0) * quads;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int r = r0 + i / quads, d = 4 * (i % quads);
-        const int64_t at = static_cast<int64_t>(w.q_lo + r) * a.NQ + head;
-        float M = kNegBig, lsum = 0.0f;
-        f32x4 v = {0, 0, 0, 0};
-        for (int s = 0; s < ns; ++s) M = fmaxf(M, ldg(ml + 2 * (s * stride + at)));
-        for (int s = 0; s < ns; ++s) {
-            const float e = fast_exp2(ldg(ml + 2 * (s * stride + at)) - M);
-            lsum = fmaf(ldg(ml + 2 * (s * stride + at) + 1), e, lsum);
-            v += ldg(reinterpret_cast<const f32x4*>(a.part + (s * stride + at) * a.hd + d)) * e;
-        }
+    const int rows_here = min(kPaCombineRows, w.nq - r0);
+    const int64_t row0 = static_cast<int64_t>(w.q_lo + r0) * a.NQ + head;
+    // the weights 2^(m_s - M) / l of each row's splits (32 lanes a row, splits j and j + 32 a lane)
+    __shared__ float s_w[kPaCombineRows][kPaMaxSplits];
+    {
+        const int r = threadIdx.x >> 5, j = threadIdx.x & 31;
+        const float* p = ml + 2 * (row0 + static_cast<int64_t>(r < rows_here ? r : 0) * a.NQ);
+        f32x2 x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            x[e] = j + 32 * e < ns ? ldg(reinterpret_cast<const f32x2*>(p + 2 * (j + 32 * e) * stride)) : f32x2{kNegBig, 0.0f};
+        float M = fmaxf(x[0].x, x[1].x);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 32));
+        const float e0 = fast_exp2(x[0].x - M), e1 = fast_exp2(x[1].x - M);
+        float lsum = fmaf(x[0].y, e0, x[1].y * e1);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor(lsum, o, 32);
         const float inv = lsum == 0.0f ? 0.0f : 1.0f / lsum;
-        const u32x2 o = {pack_f16x2(v.x * inv, v.y * inv), pack_f16x2(v.z * inv, v.w * inv)};
-        stg(reinterpret_cast<u32x2*>(a.out + (w.q_lo + r) * a.o_ts + head * a.o_hs + d), o);
+        s_w[r][j] = e0 * inv;
+        s_w[r][j + 32] = e1 * inv;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows_here * quads; i += 256) {
+        const int r = i / quads, d = 4 * (i % quads);
+        const float* p = a.part + (row0 + static_cast<int64_t>(r) * a.NQ) * a.hd + d;
+        f32x4 v = {0, 0, 0, 0};
+        for (int s = 0; s < ns; s += 8) {
+            f32x4 x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = ldg(reinterpret_cast<const f32x4*>(p + (s + e < ns ? s + e : s) * stride * a.hd));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float f = s + e < ns ? s_w[r][s + e] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = s + e < ns ? fmaf(x[e][k], f, v[k]) : v[k];
+            }
+        }
+        const u32x2 o = {pack_f16x2(v.x, v.y), pack_f16x2(v.z, v.w)};
+        stg(reinterpret_cast<u32x2*>(a.out + (w.q_lo + r0 + r) * a.o_ts + head * a.o_hs + d), o);
     }
 }
 
 constexpr int kPaWaves = 4;
 
-// Splits of a row's keys: where the queries alone make fewer workgroups than two to a CU, enough for that. (Every split
-// writes and reads hd + 2 floats a query.)
-static int64_t pa_nsplit(int64_t Tq, int64_t Tk, int64_t NQ, int64_t KT) {
+// Splits of a row's keys: where the queries alone make fewer workgroups than two to a CU (one at head_dim over 128, which
+// is what fits there), enough for that. Every split writes and reads hd + 2 floats a query: with 256 / 512 / 768 / 1024
+// workgroups aimed at, 512 queries over 16896 keys, 16 heads of 128, took 123 / 93 / 94 / 105 us, 2048 queries of 8 heads
+// 40 / 31 / 31 / 40 us; 300 queries x 2 over 3300 keys, 14 heads of 256, 67 us with 256 and 98 with 512.
+static int64_t pa_nsplit(int64_t Tq, int64_t Tk, int64_t NQ, int64_t hd, int64_t KT) {
     const int64_t groups = NQ * ceil_div64(Tq, 32 * kPaWaves), most = ceil_div64(ceil_div64(Tk, KT), kPaSplitTiles);
-    int64_t n = 512 / groups;
+    int64_t n = (hd > 128 ? 256 : 512) / groups;
     n = n < most ? n : most;
-    return n < 1 ? 1 : n > 64 ? 64 : n;
+    return n < 1 ? 1 : n > kPaMaxSplits ? kPaMaxSplits : n;
 }
 
 static int64_t pa_keys(int64_t hd) { return hd > 64 && hd <= 128 ? 32 : 64; }
@@ -368,7 +397,7 @@ using namespace soi;
 
 extern "C" size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim) {
     if (Tq < 1 || Tk < 1 || num_q_heads < 1 || head_dim < 1 || head_dim > 256) return 0;
-    const int64_t n = pa_nsplit(Tq, Tk, num_q_heads, pa_keys(head_dim));
+    const int64_t n = pa_nsplit(Tq, Tk, num_q_heads, head_dim, pa_keys(head_dim));
     return n == 1 ? 0 : static_cast<size_t>(n) * Tq * num_q_heads * (head_dim + 2) * sizeof(float);
 }
 
@@ -406,7 +435,7 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
         set_last_error("%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", what, need, workspace_bytes);
         return SOI_ERR_WORKSPACE;
     }
-    const int64_t kt = pa_keys(head_dim), nsplit = pa_nsplit(Tq, Tk, num_q_heads, kt);
+    const int64_t kt = pa_keys(head_dim), nsplit = pa_nsplit(Tq, Tk, num_q_heads, head_dim, kt);
     const PaArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
                    v_head_stride, out_token_stride, out_head_stride, cu_q, cu_k, static_cast<float*>(workspace),
                    static_cast<int>(Tq), static_cast<int>(Tk), static_cast<int>(num_q_heads),
