@@ -36,6 +36,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kKv4Waves = 4;
 constexpr int kKv4Block = 64;  // tokens a wave takes at a time
+constexpr int kv4_per_cu(int hd) { return hd == 64 ? 4 : hd == 128 ? 3 : 2; }  // workgroups that a CU's registers hold
 
 struct Kv4AttnArgs {
     const uint16_t* q;
@@ -68,35 +69,38 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive sum over the lan
     return v;
 }
 
-// Blocks per split, about `want` splits of all sequences' blocks together: whole rounds of a workgroup's waves.
-__device__ __forceinline__ int kv4_bps(const Kv4AttnArgs& a, const Kv4Cache& c, int lane) {
-    int total = 0;
-    for (int s = 0; s < c.B; s += kWave) total += s + lane < c.B ? kv4_blocks(kv4_len(c, s + lane, a.max_len)) : 0;
+// Where split y lies (FIND_SPLIT), or where the splits of sequence `at` begin: blocks per split `bps` (about `want` splits of
+// all sequences' blocks together, whole rounds of a workgroup's waves), the sequence b (-1: there is no split y) with its
+// length L, the split within it, and the index y0 of its first split. Every wave runs the same scan; up to 64 sequences are
+// one load.
+struct Kv4Place {
+    int bps, b, L, split, y0;
+};
+template <bool FIND_SPLIT>
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4AttnArgs& a, const Kv4Cache& c, int lane, int at) {
+    auto len_of = [&](int s) { return s + lane < c.B ? kv4_len(c, s + lane, a.max_len) : -1; };
+    auto blocks_of = [](int L) { return L < 0 ? 0 : kv4_blocks(L); };
+    const int len0 = len_of(0);
+    int total = blocks_of(len0);
+    for (int s = kWave; s < c.B; s += kWave) total += blocks_of(len_of(s));
     total = __builtin_amdgcn_readlane(wave_scan(total), 63);
-    const int n = (total + a.want - 1) / a.want;
-    return (n + kKv4Waves - 1) / kKv4Waves * kKv4Waves;
-}
-
-// Splits before sequence `upto`, and for `y`, where it is not negative, the sequence and its split that hold split y
-// (b = -1: none). One of the two questions a call.
-__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, const Kv4Cache& c, int bps, int lane, int upto, int y, int& b,
-                                        int& split) {
-    int base = 0;
-    b = -1;
-    split = 0;
-    for (int s = 0; s < upto; s += kWave) {
-        const int ns = s + lane < upto ? (kv4_blocks(kv4_len(c, s + lane, a.max_len)) + bps - 1) / bps : 0;
-        const int incl = wave_scan(ns);
-        const int all = __builtin_amdgcn_readlane(incl, 63);
-        if (y >= 0 && y < base + all) {
-            const int at = __builtin_ctzll(ballot(base + incl > y));
-            b = s + at;
-            split = y - base - (at ? __builtin_amdgcn_readlane(incl, at - 1) : 0);
-            return base;
+    Kv4Place p{0, -1, 0, 0, 0};
+    p.bps = ((total + a.want - 1) / a.want + kKv4Waves - 1) / kKv4Waves * kKv4Waves;
+    for (int s = 0; s < c.B; s += kWave) {
+        const int len = s ? len_of(s) : len0;
+        const int ns = (blocks_of(len) + p.bps - 1) / p.bps;
+        const int incl = wave_scan(ns), all = __builtin_amdgcn_readlane(incl, 63);
+        if (FIND_SPLIT ? at < p.y0 + all : at < s + kWave) {
+            const int i = FIND_SPLIT ? __builtin_ctzll(ballot(p.y0 + incl > at)) : at - s;
+            p.b = s + i;
+            p.L = __builtin_amdgcn_readlane(len, i);
+            p.y0 += i ? __builtin_amdgcn_readlane(incl, i - 1) : 0;
+            p.split = at - p.y0;
+            return p;
         }
-        base += all;
+        p.y0 += all;
     }
-    return base;
+    return p;
 }
 
 template <int HD, int GS>
@@ -107,8 +111,9 @@ struct Kv4Block {
     u32x4 s[SC];       // 16 bytes of the block's scales
 };
 
-template <int HD, int GS>
-__global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Cache c) {
+// BIG: pages of at least a block, so a block lies in one page and its addresses are wave-uniform but for the lane's offset.
+template <int HD, int GS, bool BIG>
+__global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_kernel(const Kv4AttnArgs a, const Kv4Cache c) {
     constexpr int W = HD / 32, U = HD / 64, G = HD / GS, DT = HD / 16, SC = Kv4Block<HD, GS>::SC;
     __shared__ float s_state[kKv4Waves][16][HD + 2];
     __shared__ __attribute__((aligned(16))) uint16_t s_scale[kKv4Waves][2][G][4][16];  // K, V; group; piece; token
@@ -116,11 +121,9 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
     const int col = lane & 15, g = lane >> 4;
     const int kvh = static_cast<int>(blockIdx.x) / a.htiles, ht = static_cast<int>(blockIdx.x) % a.htiles;
     const int y = blockIdx.y;
-    const int bps = kv4_bps(a, c, lane);
-    int b, split;
-    kv4_find(a, c, bps, lane, c.B, y, b, split);
-    if (b < 0) return;
-    const int L = __builtin_amdgcn_readfirstlane(kv4_len(c, b, a.max_len));
+    const Kv4Place at = kv4_place<true>(a, c, lane, y);
+    if (at.b < 0) return;
+    const int b = at.b, L = at.L, split = at.split, bps = at.bps;
     const int nb = kv4_blocks(L);
     const int b1 = min(nb, (split + 1) * bps);
     const int h0 = kvh * a.rep + ht * 16, nh = min(16, a.rep - ht * 16);  // the query heads of this workgroup
@@ -136,17 +139,26 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
         }
     }
 
-    // A block's operands: page ids by 16-token piece, the lane's K token in piece col >> 2, its V tokens in piece g, its
-    // scales in piece (lane >> 1) & 3: chunk (lane >> 1 is piece + 4 (group + G kv)), half lane & 1.
-    auto page_of = [&](int blk, int piece) { return kv4_page(c, b, blk * kKv4Block + 16 * piece); };
-    auto load = [&](Kv4Block<HD, GS>& x, int blk, int vid) {
-        const int kid = page_of(blk, col >> 2);
-        const int kt = (blk * kKv4Block + 16 * (col >> 2) + (col & 3)) & (c.page - 1);
-        const int vt = (blk * kKv4Block + 16 * g) & (c.page - 1);
-        const uint8_t* kp = c.k_pages + ((static_cast<int64_t>(kid < 0 ? 0 : kid) * c.NKV + kvh) * c.page + kt) * (HD / 2) +
-                            4 * W * g;
-        const int64_t vhead = static_cast<int64_t>(vid < 0 ? 0 : vid) * c.NKV + kvh;
-        const uint8_t* vp = c.v_pages + (vhead * c.page + vt) * (HD / 2) + col * (U * 8);
+    // The page of piece lane & 3 of a block, read one block before its operands are.
+    auto pages_of = [&](int blk) { return blk < b1 ? kv4_page(c, b, blk * kKv4Block + (BIG ? 0 : 16 * (lane & 3))) : -1; };
+    auto piece_page = [&](int ids, int piece) {
+        if constexpr (BIG) return __builtin_amdgcn_readfirstlane(ids);
+        const int p0 = __builtin_amdgcn_readlane(ids, 0), p1 = __builtin_amdgcn_readlane(ids, 1);
+        const int p2 = __builtin_amdgcn_readlane(ids, 2), p3 = __builtin_amdgcn_readlane(ids, 3);
+        return piece < 2 ? (piece < 1 ? p0 : p1) : (piece < 3 ? p2 : p3);
+    };
+    // A block's operands: the lane's K token in piece col >> 2, its V tokens in piece g, its scales in piece
+    // (lane >> 1) & 3: 16-byte chunk (lane >> 1 is piece + 4 (group + G kv)), half lane & 1.
+    auto slot_of = [&](int blk, int piece) {  // of the piece's first token, from the block's (BIG) or the page's first slot
+        return BIG ? 16 * piece : (blk * kKv4Block + 16 * piece) & (c.page - 1);
+    };
+    auto lead_of = [&](int blk) { return BIG ? (blk * kKv4Block) & (c.page - 1) : 0; };
+    auto head_of = [&](int id) { return static_cast<int64_t>(id < 0 ? 0 : id) * c.NKV + kvh; };
+    Kv4Block<HD, GS> x;
+    auto load_k = [&](int blk, int ids) {
+        const int kid = piece_page(ids, col >> 2), sid = piece_page(ids, (lane >> 1) & 3), lead = lead_of(blk);
+        const uint8_t* kp = c.k_pages + (head_of(kid) * c.page + lead) * (HD / 2) +
+                            (slot_of(blk, col >> 2) + (col & 3)) * (HD / 2) + 4 * W * g;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (W == 2) {
@@ -164,16 +176,18 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
                 }
             }
         }
-        {
-            const int piece = (lane >> 1) & 3, sid = page_of(blk, piece);
-            const int st = (blk * kKv4Block + 16 * piece + 8 * (lane & 1)) & (c.page - 1);
-            const int64_t head = static_cast<int64_t>(sid < 0 ? 0 : sid) * c.NKV + kvh;
+        const int st = slot_of(blk, (lane >> 1) & 3) + 8 * (lane & 1);
 #pragma unroll
-            for (int e = 0; e < SC; ++e) {
-                const int gk = (lane >> 3) + 8 * e, kv = gk / G < 1 ? 0 : 1, grp = gk % G;  // lanes past 2 G repeat V's
-                x.s[e] = ldg(reinterpret_cast<const u32x4*>((kv ? c.v_scale : c.k_scale) + (head * G + grp) * c.page + st));
-            }
+        for (int e = 0; e < SC; ++e) {
+            const int gk = (lane >> 3) + 8 * e, grp = gk % G;  // lanes past 2 G repeat V's
+            const uint16_t* sp = gk < G ? c.k_scale : c.v_scale;
+            x.s[e] = ldg(reinterpret_cast<const u32x4*>(sp + head_of(sid) * G * c.page + lead + grp * c.page + st));
         }
+    };
+    auto load_v = [&](int blk, int ids) {
+        const int vid = piece_page(ids, g);
+        const uint8_t* vp = c.v_pages + (head_of(vid) * c.page + lead_of(blk)) * (HD / 2) + slot_of(blk, g) * (HD / 2) +
+                            col * (U * 8);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if constexpr (U == 1) {
@@ -188,26 +202,22 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
             }
         }
     };
+
     f32x4 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x4{0, 0, 0, 0};
     float m = kNegBig, l = 0.0f;
 
+    // One set of operand registers: K's are loaded again as soon as the scores are done, V's after the products, so each
+    // load has about half a block's work in front of it; page ids are a block further ahead.
     int blk = split * bps + wave;
-    Kv4Block<HD, GS> cur;
-    int vid = -1;
+    int ids = pages_of(blk), next_ids = pages_of(blk + kKv4Waves);
     if (blk < b1) {
-        vid = page_of(blk, g);
-        load(cur, blk, vid);
+        load_k(blk, ids);
+        load_v(blk, ids);
     }
-    for (; blk < b1; blk += kKv4Waves) {
-        Kv4Block<HD, GS> nxt;
-        int nvid = -1;
-        if (blk + kKv4Waves < b1) {  // wave-uniform; the next block's operands are in flight during this one's products
-            nvid = page_of(blk + kKv4Waves, g);
-            load(nxt, blk + kKv4Waves, nvid);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+    auto step = [&](auto MORE) {  // MORE: another block of this wave follows
+        const int vid = piece_page(ids, g);
         // live: how many of the lane's tokens 16 g + 0 .. 15 there are
         const int left = L - blk * kKv4Block - 16 * g;
         const int live = vid < 0 ? 0 : left < 0 ? 0 : left < 16 ? left : 16;
@@ -216,7 +226,7 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
             u32x4* dst = reinterpret_cast<u32x4*>(&s_scale[wave][0][0][0][0]);
 #pragma unroll
             for (int e = 0; e < SC; ++e) {
-                u32x4 w = cur.s[e];
+                u32x4 w = x.s[e];
                 if (!whole) {  // scales of slots without a token are whatever was there: zeros, so that 0 weights stay 0
                     const int n = __shfl(live, 16 * ((lane >> 1) & 3)) - 8 * (lane & 1);
 #pragma unroll
@@ -238,7 +248,7 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
 #pragma unroll
                 for (int j = r * (GS / 32); j < (r + 1) * (GS / 32); ++j) {
                     f16x2 v[4];
-                    dequant_int4x8_bitfield(cur.k[i][j], v);
+                    dequant_int4x8_bitfield(x.k[i][j], v);
                     const f16x8 ka = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
                     sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, qf[j], sum, 0, 0, 0);
                 }
@@ -250,8 +260,15 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
                 t[3] = fmaf(sum[3], static_cast<float>(hi.y), t[3]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[4 * i + e] = t[e];
+            for (int e = 0; e < 4; ++e) {
+                s[4 * i + e] = t[e];
+                asm volatile("" : "+v"(s[4 * i + e]));  // (the compiler would keep all products and sum them up later)
+            }
+            if (i & 1) __builtin_amdgcn_sched_barrier(0);  // (and unpack all tiles at once)
         }
+        const int ids2 = pages_of(blk + 2 * kKv4Waves);
+        if constexpr (MORE) load_k(blk + kKv4Waves, next_ids);
+        __builtin_amdgcn_sched_barrier(0);
         if (!whole) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = e < live ? s[e] : -__builtin_inff();
@@ -273,44 +290,45 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
             s[e] = fast_exp2(fmaf(s[e], a.scale_log2, -m));
             l += s[e];
         }
-        // per half block (8 tokens a lane): P^T of each scale group, then its dimension tiles
+        // per half block (8 tokens a lane) and scale group: P^T, then the group's dimension tiles
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            f16x8 pb[G];
 #pragma unroll
             for (int r = 0; r < G; ++r) {
                 const u32x4 sc = *reinterpret_cast<const u32x4*>(&s_scale[wave][1][r][g][8 * half]);
+                f16x8 pb;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const f16x2 w = as_f16x2(sc[e >> 1]);
-                    pb[r][e] = static_cast<f16>(s[8 * half + e] * static_cast<float>(w[e & 1]));
+                    const f16x2 w = as_f16x2(sc[e >> 1]);  // (fma, not a product: one mixed-precision instruction)
+                    pb[e] = static_cast<f16>(fmaf(s[8 * half + e], static_cast<float>(w[e & 1]), 0.0f));
                 }
-            }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t w[4] = {cur.v[2 * half][u].x, cur.v[2 * half][u].y, cur.v[2 * half + 1][u].x,
-                                       cur.v[2 * half + 1][u].y};  // tokens (0, 1), (2, 3), (4, 5), (6, 7)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int d = r * (GS / 16); d < (r + 1) * (GS / 16); ++d) {
+                    const int u = d >> 2, n = d & 3;
+                    const uint32_t w[4] = {x.v[2 * half][u].x, x.v[2 * half][u].y, x.v[2 * half + 1][u].x,
+                                           x.v[2 * half + 1][u].y};  // tokens (0, 1), (2, 3), (4, 5), (6, 7)
                     const f16x2 bias = {(f16)-1032.0f, (f16)-1032.0f}, bias16 = {(f16)-72.0f, (f16)-72.0f};
                     const f16x2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
                     f16x2 v[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const uint32_t x = n < 2 ? w[e] : w[e] >> 8;
-                        v[e] = n & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(x, 0x00f000f0u, 0x64806480u)), sixteenth,
+                        const uint32_t y8 = n < 2 ? w[e] : w[e] >> 8;
+                        v[e] = n & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(y8, 0x00f000f0u, 0x64806480u)), sixteenth,
                                                                  bias16)
-                                     : as_f16x2(and_xor(x, 0x000f000fu, 0x64086408u)) + bias;
+                                     : as_f16x2(and_xor(y8, 0x000f000fu, 0x64086408u)) + bias;
                     }
                     const f16x8 va = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-                    const int d = 4 * u + n;
-                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb[16 * d / GS], acc[d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pb, acc[d], 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);  // (all groups at once would spill)
             }
         }
-        cur = nxt;
-        vid = nvid;
-    }
+        if constexpr (MORE) load_v(blk + kKv4Waves, next_ids);
+        ids = next_ids;
+        next_ids = ids2;
+    };
+    for (; blk + kKv4Waves < b1; blk += kKv4Waves) step(std::true_type{});  // (wave-uniform)
+    if (blk < b1) step(std::false_type{});
 
     // lane (c, g): dimensions 16 d + 4 g + 0 .. 3 of head c
     l += xor_lanes<16>(l);
@@ -349,64 +367,73 @@ __global__ __launch_bounds__(kKv4Waves * kWave, HD == 256 ? 1 : 3) void kv4_attn
     }
 }
 
-// The states of split contexts, in split order: a wave per (sequence, query head).
-constexpr int kKv4MostSplits = 1032;  // of one sequence: want + 1 at most, want <= kKv4Target
+// The states of split contexts, summed in a fixed order: a workgroup per (sequence, query head), whose four waves take
+// eight states each of every 32. The first 32 states' sums are requested with the (m, l) pairs, so a context of up to 32
+// splits is two round trips: the lengths, then all states.
+constexpr int kKv4MostSplits = 1032;  // of one sequence: want + 1 at most, want <= 1024
 
 template <int HD>
 __global__ __launch_bounds__(kKv4Waves * kWave) void kv4_combine_kernel(const Kv4AttnArgs a, const Kv4Cache c) {
-    constexpr int E = HD / 64;
-    __shared__ float s_w[kKv4Waves][kKv4MostSplits];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int h = static_cast<int>(blockIdx.x) * kKv4Waves + wave, b = blockIdx.y;
-    const int bps = kv4_bps(a, c, lane);
-    const int ns = (kv4_blocks(__builtin_amdgcn_readfirstlane(kv4_len(c, b, a.max_len))) + bps - 1) / bps;
-    if (ns == 1 || h >= a.NQ) return;  // written by its one split
-    int unused_b, unused_s;
-    const int y0 = kv4_find(a, c, bps, lane, b, -1, unused_b, unused_s);
+    constexpr int E = HD / 64, N = 8;
+    __shared__ float s_w[kKv4MostSplits], s_v[kKv4Waves][HD];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = blockIdx.x;
+    const Kv4Place at = kv4_place<false>(a, c, lane, blockIdx.y);
+    const int b = at.b, ns = (kv4_blocks(at.L) + at.bps - 1) / at.bps;
+    if (ns == 1) return;  // written by its one split
     const int64_t stride = static_cast<int64_t>(a.NQ) * (HD + 2);
-    const float* p = a.part + y0 * stride + static_cast<int64_t>(h) * (HD + 2);
-    float* sw = s_w[wave];
-    float M = kNegBig;
-    for (int s = lane; s < ns; s += kWave) {
-        const float ms = ldg(p + s * stride);
-        sw[s] = ms;
-        M = fmaxf(M, ms);
+    const float* p = a.part + at.y0 * stride + static_cast<int64_t>(h) * (HD + 2);
+    float x[N][E];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[k][e] = ldg(p + (s + k < ns ? s + k : 0) * stride + 2 + 64 * e + lane);
+    };
+    float m0 = kNegBig, l0 = 0.0f;
+    if (lane < ns) {
+        m0 = ldg(p + lane * stride);
+        l0 = ldg(p + lane * stride + 1);
     }
+    load(wave * N);
+    float M = m0;
+    for (int s = lane + kWave; s < ns; s += kWave) M = fmaxf(M, ldg(p + s * stride));
     M = wave_max_bcast(M);
     float lsum = 0.0f;
     for (int s = lane; s < ns; s += kWave) {
-        const float e = fast_exp2(sw[s] - M);
-        sw[s] = e;
-        lsum = fmaf(ldg(p + s * stride + 1), e, lsum);
+        const float e = fast_exp2((s < kWave ? m0 : ldg(p + s * stride)) - M);
+        if (wave == 0) s_w[s] = e;
+        lsum = fmaf(s < kWave ? l0 : ldg(p + s * stride + 1), e, lsum);
     }
     lsum = wave_sum_bcast(lsum);
-    __builtin_amdgcn_wave_barrier();
+    __syncthreads();  // the weights
     float v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.0f;
-    for (int s = 0; s < ns; s += 8) {
-        float x[8][E];
+    for (int s = wave * N; s < ns; s += kKv4Waves * N) {
+        if (s >= kKv4Waves * N) load(s);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
+        for (int k = 0; k < N; ++k) {
+            if (s + k >= ns) break;
+            const float w = s_w[s + k];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[k][e] = ldg(p + (s + k < ns ? s + k : s) * stride + 2 + 64 * e + lane);
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = s + k < ns ? fmaf(x[k][e], sw[s + k], v[e]) : v[e];
+            for (int e = 0; e < E; ++e) v[e] = fmaf(x[k][e], w, v[e]);
+        }
     }
 #pragma unroll
-    for (int e = 0; e < E; ++e)
-        stg(a.out + (static_cast<int64_t>(b) * a.NQ + h) * HD + 64 * e + lane,
-            f32_to_f16_bits(lsum == 0.0f ? 0.0f : v[e] / lsum));
+    for (int e = 0; e < E; ++e) s_v[wave][64 * e + lane] = v[e];
+    __syncthreads();  // the waves' sums
+    const int d = threadIdx.x;
+    if (d >= HD) return;
+    const float sum = (s_v[0][d] + s_v[1][d]) + (s_v[2][d] + s_v[3][d]);
+    stg(a.out + (static_cast<int64_t>(b) * a.NQ + h) * HD + d, f32_to_f16_bits(lsum == 0.0f ? 0.0f : sum / lsum));
 }
 
-// Splits aimed at (over all sequences) so that the workgroups are about kKv4Target, and the most there can be of them.
-constexpr int64_t kKv4Target = 768;
+// Splits aimed at (over all sequences) so that the workgroups fill the 256 CUs once, and the most there can be of them.
 struct Kv4Plan {
     int64_t want, splits;
     bool combine;
-    Kv4Plan(int64_t B, int64_t NKV, int64_t rep, int64_t max_len) {
+    Kv4Plan(int64_t B, int64_t NKV, int64_t rep, int64_t hd, int64_t max_len) {
+        const int64_t kKv4Target = 256 * kv4_per_cu(static_cast<int>(hd));
         const int64_t units = NKV * ceil_div64(rep, 16), nb = max_len < 1 ? 1 : ceil_div64(max_len, kKv4Block);
         want = kKv4Target / units < 1 ? 1 : kKv4Target / units;
         const int64_t most = B * ceil_div64(nb, kKv4Waves);  // a split has at least a block for every wave
@@ -424,7 +451,7 @@ extern "C" size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_
     if (batch < 1 || num_kv_heads < 1 || num_q_heads < num_kv_heads || num_q_heads % num_kv_heads || head_dim < 1 ||
         max_len < 0 || max_len > (int64_t(1) << 30))
         return 0;
-    const Kv4Plan p(batch, num_kv_heads, num_q_heads / num_kv_heads, max_len);
+    const Kv4Plan p(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim, max_len);
     return p.combine ? static_cast<size_t>(p.splits) * num_q_heads * (head_dim + 2) * sizeof(float) : 0;
 }
 
@@ -446,7 +473,7 @@ extern "C" int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16
     SOI_REQUIRE(scale > 0.0f && scale < __builtin_inff(), "%s: scale must be positive and finite", what);
     SOI_REQUIRE(q && out && q != out, "%s: null pointer or out = q", what);
     const int64_t rep = num_q_heads / NKV;
-    const Kv4Plan plan(B, NKV, rep, max_len);
+    const Kv4Plan plan(B, NKV, rep, hd, max_len);
     SOI_REQUIRE(plan.splits <= 65535, "%s: too many sequences", what);
     const size_t need = soi_kv4_decode_attention_workspace_bytes(B, num_q_heads, NKV, hd, max_len);
     if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3))) {
@@ -460,12 +487,18 @@ extern "C" int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16
     const Kv4Cache c = kv4_device(cache);
     const dim3 grid(static_cast<unsigned>(NKV * htiles), static_cast<unsigned>(plan.splits));
     hipStream_t s = as_stream(stream);
-#define SOI_X(H, G) hipLaunchKernelGGL((kv4_attn_kernel<H, G>), grid, dim3(kKv4Waves * kWave), 0, s, a, c)
+#define SOI_X(H, G)                                                                                         \
+    do {                                                                                                    \
+        if (cache->page_size >= kKv4Block)                                                                  \
+            hipLaunchKernelGGL((kv4_attn_kernel<H, G, true>), grid, dim3(kKv4Waves * kWave), 0, s, a, c);   \
+        else                                                                                                \
+            hipLaunchKernelGGL((kv4_attn_kernel<H, G, false>), grid, dim3(kKv4Waves * kWave), 0, s, a, c);  \
+    } while (0)
     SOI_KV4_SHAPES(SOI_X);
 #undef SOI_X
     st = launch_status(what);
     if (st || !plan.combine) return st;
-    const dim3 cgrid(static_cast<unsigned>(ceil_div64(num_q_heads, kKv4Waves)), static_cast<unsigned>(B));
+    const dim3 cgrid(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(B));
 #define SOI_C(H) hipLaunchKernelGGL((kv4_combine_kernel<H>), cgrid, dim3(kKv4Waves * kWave), 0, s, a, c)
     if (hd == 64) SOI_C(64);
     else if (hd == 128) SOI_C(128);
