@@ -75,35 +75,74 @@ __device__ __forceinline__ uint32_t xor_u(uint32_t v) {
     return __builtin_bit_cast(uint32_t, xor_lanes<MASK>(__builtin_bit_cast(float, v)));
 }
 
-// Scale bits and codes (0 .. 15, one a byte of lo / hi) of the lane's eight values, over a group of GS / 8 lanes.
-// max|x| is taken on the bit patterns: infinity and NaN come out on top. The quotient x / s of two binary16 numbers is
-// either a tie exactly or further than 2^-13 of its size from one, so one refined reciprocal decides every rounding as
-// the exact quotient would.
-template <int GS>
-__device__ __forceinline__ uint16_t kv4_quantize(const u32x4& x, uint32_t q[8]) {
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-    u16x2 m = __builtin_bit_cast(u16x2, w[0] & 0x7fff7fffu);
+// 1 / sqrt(x) to the last bits of binary64: two Newton steps on y (3 - x y^2) / 2 from the hardware's estimate.
+__device__ __forceinline__ double rsqrt_f64(double x) {
+    double y = __builtin_amdgcn_rsq(x);
 #pragma unroll
-    for (int i = 1; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
-    uint32_t top = m.x > m.y ? m.x : m.y;
-    auto take = [&](uint32_t o) { top = o > top ? o : top; };
-    take(dpp_u<0xb1>(top));
-    take(dpp_u<0x4e>(top));
-    if (GS >= 64) take(dpp_u<0x141>(top));
-    if (GS >= 128) take(dpp_u<0x128>(top));
-    const uint16_t s = f32_to_f16_bits(f16_bits_to_f32(static_cast<uint16_t>(top)) / 7.0f);
-    const float sf = f16_bits_to_f32(s);
-    const bool live = s > 0 && s < 0x7c00;
-    const float r = live ? __builtin_amdgcn_rcpf(sf) : 0.0f;
+    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return y;
+}
+
+// Lane o of a token's hd / 8 holds eight dimensions in two quads, 4 o + 0 .. 3 (x) and hd / 2 + 4 o + 0 .. 3 (y): the pairs
+// of the rotation are one lane's, so an element is widened once for both its products, and a lane needs the cos and sin
+// of four angles only.
+struct Quads {
+    u32x2 x, y;
+};
+
+// Scale bits of x's and y's group (low and high half of the result) and the codes, 0 .. 15 each: x's four in the low
+// nibbles of the bytes, y's in the high ones. max|x| is taken on the bit patterns, where infinity and NaN come out on top.
+// max / 7 is never a binary16 tie nor within 2^-15 of one, so the product with 1 / 7 rounds as the quotient would. A
+// quotient x / s of two binary16 numbers is a tie exactly or further than 2^-13 of its size from one, so one refined
+// reciprocal decides every rounding as the exact quotient would.
+template <int HD, int GS>
+__device__ __forceinline__ uint32_t kv4_quantize(const Quads& v, uint32_t& codes) {
+    const uint32_t w[4] = {v.x.x, v.x.y, v.y.x, v.y.y};
+    u16x2 m[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float v = f16_bits_to_f32(static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1))));
-        float y = v * r;
-        y = fmaf(fmaf(-y, sf, v), r, y);
-        y = fminf(fmaxf(rintf(y), -7.0f), 7.0f);
-        q[i] = live ? static_cast<uint32_t>(static_cast<int>(y)) & 15u : 0u;
+    for (int i = 0; i < 4; ++i) m[i] = __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu);
+    const u16x2 mx = __builtin_elementwise_max(m[0], m[1]), my = __builtin_elementwise_max(m[2], m[3]);
+    u16x2 top = {mx.x > mx.y ? mx.x : mx.y, my.x > my.y ? my.x : my.y};  // x's, y's
+    auto take = [&](uint32_t o) { top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, o)); };
+    auto bits = [&] { return __builtin_bit_cast(uint32_t, top); };
+    take(dpp_u<0xb1>(bits()));  // eight lanes: 32 dimensions
+    take(dpp_u<0x4e>(bits()));
+    take(dpp_u<0x141>(bits()));
+    if (GS >= 64 && HD >= 128) take(dpp_u<0x128>(bits()));  // sixteen
+    if (GS >= 128 && HD >= 256) take(xor_u<16>(bits()));    // thirty-two
+    if (GS > HD / 2) take((bits() << 16) | (bits() >> 16));  // one group for both quads
+    uint32_t scales = 0;
+    codes = 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint16_t s = f32_to_f16_bits(f16_bits_to_f32(h ? top.y : top.x) * (1.0f / 7.0f));
+        const float sf = f16_bits_to_f32(s);
+        const bool live = s > 0 && s < 0x7c00;
+        const float r = live ? __builtin_amdgcn_rcpf(sf) : 0.0f;
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = static_cast<float>(as_f16x2(w[2 * h + (i >> 1)])[i & 1]);
+            float q = e * r;
+            q = fmaf(fmaf(-q, sf, e), r, q);
+            q = __builtin_amdgcn_fmed3f(rintf(q), -7.0f, 7.0f);
+            // (a binary32 integer plus 1.5 x 2^23 has its two's complement in the low bits)
+            c |= (__builtin_bit_cast(uint32_t, q + 12582912.0f) & 15u) << (8 * i + 4 * h);
+        }
+        codes |= live ? c : 0u;
+        scales |= static_cast<uint32_t>(s) << (16 * h);
     }
-    return s;
+    return scales;
+}
+
+// Four nibbles in the low halves of the bytes -> 16 bits.
+__device__ __forceinline__ uint32_t squeeze4(uint32_t b) {
+    b = (b | (b >> 4)) & 0x00ff00ffu;
+    return (b | (b >> 8)) & 0xffffu;
+}
+__device__ __forceinline__ uint32_t stretch4(uint32_t n) {
+    n = (n | (n << 8)) & 0x00ff00ffu;
+    return (n | (n << 4)) & 0x0f0f0f0fu;
 }
 
 struct Kv4AppendArgs {
@@ -120,174 +159,227 @@ struct Kv4AppendArgs {
     double eps;
 };
 
-// One wave per hd / 8 ... lanes: a token's head is hd / 8 lanes of eight dimensions each, so a wave takes 64 / (hd / 8)
-// consecutive tokens, and `heads_per_wave` heads of them one after another with the same cos / sin values in registers.
+// A token's head is hd / 8 lanes of two quads each, so a wave takes 512 / hd consecutive tokens, and `heads_per_wave` heads
+// of them one after another with the same cos / sin values in registers, the next head's row on its way.
 //
 // The norm and the rotation are evaluated in binary64 (binary16 and binary32 operands: the products are exact), then
-// rounded to binary16 where qk_norm_rope_append rounds. A cached code is then a function of the inputs alone: a binary32
-// evaluation would now and then fall on the other side of a rounding border, and a code with it.
+// rounded to binary32 and to binary16 where qk_norm_rope_append rounds. A cached code is then a function of the inputs
+// alone: a binary32 evaluation would now and then fall on the other side of a rounding border, and a code with it. (MI355X
+// issues binary64 fma at the rate of single binary32 ones; what it costs is the conversions.)
 template <int HD, int GS>
 __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a, const Kv4Cache c) {
-    constexpr int LPT = HD / 8, TPW = kWave / LPT, W = HD / 32;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int LPT = HD / 8, TPW = kWave / LPT, W = HD / 32, H2 = HD / 2;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o = lane % LPT, i = lane / LPT;
     const int t0 = static_cast<int>(blockIdx.x) * TPW, t = t0 + i;
     const int heads = a.NQ + 2 * c.NKV;
     const int h0 = (static_cast<int>(blockIdx.y) * 4 + wave) * a.heads_per_wave;
     if (h0 >= heads) return;  // wave-uniform
+    const int h1 = min(heads, h0 + a.heads_per_wave);
+    // the first head's row does not wait for the token's place (a row of the input, whatever sequence it belongs to)
+    const uint16_t* src = a.qkv + static_cast<int64_t>(t < a.T ? t : 0) * a.qkv_stride + 4 * o;
+    auto row_of = [&](int h) {
+        const uint16_t* p = src + static_cast<int64_t>(h) * HD;
+        return Quads{ldg_any8(p), ldg_any8(p + H2)};
+    };
+    Quads next = row_of(h0);
+    Quads wq{}, wk{};
+    if (a.q_norm) {
+        wq = Quads{ldg_any8(a.q_norm + 4 * o), ldg_any8(a.q_norm + H2 + 4 * o)};
+        wk = Quads{ldg_any8(a.k_norm + 4 * o), ldg_any8(a.k_norm + H2 + 4 * o)};
+    }
     int b, pos;
     const bool found = kv4_locate<TPW>(a.cu, c.lens, c.B, t0, i, lane, b, pos) && t < a.T;
     const int id = found ? kv4_page(c, b, pos) : -1;
     const bool keep = id >= 0 && pos < a.table_rows;  // past the tables nothing is appended, q takes the last row
     const int slot = pos & (c.page - 1);
     const int row = pos < 0 ? 0 : pos < a.table_rows ? pos : a.table_rows - 1;
-    float cs[8], sn[8];
+    double cs[4], sn[4];
     {
-        const int64_t at = static_cast<int64_t>(row) * (HD / 2) + 8 * (o % (LPT / 2));
+        const int64_t at = static_cast<int64_t>(row) * H2 + 4 * o;
+        const f32x4 cv = __builtin_bit_cast(f32x4, ldg_any(a.cos_t + at)), sv = __builtin_bit_cast(f32x4, ldg_any(a.sin_t + at));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            cs[j] = ldg(a.cos_t + at + j);
-            sn[j] = ldg(a.sin_t + at + j);
+        for (int j = 0; j < 4; ++j) {
+            cs[j] = cv[j];
+            sn[j] = sv[j];
         }
     }
-    const uint16_t* src = a.qkv + (found ? static_cast<int64_t>(t) : 0) * a.qkv_stride + 8 * o;
-    const double sign = o < LPT / 2 ? -1.0 : 1.0;
-    for (int h = h0; h < h0 + a.heads_per_wave && h < heads; ++h) {
-        u32x4 x = ldg_any(src + static_cast<int64_t>(h) * HD);
+    for (int h = h0; h < h1; ++h) {
+        Quads v = next;
+        if (h + 1 < h1) next = row_of(h + 1);
         const bool is_q = h < a.NQ, is_v = h >= a.NQ + c.NKV;
         if (!is_v) {
-            const uint16_t* wn = is_q ? a.q_norm : a.k_norm;
-            if (wn) {
-                const u32x4 g = ldg_any(wn + 8 * o);
-                const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, gw[4] = {g.x, g.y, g.z, g.w};
+            if (a.q_norm) {
+                const Quads g = is_q ? wq : wk;
+                const uint32_t e[4] = {v.x.x, v.x.y, v.y.x, v.y.y}, w[4] = {g.x.x, g.x.y, g.y.x, g.y.y};
                 double ss = 0.0;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const double v = f16_bits_to_f32(static_cast<uint16_t>(xw[j >> 1] >> (16 * (j & 1))));
-                    ss = fma(v, v, ss);
+                    const float f = static_cast<float>(as_f16x2(e[j >> 1])[j & 1]);
+                    ss += static_cast<double>(f * f);  // exact in binary32
                 }
-                const double inv = 1.0 / sqrt(token_sum<LPT>(ss) / HD + a.eps);
-                uint32_t rw[4];
+                const double inv = rsqrt_f64(token_sum<LPT>(ss) / HD + a.eps);
+                uint32_t r[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const f16x2 p = as_f16x2(xw[j]), q = as_f16x2(gw[j]);
-                    rw[j] = pack_f16x2(
-                        static_cast<float>(static_cast<double>(p.x) * inv * static_cast<double>(q.x)),
-                        static_cast<float>(static_cast<double>(p.y) * inv * static_cast<double>(q.y)));
+                    const f16x2 p = as_f16x2(e[j]), q = as_f16x2(w[j]);  // element x weight: exact in binary32
+                    const float lo = static_cast<float>(p.x) * static_cast<float>(q.x);
+                    const float hi = static_cast<float>(p.y) * static_cast<float>(q.y);
+                    r[j] = pack_f16x2(static_cast<float>(lo * inv), static_cast<float>(hi * inv));
                 }
-                x = u32x4{rw[0], rw[1], rw[2], rw[3]};
+                v = Quads{u32x2{r[0], r[1]}, u32x2{r[2], r[3]}};
             }
-            const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-            uint32_t rw[4];
+            {
+                const uint32_t xa[2] = {v.x.x, v.x.y}, xb[2] = {v.y.x, v.y.y};
+                float ra[4], rb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f16x2 p = as_f16x2(xw[j]), q = as_f16x2(xor_u<LPT / 2>(xw[j]));
-                float r[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    r[e] = static_cast<float>(fma(static_cast<double>(p[e]), static_cast<double>(cs[2 * j + e]),
-                                                  sign * static_cast<double>(q[e]) * static_cast<double>(sn[2 * j + e])));
-                rw[j] = pack_f16x2(r[0], r[1]);
+                for (int j = 0; j < 4; ++j) {
+                    const double p = static_cast<float>(as_f16x2(xa[j >> 1])[j & 1]);
+                    const double q = static_cast<float>(as_f16x2(xb[j >> 1])[j & 1]);
+                    ra[j] = static_cast<float>(fma(p, cs[j], -(q * sn[j])));
+                    rb[j] = static_cast<float>(fma(q, cs[j], p * sn[j]));
+                }
+                v = Quads{u32x2{pack_f16x2(ra[0], ra[1]), pack_f16x2(ra[2], ra[3])},
+                          u32x2{pack_f16x2(rb[0], rb[1]), pack_f16x2(rb[2], rb[3])}};
             }
-            x = u32x4{rw[0], rw[1], rw[2], rw[3]};
-            if (is_q) {
-                if (found)
-                    stg(reinterpret_cast<u32x4*>(a.q_out + (static_cast<int64_t>(t) * a.NQ + h) * HD) + o, x);
-                continue;
+            uint16_t* out = is_q ? a.q_out + (static_cast<int64_t>(t) * a.NQ + h) * HD
+                                 : a.k_out ? a.k_out + (static_cast<int64_t>(t) * c.NKV + h - a.NQ) * HD : nullptr;
+            if (out && found) {
+                stg(reinterpret_cast<u32x2*>(out + 4 * o), v.x);
+                stg(reinterpret_cast<u32x2*>(out + H2 + 4 * o), v.y);
             }
-            if (a.k_out && found)
-                stg(reinterpret_cast<u32x4*>(a.k_out + (static_cast<int64_t>(t) * c.NKV + h - a.NQ) * HD) + o, x);
+            if (is_q) continue;
         }
-        uint32_t q[8];
-        const uint16_t s = kv4_quantize<GS>(x, q);
+        uint32_t codes;
+        const uint32_t s = kv4_quantize<HD, GS>(v, codes);
         const int kvh = h - a.NQ - (is_v ? c.NKV : 0);
         const int64_t head = static_cast<int64_t>(keep ? id : 0) * c.NKV + kvh;
         if (!is_v) {
-            uint32_t word = 0;
-            constexpr int order[8] = {0, 2, 4, 6, 1, 3, 5, 7};
-#pragma unroll
-            for (int n = 0; n < 8; ++n) word |= q[order[n]] << (4 * n);
+            // a quad in AWQ order is nibbles 0, 4, 1, 5 of the word's bytes 0, 2; an octet's second quad is a byte further.
+            // Even lanes take x's octet (their quad and the next lane's), odd lanes y's
+            auto awq = [](uint32_t b) { return (b & 0xfu) | (b >> 16 & 0xfu) << 4 | (b >> 8 & 0xfu) << 16 | (b >> 24) << 20; };
+            const uint32_t qx = awq(codes & 0x0f0f0f0fu), qy = awq(codes >> 4 & 0x0f0f0f0fu);
+            const uint32_t other = dpp_u<0xb1>(o & 1 ? qx : qy);
+            const uint32_t word = o & 1 ? other | qy << 8 : qx | other << 8;
+            const int oct = (o >> 1) + (o & 1 ? HD / 16 : 0);
             if (keep)
-                stg(reinterpret_cast<uint32_t*>(c.k_pages + (head * c.page + slot) * (HD / 2)) + W * (o & 3) + (o >> 2),
+                stg(reinterpret_cast<uint32_t*>(c.k_pages + (head * c.page + slot) * (HD / 2)) + W * (oct & 3) + (oct >> 2),
                     word);
         } else {
-            // lane o = 8 u + 2 n + e holds dimensions 64 u + 16 n + 8 e + j, j < 8; unit (m = 8 e + j, u) wants its
-            // nibbles n = 0 .. 3 from the four lanes of one (u, e): a 4 x 4 transpose of nibble pairs (j, j + 4)
-            uint32_t v = 0;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v |= (q[j] | (q[j + 4] << 4)) << (8 * j);  // byte j: dimensions j, j + 4
-            {
-                const uint32_t p = dpp_u<0x4e>(v);  // lane ^ 2: n ^ 1
-                v = (o & 2) ? (v & 0xff00ff00u) | ((p >> 8) & 0x00ff00ffu) : (v & 0x00ff00ffu) | ((p & 0x00ff00ffu) << 8);
-                const uint32_t r = xor_u<4>(v);     // lane ^ 4: n ^ 2
-                v = (o & 4) ? (v & 0xffff0000u) | (r >> 16) : (v & 0x0000ffffu) | (r << 16);
+            uint32_t va, vb;  // units of 16 bits: two a lane
+            int ma, ua, ub;
+            if constexpr (HD == 64) {
+                // x is nibbles n = 0, 1 (o >> 2), y is n = 2, 3; the lane pair o, o ^ 4 shares units m = 4 (o & 3) + 0 .. 3
+                const uint32_t p = xor_u<4>(codes);
+                const bool hi = o & 4;
+                const uint32_t l0 = hi ? p : codes, l1 = hi ? codes : p;      // from the lanes of n = 0 and 1
+                auto unit = [&](int j) {
+                    const uint32_t a0 = l0 >> (8 * j), a1 = l1 >> (8 * j);
+                    return (a0 & 0xfu) | (a1 & 0xfu) << 4 | (a0 & 0xf0u) << 4 | (a1 & 0xf0u) << 8;
+                };
+                va = hi ? unit(2) : unit(0);
+                vb = hi ? unit(3) : unit(1);
+                ma = 4 * (o & 3) + (hi ? 2 : 0);
+                ua = 0;
+                ub = 0;
+            } else {
+                // x is nibble n = (o >> 2) & 3 of units m = 4 (o & 3) + j, u = o >> 4, y the same of u + hd / 128: a 4 x 4
+                // transpose of the code bytes over the lanes of one o & 3, whose bits 2 and 3 are n
+                uint32_t w = codes;
+                const uint32_t p = xor_u<4>(w);
+                w = (o & 4) ? (w & 0xff00ff00u) | (p >> 8 & 0x00ff00ffu) : (w & 0x00ff00ffu) | (p & 0x00ff00ffu) << 8;
+                const uint32_t r = xor_u<8>(w);
+                w = (o & 8) ? (w & 0xffff0000u) | r >> 16 : (w & 0x0000ffffu) | r << 16;
+                va = squeeze4(w & 0x0f0f0f0fu);
+                vb = squeeze4(w >> 4 & 0x0f0f0f0fu);
+                ma = 4 * (o & 3) + (o >> 2 & 3);
+                ua = o >> 4;
+                ub = ua + HD / 128;
             }
-            // now byte n' of lane (u, n, e) is byte n of lane (u, n', e): dimensions n and n + 4 of nibble n'
-            const uint32_t lo = v & 0x0f0f0f0fu, hi = (v >> 4) & 0x0f0f0f0fu;
-            auto squeeze = [](uint32_t b4) {  // four nibbles in bytes -> 16 bits
-                b4 = (b4 | (b4 >> 4)) & 0x00ff00ffu;
-                return static_cast<uint16_t>(b4 | (b4 >> 8));
-            };
-            const int u = o >> 3, m = 8 * (o & 1) + ((o >> 1) & 3);
-            uint16_t* units = reinterpret_cast<uint16_t*>(c.v_pages + head * c.page * (HD / 2));
             if (keep) {
-                const int64_t at = (static_cast<int64_t>((slot >> 2) * 16 + m) * (HD / 64) + u) * 4 + (slot & 3);
-                stg(units + at, squeeze(lo));
-                stg(units + at + 4 * (HD / 64) * 4, squeeze(hi));  // unit m + 4
+                uint16_t* units = reinterpret_cast<uint16_t*>(c.v_pages + head * c.page * (HD / 2)) +
+                                  static_cast<int64_t>(slot >> 2) * (16 * (HD / 64) * 4) + (slot & 3);
+                stg(units + (ma * (HD / 64) + ua) * 4, static_cast<uint16_t>(va));
+                stg(units + ((ma + (HD == 64 ? 1 : 0)) * (HD / 64) + ub) * 4, static_cast<uint16_t>(vb));
             }
         }
-        if (keep && o % (GS / 8) == 0)
-            stg((is_v ? c.v_scale : c.k_scale) + (head * (HD / GS) + o / (GS / 8)) * c.page + slot, s);
+        // the scales: the first lane of each group of x, and of y where that is another group
+        if (keep && o % (GS / 4 < LPT ? GS / 4 : LPT) == 0) {
+            uint16_t* sp = (is_v ? c.v_scale : c.k_scale) + head * (HD / GS) * c.page + slot;
+            const int gx = 4 * o / GS;
+            stg(sp + gx * c.page, static_cast<uint16_t>(s));
+            if (GS <= H2) stg(sp + (gx + H2 / GS) * c.page, static_cast<uint16_t>(s >> 16));
+        }
     }
 }
 
-// The cached rows of packed tokens as binary16, k_out and v_out [T, NKV, hd]: the same lanes as the append. A value is
-// one rounding of code x scale. Tokens whose position has no page read as zeros.
-template <int HD, int GS>
+// The cached rows of packed tokens as binary16, k_out and v_out [T, NKV, hd]. Lane o of a token's hd / 8 takes dimensions
+// 8 o .. + 7: one K word, and two V units that the four lanes of one (o & 1, o >> 3) transpose between them. A value is
+// one rounding of code x scale. Tokens whose position has no page read as zeros. kHeads heads' loads go out together:
+// a head is 12 bytes a lane, too few to cover the latency alone.
+template <int HD, int GS, int kHeads>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const int32_t* __restrict__ cu, const Kv4Cache c,
                                                        uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int T,
                                                        int heads_per_wave) {
     constexpr int LPT = HD / 8, TPW = kWave / LPT, W = HD / 32;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o = lane % LPT, i = lane / LPT;
     const int t0 = static_cast<int>(blockIdx.x) * TPW, t = t0 + i;
     const int h0 = (static_cast<int>(blockIdx.y) * 4 + wave) * heads_per_wave;
     if (h0 >= c.NKV) return;  // wave-uniform
+    const int h1 = min(c.NKV, h0 + heads_per_wave);
     int b, pos;
     const bool found = kv4_locate<TPW>(cu, c.lens, c.B, t0, i, lane, b, pos) && t < T;
     const int id = found ? kv4_page(c, b, pos) : -1;
     const int slot = id >= 0 ? pos & (c.page - 1) : 0;
-    for (int h = h0; h < h0 + heads_per_wave && h < c.NKV; ++h) {
-        const int64_t head = static_cast<int64_t>(id >= 0 ? id : 0) * c.NKV + h;
-        const int64_t srow = (head * (HD / GS) + o / (GS / 8)) * c.page + slot;
-        const uint32_t kw = ldg(reinterpret_cast<const uint32_t*>(c.k_pages + (head * c.page + slot) * (HD / 2)) +
-                                W * (o & 3) + (o >> 2));
-        const uint16_t* units = reinterpret_cast<const uint16_t*>(c.v_pages + head * c.page * (HD / 2));
-        const int u = o >> 3, n = (o >> 1) & 3, m0 = 8 * (o & 1);
-        uint32_t vw = 0;  // AWQ order, so that one unpacking serves both
-        constexpr int place[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+    // lane o = 8 u + 2 n + e: units 8 e + n and 8 e + n + 4 of u hold, for n' = 0 .. 3, dimensions 64 u + 16 n' + 8 e + n
+    // and + 4, which are lane (u, n', e)'s
+    const int e = o & 1, n = o >> 1 & 3, u = o >> 3;
+    const int64_t page0 = static_cast<int64_t>(id >= 0 ? id : 0) * c.NKV;
+    const int64_t k_at = static_cast<int64_t>(slot) * (HD / 2) + 4 * (W * (o & 3) + (o >> 2));
+    const int64_t v_at = static_cast<int64_t>(slot >> 2) * (16 * (HD / 64) * 4) + ((8 * e + n) * (HD / 64) + u) * 4 + (slot & 3);
+    const int64_t s_at = static_cast<int64_t>(8 * o / GS) * c.page + slot;
+    for (int h = h0; h < h1; h += kHeads) {
+        uint32_t kw[kHeads], va[kHeads], vb[kHeads];
+        uint16_t ks[kHeads], vs[kHeads];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t unit =
-                ldg(units + (static_cast<int64_t>((slot >> 2) * 16 + m0 + j) * (HD / 64) + u) * 4 + (slot & 3));
-            vw |= ((unit >> (4 * n)) & 15u) << (4 * place[j]);
+        for (int x = 0; x < kHeads; ++x) {
+            const int64_t head = page0 + (h + x < h1 ? h + x : h);
+            kw[x] = ldg(reinterpret_cast<const uint32_t*>(c.k_pages + head * c.page * (HD / 2) + k_at));
+            const uint16_t* units = reinterpret_cast<const uint16_t*>(c.v_pages + head * c.page * (HD / 2)) + v_at;
+            va[x] = ldg(units);
+            vb[x] = ldg(units + 4 * (HD / 64) * 4);  // unit m + 4
+            ks[x] = ldg(c.k_scale + head * (HD / GS) * c.page + s_at);
+            vs[x] = ldg(c.v_scale + head * (HD / GS) * c.page + s_at);
         }
-        const uint16_t ks = ldg(c.k_scale + srow), vs = ldg(c.v_scale + srow);
-        if (!found) continue;
-        auto put = [&](uint16_t* out, uint32_t word, uint16_t s) {
-            f16x2 v[4];
-            dequant_int4x8_bitfield(word, v);
-            const f16 sh = __builtin_bit_cast(f16, s);
-            u32x4 r;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f16x2 p = v[j] * f16x2{sh, sh};
-                r[j] = id >= 0 ? __builtin_bit_cast(uint32_t, p) : 0u;
-            }
-            stg(reinterpret_cast<u32x4*>(out + (static_cast<int64_t>(t) * c.NKV + h) * HD) + o, r);
-        };
-        put(k_out, kw, ks);
-        put(v_out, vw, vs);
+        for (int x = 0; x < kHeads; ++x) {
+            if (h + x >= h1) break;
+            uint32_t w = stretch4(va[x]) | stretch4(vb[x]) << 4;  // byte n': the two codes of lane (u, n', e)
+            const uint32_t p = dpp_u<0x4e>(w);                    // lane ^ 2: n ^ 1
+            w = (o & 2) ? (w & 0xff00ff00u) | (p >> 8 & 0x00ff00ffu) : (w & 0x00ff00ffu) | (p & 0x00ff00ffu) << 8;
+            const uint32_t r = xor_u<4>(w);                       // lane ^ 4: n ^ 2
+            w = (o & 4) ? (w & 0xffff0000u) | r >> 16 : (w & 0x0000ffffu) | r << 16;
+            // byte j: dimensions j (low nibble) and j + 4; in AWQ order 0, 2, 4, 6, 1, 3, 5, 7
+            const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
+            const uint32_t vw = (lo & 0xfu) | (lo >> 16 & 0xfu) << 4 | (hi & 0xfu) << 8 | (hi >> 16 & 0xfu) << 12 |
+                                (lo >> 8 & 0xfu) << 16 | (lo >> 24) << 20 | (hi >> 8 & 0xfu) << 24 | (hi >> 24) << 28;
+            if (!found) continue;
+            auto put = [&](uint16_t* out, uint32_t word, uint16_t s) {
+                f16x2 v[4];
+                dequant_int4x8_bitfield(word, v);
+                const f16 sh = __builtin_bit_cast(f16, s);
+                u32x4 q;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f16x2 f = v[j] * f16x2{sh, sh};
+                    q[j] = id >= 0 ? __builtin_bit_cast(uint32_t, f) : 0u;
+                }
+                stg(reinterpret_cast<u32x4*>(out + (static_cast<int64_t>(t) * c.NKV + h + x) * HD) + o, q);
+            };
+            put(k_out, kw[x], ks[x]);
+            put(v_out, vw, vs[x]);
+        }
     }
 }
 
@@ -384,8 +476,8 @@ extern "C" int soi_kv4_read(const soi_kv4_cache* cache, const int32_t* cu_seqlen
     const dim3 grid(static_cast<unsigned>(tw), static_cast<unsigned>(ceil_div64(cache->num_kv_heads, 4 * hpw)));
     const Kv4Cache c = kv4_device(cache);
 #define SOI_X(H, G)                                                                                               \
-    hipLaunchKernelGGL((kv4_read_kernel<H, G>), grid, dim3(256), 0, as_stream(stream), cu_seqlens, c, k_out, v_out, \
-                       static_cast<int>(T), hpw)
+    hipLaunchKernelGGL((kv4_read_kernel<H, G, 4>), grid, dim3(256), 0, as_stream(stream), cu_seqlens, c, k_out,   \
+                       v_out, static_cast<int>(T), hpw)
     SOI_KV4_SHAPES(SOI_X);
 #undef SOI_X
     return launch_status(what);

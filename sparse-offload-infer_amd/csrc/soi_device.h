@@ -60,6 +60,12 @@ __device__ __forceinline__ u32x4 ldg_any(const void* p) {
     return *(gT*)(p);
 }
 
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+__device__ __forceinline__ u32x2 ldg_any8(const void* p) {  // 8 bytes, likewise
+    typedef const __attribute__((address_space(1))) u32x2_any gT;
+    return *(gT*)(p);
+}
+
 // A pointer known to be the same in every lane, moved to scalar registers.
 template <class T>
 __device__ __forceinline__ T* uniform_ptr(T* p) {
