@@ -48,6 +48,14 @@ __device__ __forceinline__ bool kv4_locate(const int32_t* cu, const int32_t* len
     return found;
 }
 
+// The token group of a workgroup: workgroups go to the eight XCDs in turn, so an XCD gets one contiguous eighth of the
+// groups, and the lines that neighbouring tokens share (64 tokens' scales of a group, two tokens' K words) meet in one L2.
+__device__ __forceinline__ int kv4_token_group() {
+    const int n = gridDim.x, per = (n + 7) >> 3, full = n & 7 ? n & 7 : 8;  // the first `full` XCDs have `per` workgroups
+    const int x = blockIdx.x & 7, i = static_cast<int>(blockIdx.x) >> 3;
+    return x < full ? x * per + i : full * per + (x - full) * (per - 1) + i;
+}
+
 // Sum over the LPT lanes of a token (8, 16 or 32 neighbours), in every one of them.
 template <int LPT>
 __device__ __forceinline__ double token_sum(double v) {
@@ -145,6 +153,13 @@ __device__ __forceinline__ uint32_t stretch4(uint32_t n) {
     return (n | (n << 4)) & 0x0f0f0f0fu;
 }
 
+// Two binary32 numbers rounded to binary16 by one instruction. (The empty asm keeps the compiler from making one rounding
+// of this one and the conversion from binary64 before it.)
+__device__ __forceinline__ uint32_t round_f16x2(float a, float b) {
+    asm("" : "+v"(a), "+v"(b));
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(a), static_cast<f16>(b)});
+}
+
 struct Kv4AppendArgs {
     const uint16_t* qkv;
     int64_t qkv_stride;
@@ -171,7 +186,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a, 
     constexpr int LPT = HD / 8, TPW = kWave / LPT, W = HD / 32, H2 = HD / 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o = lane % LPT, i = lane / LPT;
-    const int t0 = static_cast<int>(blockIdx.x) * TPW, t = t0 + i;
+    const int t0 = kv4_token_group() * TPW, t = t0 + i;
     const int heads = a.NQ + 2 * c.NKV;
     const int h0 = (static_cast<int>(blockIdx.y) * 4 + wave) * a.heads_per_wave;
     if (h0 >= heads) return;  // wave-uniform
@@ -225,7 +240,7 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a, 
                     const f16x2 p = as_f16x2(e[j]), q = as_f16x2(w[j]);  // element x weight: exact in binary32
                     const float lo = static_cast<float>(p.x) * static_cast<float>(q.x);
                     const float hi = static_cast<float>(p.y) * static_cast<float>(q.y);
-                    r[j] = pack_f16x2(static_cast<float>(lo * inv), static_cast<float>(hi * inv));
+                    r[j] = round_f16x2(static_cast<float>(lo * inv), static_cast<float>(hi * inv));
                 }
                 v = Quads{u32x2{r[0], r[1]}, u32x2{r[2], r[3]}};
             }
@@ -239,8 +254,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a, 
                     ra[j] = static_cast<float>(fma(p, cs[j], -(q * sn[j])));
                     rb[j] = static_cast<float>(fma(q, cs[j], p * sn[j]));
                 }
-                v = Quads{u32x2{pack_f16x2(ra[0], ra[1]), pack_f16x2(ra[2], ra[3])},
-                          u32x2{pack_f16x2(rb[0], rb[1]), pack_f16x2(rb[2], rb[3])}};
+                v = Quads{u32x2{round_f16x2(ra[0], ra[1]), round_f16x2(ra[2], ra[3])},
+                          u32x2{round_f16x2(rb[0], rb[1]), round_f16x2(rb[2], rb[3])}};
             }
             uint16_t* out = is_q ? a.q_out + (static_cast<int64_t>(t) * a.NQ + h) * HD
                                  : a.k_out ? a.k_out + (static_cast<int64_t>(t) * c.NKV + h - a.NQ) * HD : nullptr;
@@ -316,7 +331,8 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(const Kv4AppendArgs a, 
 // The cached rows of packed tokens as binary16, k_out and v_out [T, NKV, hd]. Lane o of a token's hd / 8 takes dimensions
 // 8 o .. + 7: one K word, and two V units that the four lanes of one (o & 1, o >> 3) transpose between them. A value is
 // one rounding of code x scale. Tokens whose position has no page read as zeros. kHeads heads' loads go out together:
-// a head is 12 bytes a lane, too few to cover the latency alone.
+// a head is 12 bytes a lane, too few to cover the latency alone. The rows are stored non-temporally: 66k tokens of 8 heads
+// of 128 (341 MB) take 62 us with it (5.5 TB/s), 82 us without.
 template <int HD, int GS, int kHeads>
 __global__ __launch_bounds__(256) void kv4_read_kernel(const int32_t* __restrict__ cu, const Kv4Cache c,
                                                        uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out, int T,
@@ -324,7 +340,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const int32_t* __restrict
     constexpr int LPT = HD / 8, TPW = kWave / LPT, W = HD / 32;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o = lane % LPT, i = lane / LPT;
-    const int t0 = static_cast<int>(blockIdx.x) * TPW, t = t0 + i;
+    const int t0 = kv4_token_group() * TPW, t = t0 + i;
     const int h0 = (static_cast<int>(blockIdx.y) * 4 + wave) * heads_per_wave;
     if (h0 >= c.NKV) return;  // wave-uniform
     const int h1 = min(c.NKV, h0 + heads_per_wave);
@@ -375,7 +391,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(const int32_t* __restrict
                     const f16x2 f = v[j] * f16x2{sh, sh};
                     q[j] = id >= 0 ? __builtin_bit_cast(uint32_t, f) : 0u;
                 }
-                stg(reinterpret_cast<u32x4*>(out + (static_cast<int64_t>(t) * c.NKV + h + x) * HD) + o, q);
+                stg_stream(reinterpret_cast<u32x4*>(out + (static_cast<int64_t>(t) * c.NKV + h + x) * HD) + o, q);
             };
             put(k_out, kw[x], ks[x]);
             put(v_out, vw, vs[x]);
