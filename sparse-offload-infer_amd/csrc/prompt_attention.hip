@@ -28,6 +28,8 @@ namespace soi {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -160,6 +162,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
     float m = kNegBig, l = 0.0f;
+    uint32_t odd = 0;  // not 0: a value that is not finite was replaced in a tile that not all the wave's queries see in full
 
     // Operand addresses: the lane's part below with bits flipped for the chunk, the row and the buffer added. (They stay
     // out of loop-invariant registers that way: one XOR a read is cheaper than the registers.)
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     // 2^kPaSlack, well inside binary16, and most tiles of a long row rescale nothing
     auto raise = [&](float top) {
         if (ballot(top > m + kPaSlack)) {
-            const float mn = fmaxf(m, top), w = fast_exp2(m - mn);
+            const float mn = top > m + kPaSlack ? top : m, w = fast_exp2(m - mn);  // a row does not depend on its neighbours
             m = mn;
             l *= w;
 #pragma unroll
@@ -222,14 +225,14 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
         meet(std::integral_constant<int, 0>{});
 #pragma unroll
         for (int i = 1; i < NBUF - 1; ++i) load(t0 + i, i);
-        int buf = 0, nbuf = NBUF - 1;
-        for (int t = t0; t < tiles; ++t) {
+        int buf = 0, nbuf = NBUF - 1, t = t0;
+        auto tile = [&](auto MASKED) {
             if (t > t0) meet(std::integral_constant<int, (NBUF - 2) * 2 * LOADS>{});
             load(t + NBUF - 1, nbuf);
             const int cur = buf;
             buf = buf + 1 == NBUF ? 0 : buf + 1;
             nbuf = nbuf + 1 == NBUF ? 0 : nbuf + 1;
-            if (t >= wtiles) continue;  // wave-uniform: nothing of this tile is seen here
+            if (MASKED && t >= wtiles) return;  // wave-uniform: nothing of this tile is seen here
             f32x16 z[NT];
             const uint32_t ka = k_at + cur * 2 * TILEB;
 #pragma unroll
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
                     z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const lds_f16x8*)((lds_u8*)(ka ^ (kk << 5)) + i * 32 * ROWB),
                                                                   qf[kk], z[i], 0, 0, 0);
             }
-            if (t >= whole) mask(z, t);
+            if (MASKED) mask(z, t);
             raise(highest(z));
             f16x8 pb[NJ];
 #pragma unroll
@@ -260,18 +263,39 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    s16x4 w[2];
+                    s16x4 r[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x)
-                        w[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        r[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                             (lds_s16x4*)((lds_u8*)(va ^ (d << 6 | x << 5)) + (16 * j + 8 * x) * ROWB));
-                    const f16x8 v8 = __builtin_bit_cast(
-                        f16x8, __builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pb[j], acc[d], 0, 0, 0);
+                    s16x8 v = __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    if (MASKED) {
+                        // A weight of 0 does not hide an infinity or NaN (bits from 0x7c00 and from 0xfc00 up): the products
+                        // take the largest finite number for it, and the queries that do see it get it added at the end.
+                        const u16x8 lo = __builtin_elementwise_min(__builtin_bit_cast(u16x8, v), (u16x8)(uint16_t)0xfbff);
+                        const s16x8 f = __builtin_elementwise_min(__builtin_bit_cast(s16x8, lo), (s16x8)(short)0x7bff);
+                        const u32x4 was = __builtin_bit_cast(u32x4, v), is = __builtin_bit_cast(u32x4, f), x = was ^ is;
+                        odd |= (x.x | x.y) | (x.z | x.w);
+                        v = f;
+                    }
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pb[j], acc[d], 0, 0, 0);
                 }
-        }
+        };
+        for (; t < min(whole, tiles); ++t) tile(std::false_type{});
+        for (; t < tiles; ++t) tile(std::true_type{});
     }
+    const bool patch = ballot(odd != 0) != 0;
     l += xor_lanes<32>(l);
+    // adds the values left out to the queries that see them: add(r, d, v) for each key, the wave's query r, dimension d
+    auto patched = [&](int d0, int d1, auto add) {
+        const int first = max(whole, t0) * kPaKeys, end = min(nk, tiles * kPaKeys);
+        for (int key = first; key < end; ++key)
+            for (int d = d0 + lane; d < min(d1, a.hd); d += kWave) {
+                const uint16_t v = ldg(vb + key * a.v_ts + d);
+                if ((v & 0x7fff) >= 0x7c00)
+                    for (int r = max(0, key - off - wq0); r < 32; ++r) add(r, d, f16_bits_to_f32(v));
+            }
+    };
     if (w.tiles > per) {  // a split row: its state as it is, 64 dimensions at a time through LDS
         lds_u8* so = (lds_u8*)(lds0 + wave * 32 * 256);
         float* pb = a.part + (static_cast<int64_t>(split) * a.Tq + q_lo + wq0) * a.NQ * a.hd + head * a.hd;
@@ -285,6 +309,12 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
                 *(__attribute__((address_space(3))) f32x4*)(so + n * 256 + (((2 * x + hh) ^ (n & 15)) << 4)) =
                     f32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
             }
+            if (patch)
+                patched(32 * d, 32 * d + 64, [&](int r, int dim, float v) {
+                    const int c = (dim - 32 * d) >> 2;
+                    auto* x = (__attribute__((address_space(3))) float*)(so + r * 256 + ((c ^ (r & 15)) << 4) + 4 * (dim & 3));
+                    *x += v;
+                });
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int r = 4 * i + (lane >> 4), c = lane & 15;
@@ -311,6 +341,12 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             *(__attribute__((address_space(3))) u32x2*)(so + n * ROWB + (((4 * d + x) ^ pa_swz_k<HD>(n)) << 4) + 8 * hh) =
                 u32x2{pack_f16x2(acc[d][4 * x] * inv, acc[d][4 * x + 1] * inv),
                       pack_f16x2(acc[d][4 * x + 2] * inv, acc[d][4 * x + 3] * inv)};
+    if (patch)
+        patched(0, HD, [&](int r, int dim, float v) {
+            auto* x = (__attribute__((address_space(3))) uint16_t*)(so + r * ROWB + (((dim >> 3) ^ pa_swz_k<HD>(r)) << 4) +
+                                                                    2 * (dim & 7));
+            *x = f32_to_f16_bits(f16_bits_to_f32(*x) + v);
+        });
     uint16_t* ob = a.out + head * a.o_hs;
 #pragma unroll
     for (int i = 0; i < 32 * ROWB / 1024; ++i) {

@@ -92,6 +92,34 @@ def test_strided_views_and_output(cuda):
     assert (out[:, 1::2] == 7).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_values_that_are_not_finite_reach_their_queries_only(cuda, hd):
+    """An infinity or NaN in k or v is seen from its own position on; before it, and in the other sequence, every output
+    is what it would be without it."""
+    import soinfer.ops as ops
+
+    n = [200, 90]
+    q, k, v, cu, _ = problem(cuda, n, n, 4, 2, hd, 13)
+    want = ops.prompt_attention(q, k, v, cu, cu, 200)
+    for at, dim, bad in ((150, 5, math.inf), (150, hd - 1, -math.inf), (131, 33, math.nan), (199, 0, math.nan), (0, 1, math.inf)):
+        v2 = v.clone()
+        v2[at, 1, dim] = bad
+        got = ops.prompt_attention(q, k, v2, cu, cu, 200)
+        assert torch.equal(got[:at], want[:at]) and torch.equal(got[200:], want[200:]) and torch.equal(got[:, :2], want[:, :2])
+        seen = got[at:200, 2:, dim].float()
+        assert torch.isnan(seen).all() if math.isnan(bad) else ((seen == bad) | torch.isnan(seen)).all(), (at, bad)
+        other = torch.arange(hd, device=cuda) != dim
+        assert torch.equal(got[at:200, 2:, other], want[at:200, 2:, other])
+        k2 = k.clone()
+        k2[at, 1, dim] = bad
+        got = ops.prompt_attention(q, k2, v, cu, cu, 200)
+        assert torch.equal(got[:at], want[:at]) and torch.equal(got[200:], want[200:]) and torch.equal(got[:, :2], want[:, :2])
+    v2 = v.clone()
+    v2[140, 0, 7], v2[160, 0, 7] = math.inf, -math.inf
+    got = ops.prompt_attention(q, k, v2, cu, cu, 200)
+    assert torch.equal(got[:140], want[:140]) and torch.isnan(got[160:200, :2, 7]).all()
+
+
 def test_rows_behind_the_last_sequence_stay(cuda):
     import soinfer.ops as ops
 
