@@ -84,11 +84,11 @@ __device__ __forceinline__ int pa_swz_v(int row) {
 // asm because the compiler, which cannot tell the two buffers apart, would let every LDS read wait for the loads in
 // flight (the kernel waits for them itself, at the barrier; no register is written). m0 holds the LDS address.
 template <int LOADS>
-__device__ __forceinline__ void pa_load(const uint16_t* base, int64_t bytes, const uint32_t (&off)[LOADS], uint32_t lds) {
+__device__ __forceinline__ void pa_load(const uint16_t* base, int bytes, const uint32_t (&off)[LOADS], uint32_t lds) {
     const uint64_t p = reinterpret_cast<uint64_t>(base);
     const u32x4 r = {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p))),
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(p >> 32))) & 0xffffu,
-                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00027000u};
+                     static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00027000u};
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
         asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + i * 1024),
@@ -149,11 +149,18 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     const uint16_t* vb = a.v + k_lo * a.v_ts + kvh * a.v_hs;
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)&s_kv[0][0][0]));
     const uint32_t lds = lds0 + wave * LOADS * 1024;
-    auto load = [&](int tile, int buf) {
-        const int key = tile * kPaKeys, rows = min(nk - key, kPaKeys);
-        const int64_t kn = rows > 0 ? ((rows - 1) * a.k_ts + a.hd) * 2 : 0, vn = rows > 0 ? ((rows - 1) * a.v_ts + a.hd) * 2 : 0;
-        pa_load<LOADS>(kb + key * a.k_ts, kn, ko, lds + 2 * buf * TILEB);
-        pa_load<LOADS>(vb + key * a.v_ts, vn, vof, lds + (2 * buf + 1) * TILEB);
+    // the next tile to load: its first key's rows, the keys from there on, its buffer (tiles are loaded in order)
+    const int kspan = static_cast<int>(a.k_ts) * 2, vspan = static_cast<int>(a.v_ts) * 2, hd2 = a.hd * 2;  // bytes
+    const uint16_t *k_next = kb + static_cast<int64_t>(t0) * KT * a.k_ts, *v_next = vb + static_cast<int64_t>(t0) * KT * a.v_ts;
+    int left = nk - t0 * KT, into = 0;
+    auto load = [&] {
+        const int rows = min(left, KT) - 1;
+        pa_load<LOADS>(k_next, rows < 0 ? 0 : rows * kspan + hd2, ko, lds + into);
+        pa_load<LOADS>(v_next, rows < 0 ? 0 : rows * vspan + hd2, vof, lds + into + TILEB);
+        k_next += KT * a.k_ts;
+        v_next += KT * a.v_ts;
+        left -= KT;
+        into = into == (NBUF - 1) * 2 * TILEB ? 0 : into + 2 * TILEB;
     };
 
     f32x16 acc[DT];
@@ -214,9 +221,9 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
         asm volatile("" ::: "memory");
     };
     if (t0 < tiles) {  // (workgroup-uniform)
-        pa_load<QLOADS>(a.q + (q_lo + q0) * a.q_ts + head * a.q_hs, ((min(nq - q0, QROWS) - 1) * a.q_ts + a.hd) * 2, qo,
+        pa_load<QLOADS>(a.q + (q_lo + q0) * a.q_ts + head * a.q_hs, static_cast<int>(((min(nq - q0, QROWS) - 1) * a.q_ts + a.hd) * 2), qo,
                         lds0 + 2 * TILEB + wave * QLOADS * 1024);
-        load(t0, 0);
+        load();
         meet(std::integral_constant<int, 0>{});
         f16x8 qf[KK];
 #pragma unroll
@@ -224,26 +231,42 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             qf[kk] = *(const lds_f16x8*)((lds_u8*)((k_at + 2 * TILEB + 32 * wave * ROWB) ^ (kk << 5)));
         meet(std::integral_constant<int, 0>{});
 #pragma unroll
-        for (int i = 1; i < NBUF - 1; ++i) load(t0 + i, i);
-        int buf = 0, nbuf = NBUF - 1, t = t0;
+        for (int i = 1; i < NBUF - 1; ++i) load();
+        int at = 0, t = t0;  // LDS offset of tile t
         auto tile = [&](auto MASKED) {
             if (t > t0) meet(std::integral_constant<int, (NBUF - 2) * 2 * LOADS>{});
-            load(t + NBUF - 1, nbuf);
-            const int cur = buf;
-            buf = buf + 1 == NBUF ? 0 : buf + 1;
-            nbuf = nbuf + 1 == NBUF ? 0 : nbuf + 1;
+            load();
+            const int cur = at;
+            at = at == (NBUF - 1) * 2 * TILEB ? 0 : at + 2 * TILEB;
             if (MASKED && t >= wtiles) return;  // wave-uniform: nothing of this tile is seen here
             f32x16 z[NT];
-            const uint32_t ka = k_at + cur * 2 * TILEB;
+            const uint32_t ka = k_at + cur, va = v_at + cur;
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
+                f16x8 kf[KK];
+#pragma unroll
+                for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const lds_f16x8*)((lds_u8*)(ka ^ (kk << 5)) + i * 32 * ROWB);
+                if (KK <= 8) __builtin_amdgcn_sched_barrier(0);  // all reads first: a product waits for its own only
 #pragma unroll
                 for (int r = 0; r < 16; ++r) z[i][r] = 0.0f;
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk)
-                    z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const lds_f16x8*)((lds_u8*)(ka ^ (kk << 5)) + i * 32 * ROWB),
-                                                                  qf[kk], z[i], 0, 0, 0);
+                for (int kk = 0; kk < KK; ++kk) z[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[kk], qf[kk], z[i], 0, 0, 0);
             }
+            auto v_read = [&](int d, int j) {
+                s16x4 r[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    r[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s16x4*)((lds_u8*)(va ^ (d << 6 | x << 5)) + (16 * j + 8 * x) * ROWB));
+                return (s16x8)__builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+            s16x8 vf[2][NJ];  // V of two dimension tiles, one in use and one on its way
+            auto v_fetch = [&](int d) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) vf[d & 1][j] = v_read(d, j);
+            };
+            v_fetch(0);
+            __builtin_amdgcn_sched_barrier(0);  // (requested before the softmax, which they do not wait for)
             if (MASKED) mask(z, t);
             raise(highest(z));
             f16x8 pb[NJ];
@@ -258,17 +281,12 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
 #pragma unroll
                 for (int e = 0; e < 8; e += 2)
                     l = dot2(f16x2{pb[j][e], pb[j][e + 1]}, f16x2{(f16)1.0f, (f16)1.0f}, l);
-            const uint32_t va = v_at + cur * 2 * TILEB;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
+            for (int d = 0; d < DT; ++d) {
+                if (d + 1 < DT) v_fetch(d + 1);
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) {
-                    s16x4 r[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        r[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s16x4*)((lds_u8*)(va ^ (d << 6 | x << 5)) + (16 * j + 8 * x) * ROWB));
-                    s16x8 v = __builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    s16x8 v = vf[d & 1][j];
                     if (MASKED) {
                         // A weight of 0 does not hide an infinity or NaN (bits from 0x7c00 and from 0xfc00 up): the products
                         // take the largest finite number for it, and the queries that do see it get it added at the end.
@@ -280,6 +298,8 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
                     }
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v), pb[j], acc[d], 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         };
         for (; t < min(whole, tiles); ++t) tile(std::false_type{});
         for (; t < tiles; ++t) tile(std::true_type{});
@@ -455,10 +475,10 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
     SOI_REQUIRE(scale > 0.0f && scale < __builtin_inff(), "%s: scale must be positive and finite", what);
     if (Tq == 0 || max_q == 0) return SOI_OK;
     SOI_REQUIRE(q && out && cu_q && cu_k && (Tk == 0 || (k && v)), "%s: null pointer", what);
-    SOI_REQUIRE(k_token_stride >= 0 && k_token_stride < (int64_t(1) << 24) && v_token_stride >= 0 &&
-                    v_token_stride < (int64_t(1) << 24),
-                "%s: key and value rows must be less than 2^24 elements apart", what);
-    SOI_REQUIRE(q_token_stride >= 0 && q_token_stride < (int64_t(1) << 24), "%s: query rows must be less than 2^24 elements apart",
+    SOI_REQUIRE(k_token_stride >= 0 && k_token_stride < (int64_t(1) << 22) && v_token_stride >= 0 &&
+                    v_token_stride < (int64_t(1) << 22),
+                "%s: key and value rows must be less than 2^22 elements apart", what);
+    SOI_REQUIRE(q_token_stride >= 0 && q_token_stride < (int64_t(1) << 22), "%s: query rows must be less than 2^22 elements apart",
                 what);
     SOI_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && q_token_stride % 8 == 0 &&
                     q_head_stride % 8 == 0 && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
