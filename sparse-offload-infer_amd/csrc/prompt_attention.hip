@@ -434,13 +434,15 @@ __global__ __launch_bounds__(256) void prompt_combine_kernel(const PaArgs a, int
 
 constexpr int kPaWaves = 4;
 
-// Splits of a row's keys: where the queries alone make fewer workgroups than two to a CU (one at head_dim over 128, which
-// is what fits there), enough for that. Every split writes and reads hd + 2 floats a query: with 256 / 512 / 768 / 1024
-// workgroups aimed at, 512 queries over 16896 keys, 16 heads of 128, took 123 / 93 / 94 / 105 us, 2048 queries of 8 heads
-// 40 / 31 / 31 / 40 us; 300 queries x 2 over 3300 keys, 14 heads of 256, 67 us with 256 and 98 with 512.
+// Splits of a row's keys: where the queries alone make fewer workgroups than 1024 (head_dim up to 64), 512 (up to 128) or
+// 256 (above), enough for that. Four, three and one workgroup fit on a CU; every split writes and reads hd + 2 floats a
+// query. Measured with 512 / 768 / 1024 / 1536 workgroups aimed at: five ragged parts of up to 513 queries behind up to
+// 4000 keys, 14 heads of 64, 70 / 62 / 57 / 58 us, 1024 queries over 17408 keys, 8 heads of 64, 58 / 57 / 58 / 64 us. With
+// 256 / 512 / 768 / 1024: 512 queries over 16896 keys, 16 heads of 128, 123 / 93 / 94 / 105 us, 2048 queries of 8 heads of
+// 128, 40 / 31 / 31 / 40 us. 300 queries x 2 over 3300 keys, 14 heads of 256, 67 us with 256 and 98 with 512.
 static int64_t pa_nsplit(int64_t Tq, int64_t Tk, int64_t NQ, int64_t hd, int64_t KT) {
     const int64_t groups = NQ * ceil_div64(Tq, 32 * kPaWaves), most = ceil_div64(ceil_div64(Tk, KT), kPaSplitTiles);
-    int64_t n = (hd > 128 ? 256 : 512) / groups;
+    int64_t n = (hd > 128 ? 256 : hd > 64 ? 512 : 1024) / groups;
     n = n < most ? n : most;
     return n < 1 ? 1 : n > kPaMaxSplits ? kPaMaxSplits : n;
 }
