@@ -780,7 +780,8 @@ typedef struct soi_kv4_cache {
  * none for no norm), RoPE from tables [table_rows, head_dim / 2], each rounded to binary32 and then binary16; q to q_out
  * [T, NQ, head_dim], k also to k_out [T, NKV, head_dim] if given, k and v quantized into the cache. Norm and rotation
  * are evaluated in binary64, so the codes follow from the inputs alone. A position past the tables or the cache
- * appends nothing and rotates by the last table row. */
+ * appends nothing and rotates by the last table row. T is at most (2^24 - 1) * 512 / head_dim, here and in
+ * soi_kv4_read. */
 int soi_kv4_append(const soi_kv4_cache* cache, const uint16_t* qkv, int64_t qkv_stride, const uint16_t* q_norm,
                    const uint16_t* k_norm, const float* cos_table, const float* sin_table, int64_t table_rows,
                    const int32_t* cu_seqlens, int64_t T, int64_t num_q_heads, uint16_t* q_out, uint16_t* k_out, float eps,
@@ -789,8 +790,9 @@ int soi_kv4_append(const soi_kv4_cache* cache, const uint16_t* qkv, int64_t qkv_
 int soi_kv4_read(const soi_kv4_cache* cache, const int32_t* cu_seqlens, int64_t T, uint16_t* k_out, uint16_t* v_out,
                  void* stream);
 /* out [batch, NQ, head_dim]: attention of one query token per sequence (q rows q_stride elements apart) over its
- * min(seq_lens[b], max_len) cached tokens; query head h reads KV head h / (NQ / NKV); zeros for an empty context; scale positive. The
- * workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
+ * min(seq_lens[b], max_len) cached tokens; query head h reads KV head h / (NQ / NKV); zeros for an empty context; scale
+ * positive. Contexts are split by the blocks of all sequences together, so the last bits of one can change with the lengths
+ * of the others; the same call gives the same bits. The workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
  * stream; calls that overlap need one each. */
 size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
                                                 int64_t head_dim, int64_t max_len);
@@ -800,7 +802,8 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
 /* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
  * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
  * one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
- * bytes, out 8-byte; scale positive. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
+ * bytes and rows less than 2^22 elements apart, out 8-byte and not in q's memory; scale positive. A value that is not
+ * finite reaches the queries that see its key and no others. Where the keys are split, it follows from Tq, Tk and NQ. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
  * aligned, needs no initial value and may be reused by the next call on the stream; calls that overlap need one each. */
 size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim);
 int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,

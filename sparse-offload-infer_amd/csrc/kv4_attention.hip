@@ -24,6 +24,14 @@
 // none across two sequences, bps following from the sum of the lengths on the device. Workgroup (head, y) finds split y
 // by a scan over the sequences. A sequence of one split is written at once; the states of more are combined in split
 // order by a second launch.
+//
+// Measured: 4 contexts of up to 131072 tokens (386002 in all), 64 / 8 heads of 128, groups of 64 (420 MB): 84 us, 5.0 TB/s,
+// what a large copy reaches on this card. 48 contexts of 1870 tokens on average, 32 / 8 heads, groups of 32, pages of 16
+// (104 MB): 34 us, 30.5 of them the first launch (3.4 TB/s: a page is 1 KB of K here, each wave waits for its table entries,
+// and the nibbles' arithmetic is most of a block's time); one context of 2000: 8.6 us, two dependent launches of 5.4 and
+// 3.6 us.
+// Registers, not LDS, set the workgroups of a CU (4 / 3 / 2 for 64 / 128 / 256 dimensions); K and V registers are loaded
+// again as soon as their products are issued, so that a block's loads are in flight during the rest of the block before.
 #include "soi_host.h"
 #include "soi_kv4.h"
 #include "soi_attn.h"

@@ -82,6 +82,15 @@ def test_call_checks(lib):
     assert st == 2 and "workspace" in error(lib, st)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_more_tokens_than_one_launch(lib, hd):
+    """512 / hd tokens a workgroup of 256, and a grid holds fewer than 2^32 work items."""
+    c = C.byref(cache(head_dim=hd, group_size=32))
+    T = ((1 << 24) - 1) * (512 // hd) + 1
+    assert "tokens" in error(lib, lib.soi_kv4_append(c, 16, 8 * hd, None, None, 16, 16, 4, 16, T, 4, 16, None, 1e-6, None))
+    assert "tokens" in error(lib, lib.soi_kv4_read(c, 16, T, 16, 32, None))
+
+
 def test_workspace_query(lib):
     q = lib.soi_kv4_decode_attention_workspace_bytes
     assert q(1, 4, 2, 128, 64) == 0 and q(1, 4, 2, 128, 0) == 0  # one split: none

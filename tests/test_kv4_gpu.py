@@ -339,6 +339,63 @@ def test_attention_in_graphs_with_one_workspace(cuda):
             assert torch.equal(out[i], ops.kv4_decode_attention(q[i], *c, table, lt, max_len=512))
 
 
+def test_pages_past_4_gib(cuda):
+    """A cache whose K and V pages are 4.6 GB each: the same bytes and bits from its last pages as from a small one's."""
+    import soinfer.ops as ops
+
+    NQ, NKV, hd, gs, page, news = 8, 8, 128, 64, 64, [150, 1, 70]
+    table, few = table_of(news, page, 3, extra=0)
+    P = 140000
+    up = lambda x: torch.from_numpy(x).to(cuda)  # noqa: E731
+    p = append_problem(cuda, [0, 0, 0], news, NQ, NKV, hd, gs, page, True, 3)
+    lens, cu = up(p["lens"]), up(p["cu"])
+
+    def run(pages, at):
+        c = [torch.empty((pages, NKV, page, hd // 2), dtype=torch.uint8, device=cuda),
+             torch.empty((pages, NKV, hd // gs, page), dtype=torch.float16, device=cuda),
+             torch.empty((pages, NKV, page, hd // 2), dtype=torch.uint8, device=cuda),
+             torch.empty((pages, NKV, hd // gs, page), dtype=torch.float16, device=cuda)]
+        for x in c:
+            x[at:at + few].fill_(7)
+        t = up(np.where(table < 0, -1, table + at).astype(np.int32))
+        q = ops.kv4_append(up(p["qkv"]), up(p["w"][0]), up(p["w"][1]), up(p["cos"]), up(p["sin"]), *c, t, lens, cu, NQ)
+        return [q, *ops.kv4_read(*c, t, lens, cu, sum(news)),
+                ops.kv4_decode_attention(q[cu[1:].long() - 1], *c, t, lens, max_len=150), *(x[at:at + few].clone() for x in c)]
+
+    for got, want in zip(run(P, P - few), run(few, 0)):
+        R.same(got, want.cpu().numpy(), "far pages")
+
+
+def test_on_two_streams_at_once(cuda):
+    """Calls that overlap on two streams, each with its own workspace, give what they give alone."""
+    import soinfer.ops as ops
+
+    c, table, lt, held = filled(cuda, [900, 40, 300], 2, 128, 64, 64, 10)
+    q = [queries(cuda, 3, 8, 128, s) for s in (1, 2)]
+    want = [ops.kv4_decode_attention(x, *c, table, lt, max_len=900) for x in q]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.kv4_decode_attention(q[i], *c, table, lt, max_len=900))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_two_sequences_of_the_same_pages(cuda):
+    """A shared beginning: two sequences name the same pages, and a third ends inside them."""
+    import soinfer.ops as ops
+
+    c, table, lt, held = filled(cuda, [130], 2, 64, 32, 16, 11)
+    table, lt = table.expand(3, -1).contiguous(), torch.tensor([130, 130, 50], dtype=torch.int32, device=cuda)
+    q = queries(cuda, 1, 4, 64, 3).expand(3, -1, -1).contiguous()
+    got = ops.kv4_decode_attention(q, *c, table, lt, max_len=130)
+    check_attention(got, q, [held[0], held[0], [x[:50] for x in held[0]]], "shared pages")
+    assert torch.equal(got[0], got[1])
+
+
 def test_refusals(cuda):
     import soinfer.ops as ops
 

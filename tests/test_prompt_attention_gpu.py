@@ -165,6 +165,64 @@ def test_same_bits_again_and_in_a_graph(cuda):
         assert torch.equal(out, ops.prompt_attention(q, k, v, cu, cu, 300))
 
 
+def test_rows_far_apart(cuda):
+    """Offsets past 4 GiB: rows of q, k, v and out nearly 2^22 elements apart give the bits of contiguous ones."""
+    import soinfer.ops as ops
+
+    n, NQ, NKV, hd, stride = [300, 290], 4, 2, 64, (1 << 22) - 8
+    q, k, v, cu, _ = problem(cuda, n, n, NQ, NKV, hd, 12)
+    want = ops.prompt_attention(q, k, v, cu, cu, 300)
+    base, outs = (torch.empty(sum(n) * stride, dtype=torch.float16, device=cuda) for _ in range(2))
+    far = []
+    for x, b, at in ((q, base, 0), (k, base, 4096), (v, base, 8192), (torch.zeros_like(q), outs, 0)):
+        far.append(b.as_strided(x.shape, (stride, hd, 1), at))
+        far[-1].copy_(x)
+    ops.prompt_attention(*far[:3], cu, cu, 300, out=far[3])
+    assert torch.equal(far[3], want)
+    with pytest.raises(RuntimeError, match="apart"):
+        ops.prompt_attention(q, base.as_strided((500, NKV, hd), (1 << 22, hd, 1)), v[:500], cu, cu, 300)
+
+
+def test_rows_that_overlap(cuda):
+    """One key row and one value row for all positions (stride 0): every query gets that value."""
+    import soinfer.ops as ops
+
+    n = [70]
+    q, k, v, cu, _ = problem(cuda, n, n, 4, 2, 64, 13)
+    k, v = k[:1].expand(70, -1, -1), v[:1].expand(70, -1, -1)
+    check(ops.prompt_attention(q, k, v, cu, cu, 70), q, k, v, n, n, "one row")
+
+
+def test_sequences_that_do_not_start_at_row_0(cuda):
+    """cu starts behind rows of no sequence, which stay as they are, as do those behind the last."""
+    import soinfer.ops as ops
+
+    q, k, v, _, _ = problem(cuda, [100], [110], 4, 2, 128, 14)
+    at = lambda *x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    out = torch.full_like(q, 3.0)
+    ops.prompt_attention(q, k, v, at(10, 40, 40, 90), at(20, 60, 60, 110), 50, out=out)
+    check(out[10:90], q[10:90], k[20:110], v[20:110], [30, 0, 50], [40, 0, 50], "inner rows")
+    assert (out[:10] == 3).all() and (out[90:] == 3).all()
+
+
+def test_on_two_streams_at_once(cuda):
+    """Calls with split keys that overlap on two streams, each with its own workspace, give what they give alone."""
+    import soinfer.ops as ops
+
+    q, k, v, cu_q, cu_k = problem(cuda, [60, 9], [2500, 700], 8, 2, 128, 15)
+    q = [q, q.flip(0).contiguous()]
+    want = [ops.prompt_attention(x, k, v, cu_q, cu_k, 60) for x in q]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.prompt_attention(q[i], k, v, cu_q, cu_k, 60))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
 def test_refusals(cuda):
     import soinfer.ops as ops
 
