@@ -6,8 +6,8 @@
 // a query that sees no key gives zeros. The framework's other prompt attention (prompt.hip) takes one sequence over a
 // contiguous cache in the decode step's order of sums, on v_dot2; this one takes the tile order the matrix cores want.
 //
-// A workgroup of NW waves owns 32 NW queries of one head; a wave owns 32 of them (v_mfma_f32_32x32x16_f16, lane
-// n = lane & 31 is a query, h = lane >> 5):
+// A workgroup of NW waves owns 32 NW queries of one head, or fewer of two or four heads of one KV head; a wave owns 32 of one
+// head (v_mfma_f32_32x32x16_f16, lane n = lane & 31 is a query, h = lane >> 5):
 //   * S^T = K Q^T: lane (n, h) ends with the scores of query n and keys 8 (r >> 2) + 4 h + (r & 3), r < 16, of each
 //     32-key tile: a row's maximum is a lane's own but for one swap with lane + 32;
 //   * O^T = V^T P^T takes these scores, exponentiated, as its B operand as they lie. The k slots of V are then
@@ -22,9 +22,9 @@
 // Bound: 4 hd operations a (query, key, head) on the matrix cores, one exponential each on the vector units (at head_dim
 // 64 both take 512 cycles for 32 x 64 scores). The running sum takes the binary16 weights that the products use, the
 // maximum is a base that is raised only when a score passes it by 8 binades. One sequence of 16384 tokens, 16 / 8 heads of
-// 128: 1.07 ms, 1024 TFLOP/s (at the 1.8 GHz that the power limit leaves; a matrix product of 8192 reaches 1160, or 1360
+// 128: 1.05 ms, 1048 TFLOP/s (at the 1.8 GHz that the power limit leaves; a matrix product of 8192 reaches 1160, or 1360
 // by its kernel alone), matrix units busy 63 % of the cycles, vector units 58 %. Twenty prompts of 1 to 1000 tokens, 32 / 8
-// heads: 102 us.
+// heads: 91 us.
 //
 // Tile, buffers and occupancy, 128 dimensions: 32 keys, three buffers (two tiles in flight), three workgroups to a CU
 // against 64 keys, two buffers, two workgroups: 1.07 / 1.07 ms and 119 / 135 us for the two above, and against 32 keys,
@@ -60,6 +60,7 @@ struct PaArgs {
     const int32_t *cu_q, *cu_k;
     float* part;  // split rows: acc [nsplit][Tq][NQ][hd], then (m, l) [nsplit][Tq][NQ][2]
     int Tq, Tk, NQ, NKV, hd, nsplit;
+    int hshift;  // a workgroup's queries are those of 2^hshift heads of one KV head
     float scale_log2;
 };
 
@@ -131,16 +132,20 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     const int n = lane & 31, hh = lane >> 5;
     // heads of one KV head lie NKV apart in x: with NKV a multiple of 8 they run on one XCD and share its L2
     const int split = static_cast<int>(blockIdx.x) / a.NQ, hx = static_cast<int>(blockIdx.x) % a.NQ;
-    const int kvh = hx % a.NKV, rep = a.NQ / a.NKV;
-    const int head = kvh * rep + hx / a.NKV;
-    const PaRows w(a, blockIdx.y, static_cast<int>(gridDim.z - 1 - blockIdx.z), 32 * NW, KT);  // the longest rows first
+    const int kvh = hx % a.NKV, rep = a.NQ / a.NKV, hmask = (1 << a.hshift) - 1;
+    const int head = kvh * rep + ((hx / a.NKV) & ~hmask) + (wave & hmask);
+    // Neighbours in x have the other parts of the same 32 NW queries, and the longest rows come first. Which neighbour has
+    // which part changes with y and z: workgroups go to the CUs in turn, and the same CUs would get all the long ones.
+    const int part = (hx / a.NKV + static_cast<int>(blockIdx.y + blockIdx.z)) & hmask;
+    const int qtile = static_cast<int>(gridDim.z - 1 - blockIdx.z) << a.hshift | part;
+    const PaRows w(a, blockIdx.y, qtile, 32 * NW >> a.hshift, KT);
     const int q_lo = w.q_lo, nq = w.nq, k_lo = w.k_lo, nk = w.nk, off = w.off, q0 = w.q0;
     if (q0 >= nq) return;
     auto clamp = [](int x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : x; };
     const int per = pa_split_tiles(w.tiles, a.nsplit), t0 = split * per, tiles = min(w.tiles, t0 + per);
     if (split > 0 && t0 >= w.tiles) return;
-    const int wq0 = q0 + 32 * wave;
-    const int last = wq0 + n + off;  // the last key that the lane's query sees
+    const int wq0 = q0 + 32 * (wave >> a.hshift);
+    const int last = wq0 + n + off - 4 * hh;  // the last key that the lane's query sees, less the lane's 4 hh
 
     // Tile loads: the buffer descriptor starts at the tile's first key and ends with the sequence's last one, so rows past
     // the end arrive as zeros, and so do the chunks between hd and HD (their offset is past any end). The lanes' offsets
@@ -153,13 +158,13 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
         ko[i] = 8 * ck < a.hd ? static_cast<uint32_t>(r * a.k_ts + 8 * ck) * 2 : 0xfffffff0u;
         vof[i] = 8 * cv < a.hd ? static_cast<uint32_t>(r * a.v_ts + 8 * cv) * 2 : 0xfffffff0u;
     }
-    // the workgroup's queries, loaded like a tile into the buffers that no key tile needs yet
-    constexpr int QROWS = 32 * NW, QLOADS = QROWS * ROWB / 1024 / NW;
-    static_assert((NBUF - 1) * 2 * KT >= QROWS, "room for the queries");
+    // a wave's 32 queries, loaded like a tile into the buffers that no key tile needs yet
+    constexpr int QLOADS = 32 * ROWB / 1024;
+    static_assert((NBUF - 1) * 2 * KT >= 32 * NW, "room for the queries");
     uint32_t qo[QLOADS];
 #pragma unroll
     for (int i = 0; i < QLOADS; ++i) {
-        const int id = (wave * QLOADS + i) * 64 + lane, r = id / CPR, c = (id % CPR) ^ pa_swz_k<HD>(r);
+        const int id = i * 64 + lane, r = id / CPR, c = (id % CPR) ^ pa_swz_k<HD>(r);
         qo[i] = 8 * c < a.hd ? static_cast<uint32_t>(r * a.q_ts + 8 * c) * 2 : 0xfffffff0u;
     }
     const uint16_t* kb = a.k + k_lo * a.k_ts + kvh * a.k_hs;
@@ -197,15 +202,15 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     const uint32_t v_at = lds0 + TILEB + vr * ROWB +
                           (((2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ pa_swz_v<HD>(vr)) << 4) + 8 * (lane & 1);
 
-    // the tiles that all queries of the wave see in full
-    const int wtiles = (clamp(min(wq0 + 32, nq) + off, 0, nk) + kPaKeys - 1) / kPaKeys;
-    const int whole = wq0 + off + 1 < 0 ? 0 : (wq0 + off + 1) / kPaKeys;
+    // the tiles that the wave's queries see any of, and that they all see in full (none for a wave without queries)
+    const int wtiles = wq0 < nq ? (clamp(min(wq0 + 32, nq) + off, 0, nk) + kPaKeys - 1) / kPaKeys : 0;
+    const int whole = wq0 >= nq || wq0 + off + 1 < 0 ? 0 : (wq0 + off + 1) / kPaKeys;
     auto mask = [&](f32x16 (&z)[NT], int tile) {
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int key = tile * kPaKeys + 32 * i + 8 * (r >> 2) + 4 * hh + (r & 3);
+                const int key = tile * kPaKeys + 32 * i + 8 * (r >> 2) + (r & 3);
                 z[i][r] = key <= last ? z[i][r] : -__builtin_inff();
             }
     };
@@ -238,8 +243,9 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
         asm volatile("" ::: "memory");
     };
     if (t0 < tiles) {  // (workgroup-uniform)
-        pa_load<QLOADS>(a.q + (q_lo + q0) * a.q_ts + head * a.q_hs, static_cast<int>(((min(nq - q0, QROWS) - 1) * a.q_ts + a.hd) * 2), qo,
-                        lds0 + 2 * TILEB + wave * QLOADS * 1024);
+        const int rows = min(nq - wq0, 32) - 1;
+        pa_load<QLOADS>(a.q + (q_lo + min(wq0, nq)) * a.q_ts + head * a.q_hs,
+                        rows < 0 ? 0 : static_cast<int>(rows * a.q_ts + a.hd) * 2, qo, lds0 + 2 * TILEB + wave * QLOADS * 1024);
         load();
         meet(std::integral_constant<int, 0>{});
         f16x8 qf[KK];
@@ -323,11 +329,13 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     }
     const bool patch = ballot(odd != 0) != 0;
     l += xor_lanes<32>(l);
+    // the lane once more, from the hardware: nothing of it stays in registers through the tiles
+    const int elane = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), en = elane & 31, ehh = elane >> 5;
     // adds the values left out to the queries that see them: add(r, d, v) for each key, the wave's query r, dimension d
     auto patched = [&](int d0, int d1, auto add) {
         const int first = max(whole, t0) * kPaKeys, end = min(nk, tiles * kPaKeys);
         for (int key = first; key < end; ++key)
-            for (int d = d0 + lane; d < min(d1, a.hd); d += kWave) {
+            for (int d = d0 + elane; d < min(d1, a.hd); d += kWave) {
                 const uint16_t v = ldg(vb + key * a.v_ts + d);
                 if ((v & 0x7fff) >= 0x7c00)
                     for (int r = max(0, key - off - wq0); r < 32; ++r) add(r, d, f16_bits_to_f32(v));
@@ -343,7 +351,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             for (int x = 0; x < 8; ++x) {
                 const f32x16& v = acc[d + (x >> 2)];
                 const int r = 4 * (x & 3);
-                *(__attribute__((address_space(3))) f32x4*)(so + n * 256 + (((2 * x + hh) ^ (n & 15)) << 4)) =
+                *(__attribute__((address_space(3))) f32x4*)(so + en * 256 + (((2 * x + ehh) ^ (en & 15)) << 4)) =
                     f32x4{v[r], v[r + 1], v[r + 2], v[r + 3]};
             }
             if (patch)
@@ -354,15 +362,15 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
                 });
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 4), c = lane & 15;
+                const int r = 4 * i + (elane >> 4), c = elane & 15;
                 const f32x4 o = *(const __attribute__((address_space(3))) f32x4*)(so + r * 256 + ((c ^ (r & 15)) << 4));
                 if (wq0 + r < nq && 32 * d + 4 * c < a.hd)
                     stg(reinterpret_cast<f32x4*>(pb + static_cast<int64_t>(r) * a.NQ * a.hd + 32 * d + 4 * c), o);
             }
         }
-        if (hh == 0 && wq0 + n < nq) {
+        if (ehh == 0 && wq0 + en < nq) {
             float* ml = a.part + static_cast<int64_t>(a.nsplit) * a.Tq * a.NQ * a.hd +
-                        2 * ((static_cast<int64_t>(split) * a.Tq + q_lo + wq0 + n) * a.NQ + head);
+                        2 * ((static_cast<int64_t>(split) * a.Tq + q_lo + wq0 + en) * a.NQ + head);
             stg(reinterpret_cast<f32x2*>(ml), f32x2{m, l});
         }
         return;
@@ -375,7 +383,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-            *(__attribute__((address_space(3))) u32x2*)(so + n * ROWB + (((4 * d + x) ^ pa_swz_k<HD>(n)) << 4) + 8 * hh) =
+            *(__attribute__((address_space(3))) u32x2*)(so + en * ROWB + (((4 * d + x) ^ pa_swz_k<HD>(en)) << 4) + 8 * ehh) =
                 u32x2{pack_f16x2(acc[d][4 * x] * inv, acc[d][4 * x + 1] * inv),
                       pack_f16x2(acc[d][4 * x + 2] * inv, acc[d][4 * x + 3] * inv)};
     if (patch)
@@ -387,7 +395,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     uint16_t* ob = a.out + head * a.o_hs;
 #pragma unroll
     for (int i = 0; i < 32 * ROWB / 1024; ++i) {
-        const int id = i * 64 + lane, r = id / CPR, c = id % CPR;  // (a wave's LDS writes and reads are in order)
+        const int id = i * 64 + elane, r = id / CPR, c = id % CPR;  // (a wave's LDS writes and reads are in order)
         const u32x4 o = *(const __attribute__((address_space(3))) u32x4*)(so + r * ROWB + ((c ^ pa_swz_k<HD>(r)) << 4));
         if (wq0 + r < nq && 8 * c < a.hd) stg_any(ob + (q_lo + wq0 + r) * a.o_ts + 8 * c, o);
     }
@@ -451,6 +459,13 @@ __global__ __launch_bounds__(256) void prompt_combine_kernel(const PaArgs a, int
 
 constexpr int kPaWaves = 4;
 
+// Heads that share a workgroup (as a power of two): waves of different heads of one KV head read the same tiles for the same
+// queries, so none of them idles while another finishes the tiles of later queries, and few queries fill a workgroup.
+// With one / four heads of 32 / 8 (of 128 dimensions) a workgroup: 80 prompts of 16 tokens 22 / 12 us, 80 of 128 48 / 43,
+// 20 of 512 81 / 75, 20 of up to 1000 (10577 in all) 122 / 108, 10 of 1024 121 / 118. The parts have to be neighbours (in
+// the order of the sequences' rows instead, the 20 ragged prompts take 140 us: K and V leave the L2 between them).
+static int pa_hshift(int64_t rep) { return rep % 4 == 0 ? 2 : rep % 2 == 0 ? 1 : 0; }
+
 // Splits of a row's keys: where the queries alone make fewer workgroups than 1024 (head_dim up to 64), 512 (up to 128) or
 // 256 (above), enough for that. Four, three and one workgroup fit on a CU; every split writes and reads hd + 2 floats a
 // query. Measured with 512 / 768 / 1024 / 1536 workgroups aimed at: five ragged parts of up to 513 queries behind up to
@@ -510,11 +525,13 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
         set_last_error("%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", what, need, workspace_bytes);
         return SOI_ERR_WORKSPACE;
     }
+    const int hshift = pa_hshift(num_q_heads / num_kv_heads), rows = 32 * kPaWaves >> hshift;
     const int64_t kt = pa_keys(head_dim), nsplit = pa_nsplit(Tq, Tk, num_q_heads, head_dim, kt);
     const PaArgs a{q, k, v, out, q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride,
                    v_head_stride, out_token_stride, out_head_stride, cu_q, cu_k, static_cast<float*>(workspace),
                    static_cast<int>(Tq), static_cast<int>(Tk), static_cast<int>(num_q_heads),
-                   static_cast<int>(num_kv_heads), static_cast<int>(head_dim), static_cast<int>(nsplit), scale * kLog2e};
+                   static_cast<int>(num_kv_heads), static_cast<int>(head_dim), static_cast<int>(nsplit), hshift,
+                   scale * kLog2e};
     constexpr int NW = kPaWaves;
     const unsigned qtiles = static_cast<unsigned>(ceil_div64(max_q, 32 * NW));
     const dim3 grid(static_cast<unsigned>(num_q_heads * nsplit), static_cast<unsigned>(batch), qtiles);
@@ -529,6 +546,6 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
     if (status || nsplit == 1) return status;
     hipLaunchKernelGGL(prompt_combine_kernel, dim3(static_cast<unsigned>(num_q_heads), static_cast<unsigned>(batch),
                             static_cast<unsigned>(ceil_div64(max_q, kPaCombineRows))),
-                       dim3(256), 0, st, a, 32 * NW, static_cast<int>(kt));
+                       dim3(256), 0, st, a, rows, static_cast<int>(kt));
     return launch_status(what);
 }
