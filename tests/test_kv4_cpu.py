@@ -118,6 +118,14 @@ def test_prompt_attention_checks(lib):
     assert lib.soi_prompt_attention(*ok[:14], 0, *ok[15:]) == 0
 
 
+@pytest.mark.parametrize("at", [1, 4, 7])
+def test_prompt_rows_too_far_apart(lib, at):
+    """128 rows of a tile, and the bytes behind the first, have to fit a 32-bit offset."""
+    args = [16, 512, 128, 32, 256, 128, 48, 256, 128, 64, 64, 1, 8, 8, 8, 4, 2, 128, 1024, 512, 128, 1.0, None, 0, None]
+    args[at] = 1 << 22
+    assert "apart" in error(lib, lib.soi_prompt_attention(*args))
+
+
 def test_prompt_workspace_query(lib):
     q = lib.soi_prompt_attention_workspace_bytes
     assert q(8, 100, 4, 128) == 0 and q(0, 4096, 4, 128) == 0 and q(1 << 16, 1 << 16, 16, 128) == 0

@@ -76,6 +76,25 @@ def test_queries_without_keys_give_zeros(cuda):
     assert (got[:30] == 0).all() and (got[40:110] == 0).all()
 
 
+@pytest.mark.parametrize("NQ,NKV", [(2, 2), (2, 1), (4, 1), (14, 2)])
+def test_no_keys_at_all(cuda, NQ, NKV):
+    import soinfer.ops as ops
+
+    q, _, _, cu_q, cu_k = problem(cuda, [40, 3], [0, 0], NQ, NKV, 64, 16)
+    empty = torch.empty((0, NKV, 64), dtype=torch.float16, device=cuda)
+    assert (ops.prompt_attention(q, empty, empty, cu_q, cu_k, 40) == 0).all()
+
+
+@pytest.mark.parametrize("rep", [1, 2, 3, 4, 6, 7, 8, 12])
+def test_heads_that_share_a_workgroup(cuda, rep):
+    """Every part of a workgroup's queries, with and without a cached beginning, for each number of heads a KV head has."""
+    import soinfer.ops as ops
+
+    nq, nk = [1, 32, 33, 95, 128, 129, 200], [1, 40, 33, 300, 128, 777, 200]
+    q, k, v, cu_q, cu_k = problem(cuda, nq, nk, 3 * rep, 3, 64, 17 + rep)
+    check(ops.prompt_attention(q, k, v, cu_q, cu_k, 200), q, k, v, nq, nk, f"rep {rep}")
+
+
 def test_strided_views_and_output(cuda):
     """q, k, v as views of one fused projection, the output into every other head of a wider tensor."""
     import soinfer.ops as ops
