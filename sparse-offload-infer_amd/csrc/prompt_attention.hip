@@ -22,9 +22,9 @@
 // Bound: 4 hd operations a (query, key, head) on the matrix cores, one exponential each on the vector units (at head_dim
 // 64 both take 512 cycles for 32 x 64 scores). The running sum takes the binary16 weights that the products use, the
 // maximum is a base that is raised only when a score passes it by 8 binades. One sequence of 16384 tokens, 16 / 8 heads of
-// 128: 1.05 ms, 1048 TFLOP/s (at the 1.8 GHz that the power limit leaves; a matrix product of 8192 reaches 1160, or 1360
+// 128: 1.05 ms, 1050 TFLOP/s (at the 1.8 GHz that the power limit leaves; a matrix product of 8192 reaches 1160, or 1360
 // by its kernel alone), matrix units busy 63 % of the cycles, vector units 58 %. Twenty prompts of 1 to 1000 tokens, 32 / 8
-// heads: 91 us.
+// heads: 91 to 93 us.
 //
 // Tile, buffers and occupancy, 128 dimensions: 32 keys, three buffers (two tiles in flight), three workgroups to a CU
 // against 64 keys, two buffers, two workgroups: 1.07 / 1.07 ms and 119 / 135 us for the two above, and against 32 keys,
@@ -125,6 +125,10 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     constexpr int kPaKeys = KT;
     constexpr int CPR = HD / 8, ROWB = HD * 2, TILEB = kPaKeys * ROWB;  // chunks and bytes of a row, bytes of a tile
     constexpr int KK = HD / 16, DT = HD / 32, NT = kPaKeys / 32, NJ = kPaKeys / 16;
+    // Operand addresses of every chunk in registers and a loop of three tiles, one a buffer, whose offsets the reads then
+    // carry: 14 vector instructions fewer a tile. 16384 tokens, 16 / 8 heads: 1176 -> 1150 us on one card. (The other
+    // instances have no registers left for it.)
+    constexpr bool PRE = HD == 128 && NBUF == 3;
     constexpr int LOADS = TILEB / 1024 / NW;  // 1 KB loads per wave and tile
     static_assert(TILEB % (1024 * NW) == 0, "whole loads per wave");
     __shared__ __attribute__((aligned(1024))) uint8_t s_kv[NBUF][2][TILEB];
@@ -193,8 +197,7 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
     float m = kNegBig, l = 0.0f;
     uint32_t odd = 0;  // not 0: a value that is not finite was replaced in a tile that not all the wave's queries see in full
 
-    // Operand addresses: the lane's part below with bits flipped for the chunk, the row and the buffer added. (They stay
-    // out of loop-invariant registers that way: one XOR a read is cheaper than the registers.)
+    // Operand addresses: the lane's part below with bits flipped for the chunk, the row and the buffer added.
     // K: key n of 32, chunk 2 kk + hh
     const uint32_t k_at = lds0 + n * ROWB + ((hh ^ pa_swz_k<HD>(n)) << 4);
     // V: token vr + 8 x + 16 j, four dimensions of chunk 4 d + ...; 8 x flips bit 1 of the swizzle
@@ -256,11 +259,24 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
 #pragma unroll
         for (int i = 1; i < NBUF - 1; ++i) load();
         int at = 0, t = t0;  // LDS offset of tile t
-        auto tile = [&](auto MASKED) {
+        uint32_t kx[PRE ? KK : 1], vx[PRE ? 2 * DT : 1];
+        if constexpr (PRE) {
+#pragma unroll
+            for (int i = 0; i < KK; ++i) {
+                kx[i] = k_at ^ (i << 5);
+                asm volatile("" : "+v"(kx[i]));  // (kept: the compiler would flip the bits again for every read)
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * DT; ++i) {
+                vx[i] = v_at ^ (i << 5);
+                asm volatile("" : "+v"(vx[i]));
+            }
+        }
+        auto tile = [&](auto MASKED, auto BUF) {  // BUF: the tile's buffer, -1 where only `at` says it
             if (t > t0) meet(std::integral_constant<int, (NBUF - 2) * 2 * LOADS>{});
             load();
-            const int cur = at;
-            at = at == (NBUF - 1) * 2 * TILEB ? 0 : at + 2 * TILEB;
+            const int cur = BUF < 0 ? at : BUF * 2 * TILEB;
+            if (BUF < 0) at = at == (NBUF - 1) * 2 * TILEB ? 0 : at + 2 * TILEB;
             if (MASKED && t >= wtiles) return;  // wave-uniform: nothing of this tile is seen here
             f32x16 z[NT];
             const uint32_t ka = k_at + cur, va = v_at + cur;
@@ -268,7 +284,9 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             for (int i = 0; i < NT; ++i) {
                 f16x8 kf[KK];
 #pragma unroll
-                for (int kk = 0; kk < KK; ++kk) kf[kk] = *(const lds_f16x8*)((lds_u8*)(ka ^ (kk << 5)) + i * 32 * ROWB);
+                for (int kk = 0; kk < KK; ++kk)
+                    kf[kk] = *(const lds_f16x8*)((lds_u8*)(PRE ? kx[PRE ? kk : 0] : ka ^ (kk << 5)) + (PRE ? cur : 0) +
+                                                 i * 32 * ROWB);
                 if (KK <= 8) __builtin_amdgcn_sched_barrier(0);  // all reads first: a product waits for its own only
 #pragma unroll
                 for (int r = 0; r < 16; ++r) z[i][r] = 0.0f;
@@ -280,7 +298,8 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
                     r[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s16x4*)((lds_u8*)(va ^ (d << 6 | x << 5)) + (16 * j + 8 * x) * ROWB));
+                        (lds_s16x4*)((lds_u8*)(PRE ? vx[PRE ? 2 * d + x : 0] : va ^ (d << 6 | x << 5)) + (PRE ? cur : 0) +
+                                     (16 * j + 8 * x) * ROWB));
                 return (s16x8)__builtin_shufflevector(r[0], r[1], 0, 1, 2, 3, 4, 5, 6, 7);
             };
             s16x8 vf[2][NJ];  // V of two dimension tiles, one in use and one on its way
@@ -324,8 +343,19 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        for (; t < min(whole, tiles); ++t) tile(std::false_type{});
-        for (; t < tiles; ++t) tile(std::true_type{});
+        const int full = min(whole, tiles);
+        using std::integral_constant;
+        if constexpr (PRE)
+            while (t + NBUF <= full) {
+                tile(std::false_type{}, integral_constant<int, 0>{});
+                ++t;
+                tile(std::false_type{}, integral_constant<int, 1>{});
+                ++t;
+                tile(std::false_type{}, integral_constant<int, 2>{});
+                ++t;
+            }
+        for (; t < full; ++t) tile(std::false_type{}, integral_constant<int, -1>{});
+        for (; t < tiles; ++t) tile(std::true_type{}, integral_constant<int, -1>{});
     }
     const bool patch = ballot(odd != 0) != 0;
     l += xor_lanes<32>(l);
