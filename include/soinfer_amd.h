@@ -792,7 +792,9 @@ int soi_kv4_read(const soi_kv4_cache* cache, const int32_t* cu_seqlens, int64_t 
 /* out [batch, NQ, head_dim]: attention of one query token per sequence (q rows q_stride elements apart) over its
  * min(seq_lens[b], max_len) cached tokens; query head h reads KV head h / (NQ / NKV); zeros for an empty context; scale
  * positive. Contexts are split by the blocks of all sequences together, so the last bits of one can change with the lengths
- * of the others; the same call gives the same bits. The workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
+ * of the others; the same call gives the same bits. The product of a token's weight and a V scale is rounded to binary16
+ * relative to the largest weight times the largest V scale of its split: to 2^-11 of itself down to 2^-28 of that, and to 0
+ * below 2^-40 (scales below 2^-14 counting as 2^-14 for the largest). The workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
  * stream; calls that overlap need one each. */
 size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
                                                 int64_t head_dim, int64_t max_len);

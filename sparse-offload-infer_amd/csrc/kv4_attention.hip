@@ -15,8 +15,10 @@
 //   * O^T = V^T P^T: the lane's own scores are its B operand (k slots (g, 0 .. 7) of half a block: tokens 16 g + 8 half
 //     + 0 .. 7); the A operand of 16 dimensions is a nibble of its V units. V's scale enters with p, in binary32,
 //     before the one rounding to binary16 that the matrix cores need; the sum of p is taken unrounded;
-//   * the running maximum is one per head and wave (two lane swaps a block), sums are rescaled only in a block that
-//     raises one of them.
+//   * p = 2^(score - base), where the base keeps the largest p times the wave's largest V scale so far in [2^14, 2^15): the
+//     products fill binary16's range whatever V's size, are rounded by 2^-11 of their own value down to 2^-28 of the
+//     largest, and end in 0 below 2^-40 of it (V scales below 2^-14 count as 2^-14 here);
+//   * the base is one per head and wave (two lane swaps a block), sums are rescaled only in a block that raises one of them.
 // No operand is reordered between lanes. The scales of a block pass through LDS (a wave's own part: each lane loads 16
 // bytes of them, and reads back the 32 bytes it needs of each group), K and V go straight to registers, a block ahead.
 //
@@ -41,6 +43,7 @@
 namespace soi {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kKv4Waves = 4;
 constexpr int kKv4Block = 64;  // tokens a wave takes at a time
@@ -214,7 +217,11 @@ __global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_ke
     f32x4 acc[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x4{0, 0, 0, 0};
-    float m = kNegBig, l = 0.0f;
+    float m = kNegBig, l = 0.0f;  // m: the base of the exponents, the running maximum less `lift`
+    // the wave's V scales so far are below 2^(15 - lift), whose bits are `cap` (but for those that are not finite, whose
+    // products are infinite or NaN whatever the base)
+    float lift = 29.0f;
+    uint32_t cap = 1u << 10;
 
     // One set of operand registers: K's are loaded again as soon as the scores are done, V's after the products, so each
     // load has about half a block's work in front of it; page ids are a block further ahead.
@@ -230,6 +237,8 @@ __global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_ke
         const int left = L - blk * kKv4Block - 16 * g;
         const int live = vid < 0 ? 0 : left < 0 ? 0 : left < 16 ? left : 16;
         const bool whole = ballot(live < 16) == 0;
+        u32x4 vs;  // 8 of the block's V scales, in the lanes kVLanes
+        constexpr uint64_t kVLanes = SC == 2 ? ~0ull : ~0ull << (8 * G % 64);
         {
             u32x4* dst = reinterpret_cast<u32x4*>(&s_scale[wave][0][0][0][0]);
 #pragma unroll
@@ -242,8 +251,31 @@ __global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_ke
                         w[k] = 2 * k + 1 < n ? w[k] : 2 * k < n ? w[k] & 0xffffu : 0u;
                 }
                 if (lane + 64 * e < 16 * G) dst[lane + 64 * e] = w;
+                vs = w;
             }
             __builtin_amdgcn_wave_barrier();
+        }
+        float up = 0.0f;  // binades by which the base moves for the block's V scales
+        auto most_of = [](const u32x4& w) {
+            const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, w.x), __builtin_bit_cast(u16x2, w.y));
+            const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, w.z), __builtin_bit_cast(u16x2, w.w));
+            const u16x2 c = __builtin_elementwise_max(a, b);
+            return static_cast<uint32_t>(max(c.x, c.y));
+        };
+        if (ballot(most_of(vs) >= cap) & kVLanes) {  // (wave-uniform): a larger scale than any before, or not a finite one
+            u32x4 w = vs & 0x7fff7fffu;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const u16x2 b = __builtin_bit_cast(u16x2, w[k]);
+                w[k] = __builtin_bit_cast(uint32_t, b & (b < (uint16_t)0x7c00));
+            }
+            const float top = wave_max_bcast(kVLanes >> lane & 1 ? static_cast<float>(most_of(w)) : 0.0f);
+            const int field = static_cast<int>(top) >> 10;  // the exponent's bits
+            if (((field + 1) << 10) > static_cast<int>(cap)) {
+                up = lift - (29 - field);
+                lift = 29 - field;
+                cap = (field + 1) << 10;
+            }
         }
 
         float s[16];
@@ -285,9 +317,10 @@ __global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_ke
 #pragma unroll
         for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
         top = fmaxf(top, xor_lanes<16>(top));
-        top = fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
-        if (ballot(top > m)) {
-            const float mn = fmaxf(m, top), w = fast_exp2(m - mn);
+        top = fmaf(fmaxf(top, xor_lanes<32>(top)), a.scale_log2, -lift);
+        const float from = m + up;
+        if (ballot(top > from) || up > 0.0f) {
+            const float mn = fmaxf(from, top), w = fast_exp2(m - mn);
             m = mn;
             l *= w;
 #pragma unroll
