@@ -100,7 +100,9 @@ __device__ __forceinline__ int pa_swz_v(int row) {
 
 // A wave's 1 KB pieces of a tile into LDS: lane offsets `off` from `base`, zeros from `bytes` on. The load is written in
 // asm because the compiler, which cannot tell the two buffers apart, would let every LDS read wait for the loads in
-// flight (the kernel waits for them itself, at the barrier; no register is written). m0 holds the LDS address.
+// flight (the kernel waits for them itself, at the barrier; no register but m0 is written). m0 holds the LDS address. The
+// compiler does not count wait states inside assembly: with the s_nop the load is 5 of them behind whatever came before, as
+// many as a vector instruction's write to the descriptor's registers (a readfirstlane or readlane) has to be ahead of it.
 template <int LOADS>
 __device__ __forceinline__ void pa_load(const uint16_t* base, int bytes, const uint32_t (&off)[LOADS], uint32_t lds) {
     const uint64_t p = reinterpret_cast<uint64_t>(base);
@@ -109,9 +111,9 @@ __device__ __forceinline__ void pa_load(const uint16_t* base, int bytes, const u
                      static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(bytes)), 0x00027000u};
 #pragma unroll
     for (int i = 0; i < LOADS; ++i)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + i * 1024),
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + i * 1024),
                      "v"(off[i]), "s"(r)
-                     : "memory");
+                     : "memory", "m0");
 }
 
 // 16 bytes to any address
