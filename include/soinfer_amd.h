@@ -805,7 +805,8 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
  * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
  * one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
  * bytes and rows less than 2^22 elements apart, out 8-byte and not in q's memory; scale positive. A value that is not
- * finite reaches the queries that see its key and no others. Where the keys are split, it follows from Tq, Tk and NQ. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
+ * finite reaches the queries that see its key and no others. Weights are rounded to binary16, by 2^-11 of themselves down
+ * to 2^-21 of a query's largest, and to 0 below 2^-32 of it. Where the keys are split, it follows from Tq, Tk and NQ. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
  * aligned, needs no initial value and may be reused by the next call on the stream; calls that overlap need one each. */
 size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim);
 int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,

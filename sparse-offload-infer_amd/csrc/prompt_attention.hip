@@ -21,7 +21,7 @@
 //
 // Bound: 4 hd operations a (query, key, head) on the matrix cores, one exponential each on the vector units (at head_dim
 // 64 both take 512 cycles for 32 x 64 scores). The running sum takes the binary16 weights that the products use, the
-// maximum is a base that is raised only when a score passes it by 8 binades. One sequence of 16384 tokens, 16 / 8 heads of
+// base of the exponents lies 7 to 15 binades below the row's maximum. One sequence of 16384 tokens, 16 / 8 heads of
 // 128: 1.05 ms, 1050 TFLOP/s (at the 1.8 GHz that the power limit leaves; a matrix product of 8192 reaches 1160, or 1360
 // by its kernel alone), matrix units busy 63 % of the cycles, vector units 58 %. Twenty prompts of 1 to 1000 tokens, 32 / 8
 // heads: 91 to 93 us.
@@ -51,7 +51,9 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 typedef __attribute__((address_space(3))) f16x8 lds_f16x8;
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-constexpr float kPaSlack = 8.0f;
+// A row's largest weight lies between 2^kPaLow and 2^kPaHigh (below 65504): weights are rounded by 2^-11 of themselves down to
+// 2^-21 of the largest, and end in 0 below 2^-32 of it.
+constexpr float kPaLow = 7.0f, kPaHigh = 15.0f;
 
 struct PaArgs {
     const uint16_t *q, *k, *v;
@@ -227,11 +229,11 @@ __global__ __launch_bounds__(NW * kWave, OCC) void prompt_attention_kernel(const
             for (int r = 0; r < 16; ++r) top = fmaxf(top, z[i][r]);
         return fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
     };
-    // m is the base of the exponents, raised only where a score would pass it by more than 2^kPaSlack: weights then reach
-    // 2^kPaSlack, well inside binary16, and most tiles of a long row rescale nothing
+    // m is the base of the exponents, raised only where a weight would pass 2^kPaHigh, and then to where it is 2^kPaLow: most
+    // tiles of a long row rescale nothing
     auto raise = [&](float top) {
-        if (ballot(top > m + kPaSlack)) {
-            const float mn = top > m + kPaSlack ? top : m, w = fast_exp2(m - mn);  // a row does not depend on its neighbours
+        if (ballot(top > m + kPaHigh)) {
+            const float mn = top > m + kPaHigh ? top - kPaLow : m, w = fast_exp2(m - mn);  // a row does not depend on its neighbours
             m = mn;
             l *= w;
 #pragma unroll
