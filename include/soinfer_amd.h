@@ -780,7 +780,8 @@ typedef struct soi_kv4_cache {
  * none for no norm), RoPE from tables [table_rows, head_dim / 2], each rounded to binary32 and then binary16; q to q_out
  * [T, NQ, head_dim], k also to k_out [T, NKV, head_dim] if given, k and v quantized into the cache. Norm and rotation
  * are evaluated in binary64, so the codes follow from the inputs alone. A position past the tables or the cache
- * appends nothing and rotates by the last table row. T is at most (2^24 - 1) * 512 / head_dim, here and in
+ * appends nothing and rotates by the last table row; where seq_lens counts it, a read or the attention still takes what its
+ * slot held before. T is at most (2^24 - 1) * 512 / head_dim, here and in
  * soi_kv4_read. */
 int soi_kv4_append(const soi_kv4_cache* cache, const uint16_t* qkv, int64_t qkv_stride, const uint16_t* q_norm,
                    const uint16_t* k_norm, const float* cos_table, const float* sin_table, int64_t table_rows,

@@ -418,7 +418,8 @@ def kv4_append(qkv: torch.Tensor, q_norm: torch.Tensor | None, k_norm: torch.Ten
     and k by q_norm / k_norm [hd] (None, None: no norm), RoPE by the fp32 tables [positions, hd / 2]; k and v are
     quantized (symmetric INT4, one fp16 scale per group) into the pages block_table [B, max_blocks] names. Returns the
     rotated q [T, num_q_heads, hd] (q_out if given); the rotated k also goes to k_out [T, NKV, hd] if given. Rows behind
-    the last sequence are left as they are; a position without a page, or past the tables, is not appended."""
+    the last sequence are left as they are; a position without a page, or past the tables, is not appended
+    (a slot of a page that is skipped so keeps what it held, which later calls read if seq_lens counts it)."""
     return _C.kv4_append(qkv, q_norm, k_norm, cos_table, sin_table, k_pages, k_scale, v_pages, v_scale, block_table,
                          seq_lens, cu_seqlens, num_q_heads, eps, k_out, q_out)
 

@@ -124,9 +124,21 @@ class PagedKV4:
     def _layer(self, layer: int):
         return self.k_pages[layer], self.k_scale[layer], self.v_pages[layer], self.v_scale[layer]
 
+    @staticmethod
+    def _need_rows(what: str, step: Step, *rows: torch.Tensor) -> None:
+        for x in rows:
+            if x.shape[0] < step.tokens:
+                raise ValueError(f"PagedKV4.{what}: the step has {step.tokens} rows, got {x.shape[0]}")
+
     def append(self, layer: int, step: Step, qkv: torch.Tensor, q_norm, k_norm, cos_table: torch.Tensor,
                sin_table: torch.Tensor, num_q_heads: int, eps: float = 1e-6, keep_k: bool = False):
-        """ops.kv4_append of the step's rows: the rotated q, or (q, rotated k) with keep_k."""
+        """ops.kv4_append of the step's rows: the rotated q, or (q, rotated k) with keep_k. Rows past the step's are left out;
+        ValueError where rows are missing or a new position is past the tables, as the step's tokens count as cached."""
+        self._need_rows("append", step, qkv)
+        last = max((ln for n, ln in zip(step.new, step.lens) if n), default=0)
+        if min(cos_table.shape[0], sin_table.shape[0]) < last:
+            raise ValueError(f"PagedKV4.append: the step needs {last} positions of the RoPE tables, got "
+                             f"{cos_table.shape[0]} and {sin_table.shape[0]}")
         k_out = None
         if keep_k:
             k_out = torch.empty((qkv.shape[0], self.num_kv_heads, self.head_dim), dtype=torch.float16, device=qkv.device)
@@ -149,6 +161,7 @@ class PagedKV4:
                scale: float | None = None) -> torch.Tensor:
         """Causal attention of the step's rows. With k and v, the new rows' own (sequences that begin with this step);
         without, over everything cached, read back from the pages (prompts that continue a context)."""
+        self._need_rows("prompt", step, q, *(x for x in (k, v) if x is not None))
         if k is not None:
             if any(n != ln for n, ln in zip(step.new, step.lens)):
                 raise ValueError("PagedKV4.prompt: k and v of the new rows only serve sequences that begin with them")
