@@ -513,6 +513,21 @@ static int64_t pa_nsplit(int64_t Tq, int64_t Tk, int64_t NQ, int64_t hd, int64_t
     return n < 1 ? 1 : n > kPaMaxSplits ? kPaMaxSplits : n;
 }
 
+// Whether two of the rows i ts + j hs + 0 .. hd - 1 (i < T, j < H) share an element: for a distance of dj heads only the two
+// distances of tokens nearest to -dj hs / ts can bring them together.
+static bool pa_rows_meet(int64_t T, int64_t H, int64_t ts, int64_t hs, int64_t hd) {
+    if (hs >= hd && ts >= (H - 1) * hs + hd) return false;  // the usual order
+    if (T > 1 && ts < hd && ts > -hd) return true;
+    for (int64_t dj = 1; dj < H; ++dj) {
+        const int64_t at = dj * hs, near = T > 1 ? -at / ts : 0;
+        for (int64_t di = near - 1; di <= near + 1; ++di) {
+            const int64_t d = di * ts + at;
+            if (di < T && di > -T && d < hd && d > -hd) return true;
+        }
+    }
+    return false;
+}
+
 static int64_t pa_keys(int64_t hd) { return hd > 64 && hd <= 128 ? 32 : 64; }
 
 }  // namespace soi
@@ -554,6 +569,7 @@ extern "C" int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, i
                 "%s: q, k and v must be 16-byte aligned with strides of whole 16 bytes", what);
     SOI_REQUIRE((reinterpret_cast<uintptr_t>(out) & 7u) == 0 && out_token_stride % 4 == 0 && out_head_stride % 4 == 0,
                 "%s: out must be 8-byte aligned with strides of whole 8 bytes", what);
+    SOI_REQUIRE(!pa_rows_meet(Tq, num_q_heads, out_token_stride, out_head_stride, head_dim), "%s: rows of out overlap", what);
     const size_t need = soi_prompt_attention_workspace_bytes(Tq, Tk, num_q_heads, head_dim);
     if (need && (!workspace || workspace_bytes < need || !aligned16(workspace))) {
         set_last_error("%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", what, need, workspace_bytes);
