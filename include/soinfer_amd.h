@@ -795,8 +795,8 @@ int soi_kv4_read(const soi_kv4_cache* cache, const int32_t* cu_seqlens, int64_t 
  * positive. Contexts are split by the blocks of all sequences together, so the last bits of one can change with the lengths
  * of the others; the same call gives the same bits. The product of a token's weight and a V scale is rounded to binary16
  * relative to the largest weight times the largest V scale of its split: to 2^-11 of itself down to 2^-28 of that, and to 0
- * below 2^-40 (scales below 2^-14 counting as 2^-14 for the largest). The workspace (0 bytes where a context is not split) needs no initial value and may be reused by the next call on the
- * stream; calls that overlap need one each. */
+ * below 2^-40 (scales below 2^-14 counting as 2^-14 for the largest). The workspace (0 bytes where a context is not split)
+ * needs no initial value and may be reused by the next call on the stream; calls that overlap need one each. */
 size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
                                                 int64_t head_dim, int64_t max_len);
 int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,
@@ -805,10 +805,10 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
 /* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
  * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
  * one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
- * bytes and rows less than 2^22 elements apart, out 8-byte, its rows apart from each other and
- * not in q's memory; scale positive. A value that is not
- * finite reaches the queries that see its key and no others. Weights are rounded to binary16, by 2^-11 of themselves down
- * to 2^-21 of a query's largest, and to 0 below 2^-32 of it. Where the keys are split, it follows from Tq, Tk and NQ. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
+ * bytes and rows less than 2^22 elements apart, out 8-byte, its rows apart from each other and not in q's memory; scale
+ * positive. A value that is not finite reaches the queries that see its key and no others. Weights are rounded to
+ * binary16, by 2^-11 of themselves down to 2^-21 of a query's largest, and to 0 below 2^-32 of it. Where the keys are
+ * split, it follows from Tq, Tk and NQ. The workspace (0 bytes unless the queries are few and their keys split) is 16-byte
  * aligned, needs no initial value and may be reused by the next call on the stream; calls that overlap need one each. */
 size_t soi_prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t num_q_heads, int64_t head_dim);
 int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, const uint16_t* k,

@@ -28,10 +28,11 @@
 // order by a second launch.
 //
 // Measured: 4 contexts of up to 131072 tokens (386002 in all), 64 / 8 heads of 128, groups of 64 (420 MB): 84 us, 5.0 TB/s,
-// what a large copy reaches on this card. 48 contexts of 1870 tokens on average, 32 / 8 heads, groups of 32, pages of 16
-// (104 MB): 34 us, 30.5 of them the first launch (3.4 TB/s: a page is 1 KB of K here, each wave waits for its table entries,
-// and the nibbles' arithmetic is most of a block's time); one context of 2000: 8.6 us, two dependent launches of 5.4 and
-// 3.6 us.
+// what a large copy reaches on this card (a pure read can reach 7). 48 contexts of 1870 tokens on average, 32 / 8 heads,
+// groups of 32, pages of 16 (104 MB): 35 to 36 us, 31.4 of them the first launch (3.3 TB/s: a page is 1 KB of K here, each
+// wave waits for its table entries, and the nibbles' arithmetic is most of a block's time; 1.3 us of it came with the base
+// that follows V's scales, most of that in a wave's first block); one context of 2000: 8.5 us, two dependent launches of
+// 5.4 and 3.4 us. Heads of 256: 8 contexts, 251773 tokens, 16 / 2 heads, groups of 64 (137 MB): 36 us, 3.8 TB/s.
 // Registers, not LDS, set the workgroups of a CU (4 / 3 / 2 for 64 / 128 / 256 dimensions); K and V registers are loaded
 // again as soon as their products are issued, so that a block's loads are in flight during the rest of the block before.
 #include "soi_host.h"

@@ -16,8 +16,8 @@
 //   * the output's rescaling is lane-wise too (a lane's accumulators are all of its own query).
 // K and V tiles go from memory into LDS without passing through registers (buffer_load .. lds, whose descriptor ends with
 // the sequence's last row, so that rows behind it arrive as zeros), the next tiles' loads in flight during a tile's
-// products; 16-byte chunks are XOR-swizzled on the way so that the operand reads spread over the banks (conflicts: 0.4 %
-// of the LDS cycles). The queries come in and the outputs leave through LDS too, as whole rows.
+// products; 16-byte chunks are XOR-swizzled on the way so that the operand reads spread over the banks (conflicts: 0.1 %
+// of the busy cycles). The queries come in and the outputs leave through LDS too, as whole rows.
 //
 // Bound: 4 hd operations a (query, key, head) on the matrix cores, one exponential each on the vector units (at head_dim
 // 64 both take 512 cycles for 32 x 64 scores). The running sum takes the binary16 weights that the products use, the
@@ -29,7 +29,10 @@
 // Tile, buffers and occupancy, 128 dimensions: 32 keys, three buffers (two tiles in flight), three workgroups to a CU
 // against 64 keys, two buffers, two workgroups: 1.07 / 1.07 ms and 119 / 135 us for the two above, and against 32 keys,
 // four buffers, two workgroups: 1.10 ms and 137 us. Many workgroups hide each other's starts and masked tiles. No
-// instance spills: a version that did lost a register of Q on its way back from the accumulation registers.
+// instance may spill (the build sees to it): a version that did came back with a register of Q lost, why was never found.
+// The instance above 128 dimensions, one workgroup to a CU, keeps its accumulators in accumulation registers, where its
+// products write them, and moves all of them for every tile: 8192 tokens, 8 / 4 heads of 256, 359 us (765 TFLOP/s). These
+// moves are of whole registers: nothing between the first tile and the last changes which lanes run.
 //
 // Tiles that the wave sees in full run a loop without masks. In the others a value that is not finite has to stay out of
 // the rows that do not see its key, though their weight for it is 0: the products take the largest finite number in its
@@ -500,8 +503,10 @@ constexpr int kPaWaves = 4;
 // the order of the sequences' rows instead, the 20 ragged prompts take 140 us: K and V leave the L2 between them).
 static int pa_hshift(int64_t rep) { return rep % 4 == 0 ? 2 : rep % 2 == 0 ? 1 : 0; }
 
-// Splits of a row's keys: where the queries alone make fewer workgroups than 1024 (head_dim up to 64), 512 (up to 128) or
-// 256 (above), enough for that. Four, three and one workgroup fit on a CU; every split writes and reads hd + 2 floats a
+// Splits of a row's keys: where the heads and the 128-query tiles of all rows together make fewer workgroups than 1024
+// (head_dim up to 64), 512 (up to 128) or 256 (above), as many as fit into that. The count is a rough one: it knows neither
+// the batch nor the heads that share a workgroup, so that one short sequence with four heads to a workgroup is split into
+// fewer workgroups than that, and many sequences of a few queries into more. Four, three and one workgroup fit on a CU; every split writes and reads hd + 2 floats a
 // query. Measured with 512 / 768 / 1024 / 1536 workgroups aimed at: five ragged parts of up to 513 queries behind up to
 // 4000 keys, 14 heads of 64, 70 / 62 / 57 / 58 us, 1024 queries over 17408 keys, 8 heads of 64, 58 / 57 / 58 / 64 us. With
 // 256 / 512 / 768 / 1024: 512 queries over 16896 keys, 16 heads of 128, 123 / 93 / 94 / 105 us, 2048 queries of 8 heads of
