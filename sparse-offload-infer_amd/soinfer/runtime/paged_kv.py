@@ -161,11 +161,12 @@ class PagedKV4:
                scale: float | None = None) -> torch.Tensor:
         """Causal attention of the step's rows. With k and v, the new rows' own (sequences that begin with this step);
         without, over everything cached, read back from the pages (prompts that continue a context)."""
-        self._need_rows("prompt", step, q, *(x for x in (k, v) if x is not None))
         if k is not None:
             if any(n != ln for n, ln in zip(step.new, step.lens)):
                 raise ValueError("PagedKV4.prompt: k and v of the new rows only serve sequences that begin with them")
+            self._need_rows("prompt", step, q, k, v)
             cu_k = step.cu_seqlens
         else:
+            self._need_rows("prompt", step, q)
             k, v, cu_k = self.read(layer, step)
         return ops.prompt_attention(q, k, v, step.cu_seqlens, cu_k, step.max_new, scale)

@@ -56,3 +56,13 @@ def test_prompt_needs_every_row_of_the_step(cache):
     for bad in ((q[:4], k, v), (q, k[:4], v), (q, k, v[:4])):
         with pytest.raises(ValueError, match="5 rows"):
             cache.prompt(0, step, *bad)
+
+
+def test_rows_of_a_context_are_named_first(cache):
+    """k and v of the new rows for a sequence that had some already: that is the mistake, however many rows there are."""
+    a = cache.add()
+    cache.step({a: 5})
+    step = cache.step({a: 3})
+    q, k, v = (torch.zeros((2, h, HD), dtype=torch.float16) for h in (NQ, NKV, NKV))
+    with pytest.raises(ValueError, match="begin"):
+        cache.prompt(0, step, q, k, v)
