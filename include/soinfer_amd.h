@@ -803,8 +803,8 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
                              int64_t max_len, uint16_t* out, float scale, void* workspace, size_t workspace_bytes,
                              void* stream);
 /* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
- * nq = cu_q[b+1] - cu_q[b] <= max_q queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys j <= i + nk - nq, and
- * one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
+ * nq = cu_q[b+1] - cu_q[b] <= max_q <= 524280 queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys
+ * j <= i + nk - nq, and one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16
  * bytes and rows less than 2^22 elements apart, out 8-byte, its rows apart from each other and not in q's memory; scale
  * positive. A value that is not finite reaches the queries that see its key and no others. Weights are rounded to
  * binary16, by 2^-11 of themselves down to 2^-21 of a query's largest, and to 0 below 2^-32 of it. Where the keys are

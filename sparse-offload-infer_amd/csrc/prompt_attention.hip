@@ -506,8 +506,8 @@ static int pa_hshift(int64_t rep) { return rep % 4 == 0 ? 2 : rep % 2 == 0 ? 1 :
 // Splits of a row's keys: where the heads and the 128-query tiles of all rows together make fewer workgroups than 1024
 // (head_dim up to 64), 512 (up to 128) or 256 (above), as many as fit into that. The count is a rough one: it knows neither
 // the batch nor the heads that share a workgroup, so that one short sequence with four heads to a workgroup is split into
-// fewer workgroups than that, and many sequences of a few queries into more. Four, three and one workgroup fit on a CU; every split writes and reads hd + 2 floats a
-// query. Measured with 512 / 768 / 1024 / 1536 workgroups aimed at: five ragged parts of up to 513 queries behind up to
+// fewer workgroups than that, and many sequences of a few queries into more. Four, three and one workgroup fit on a CU;
+// every split writes and reads hd + 2 floats a query. Measured with 512 / 768 / 1024 / 1536 workgroups aimed at: five ragged parts of up to 513 queries behind up to
 // 4000 keys, 14 heads of 64, 70 / 62 / 57 / 58 us, 1024 queries over 17408 keys, 8 heads of 64, 58 / 57 / 58 / 64 us. With
 // 256 / 512 / 768 / 1024: 512 queries over 16896 keys, 16 heads of 128, 123 / 93 / 94 / 105 us, 2048 queries of 8 heads of
 // 128, 40 / 31 / 31 / 40 us. 300 queries x 2 over 3300 keys, 14 heads of 256, 67 us with 256 and 98 with 512.

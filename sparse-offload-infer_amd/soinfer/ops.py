@@ -441,10 +441,9 @@ def kv4_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.
     """out [B, NQ, hd]: attention of one query token per sequence, q [B, NQ, hd] fp16 (rotated), over its seq_lens[b]
     cached tokens (at most max_len, which sets the split of long contexts: pass the longest length the host knows;
     default: all the block table holds). Query head h reads KV head h // (NQ // NKV); scale 1/sqrt(hd) by default; an
-    empty context gives zeros. Weights times V scales below 2^-40 of the largest weight times the largest scale count as 0. A
-    long context is split by what the batch holds in all, so a sequence's last bits can change
-    with its neighbours' lengths. workspace (uint8, _C.kv4_decode_attention_workspace_bytes) and out are allocated unless
-    given; a workspace needs no initial value, and calls that overlap need one each."""
+    empty context gives zeros. Weights times V scales below 2^-40 of the largest weight times the largest scale count as 0.
+    A long context is split by what the batch holds in all, so a sequence's last bits can change with its neighbours'
+    lengths. workspace (uint8, _C.kv4_decode_attention_workspace_bytes) and out are allocated unless given; a workspace needs no initial value, and calls that overlap need one each."""
     return _C.kv4_decode_attention(q, k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, max_len, scale, out,
                                    workspace)
 
@@ -454,11 +453,11 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of packed prompts on the matrix cores: q [Tq, NQ, hd], k and v [Tk, NKV, hd] fp16 (any token and
     head strides with contiguous dimensions: views of a fused projection work), hd a multiple of 8 up to 256. Sequence
-    b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 (at most max_q), its keys rows cu_k[b] .. cu_k[b + 1] - 1; query i of
-    nq sees keys j <= i + nk - nq, so more keys than queries continue a context. A query without a key gives zeros; rows
+    b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 (at most max_q, itself at most 524280), its keys rows
+    cu_k[b] .. cu_k[b + 1] - 1; query i of nq sees keys j <= i + nk - nq, so more keys than queries continue a context. A query without a key gives zeros; rows
     behind the last sequence are left as they are. q, k and v start on 16 bytes, their strides are multiples of 8 below
-    2^22; out lies outside the memory q spans, its rows apart from each other. Weights below 2^-32 of a query's largest count as
-    0. Where few queries have their keys split over workgroups, the split (and the
+    2^22; out lies outside the memory q spans, its rows apart from each other. Weights below 2^-32 of a query's largest
+    count as 0. Where few queries have their keys split over workgroups, the split (and the
     last bits of a row with it) follows from Tq, Tk and NQ. out and workspace (uint8, _C.prompt_attention_workspace_bytes)
     are allocated unless given; a workspace needs no initial value, and calls that overlap need one each."""
     return _C.prompt_attention(q, k, v, cu_q, cu_k, max_q, scale, out, workspace)

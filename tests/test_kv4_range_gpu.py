@@ -164,3 +164,22 @@ def test_values_that_are_not_finite(cuda):
         got[0, 3:] = want[0, 3:]
         assert torch.equal(got, want)
         ks[0][350, 1, 40] = was
+
+
+@pytest.mark.parametrize("NQ,hd,gs,page", [(2, 64, 32, 64), (2, 128, 128, 16), (17, 256, 32, 64), (2, 256, 64, 16)])
+@pytest.mark.parametrize("strong", [[], [130], [1400], [5, 700, 1533, 2900]])
+def test_sizes_that_change_within_a_wave(cuda, NQ, hd, gs, page, strong):
+    """256 sequences of the same pages, so that a wave takes three blocks of 64 tokens and more, and V of another size every
+    150 tokens: up and down, with strong keys (whose own V is 0) here and there."""
+    import soinfer.ops as ops
+
+    n, B = 3001, 256
+    q, k, v = strong_key(cuda, n, NQ, 1, hd, 12, 1.0, strong, hd)
+    sizes = 2.0 ** np.array([-12, -3, -9, 0, -6, 4, -12, 8, -2, -12])
+    v = (v * sizes[np.arange(n) // 150 % 10][:, None, None]).astype(np.float16)
+    c, table, lt, held = cache_of(cuda, [k], [v], page, gs, 7)
+    qd = torch.from_numpy(q).to(cuda)
+    got = ops.kv4_decode_attention(qd.expand(B, -1, -1).contiguous(), *c, table.expand(B, -1).contiguous(), lt.expand(B).contiguous())
+    ref, bound = expect(qd.double(), *held[0], 1 / math.sqrt(hd))
+    R.assert_within(got[0], ref, bound, f"strong {strong}")
+    R.assert_within(got[-1], ref, bound, f"strong {strong}, last")
