@@ -1,4 +1,4 @@
-"""Callers of the hot path: the DIP / cache-aware DIP MLP drivers."""
-from . import dip
+"""Callers of the hot path: the DIP / cache-aware DIP MLP drivers, and the paged KV cache of several sequences."""
+from . import dip, paged_kv
 
-__all__ = ["dip"]
+__all__ = ["dip", "paged_kv"]
