@@ -818,6 +818,29 @@ int soi_prompt_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_he
                          uint16_t* out, int64_t out_token_stride, int64_t out_head_stride, float scale, void* workspace,
                          size_t workspace_bytes, void* stream);
 
+/* --------------------------------------------------------------------------
+ * The linears of several tokens in 8 bits. Activation rows and weight rows
+ * are symmetric INT8, value q s with one binary32 scale a row: for each token
+ * and for each output channel (the per_channel rows of the quantizer). K and H
+ * are multiples of 16; q rows are contiguous and 16-byte aligned.
+ * ------------------------------------------------------------------------ */
+/* Rows x [T, H] (x_stride elements apart, 2-byte aligned) -> q [T, H], scale [T]: of x itself (weight NULL), of its RMSNorm
+ * n = h w / sqrt(mean h^2 + eps), h = x, or with residual (rows residual_stride apart) of the norm of
+ * h = fp16(x + residual), which goes to sum [T, H]. scale = fp32(max|n| / 127), q = round_half_even(n / scale); the norm is
+ * evaluated in binary64 and not rounded before it is quantized. A row of zeros has scale 0; one that holds a value that is
+ * not finite gets a scale that is not finite and codes 0 (its products are NaN). T < 2^22, H <= 65536. */
+int soi_int8_rows(const uint16_t* x, int64_t x_stride, const uint16_t* residual, int64_t residual_stride,
+                  const uint16_t* weight, double eps, int64_t T, int64_t H, int8_t* q, float* scale, uint16_t* sum,
+                  void* stream);
+/* y [T, N] = fp16(x_scale[t] w_scale[n] sum_k x[t, k] Wq[n, k] (+ residual[t, n], NULL for none; may be y)): sums in 32-bit
+ * integers (exact for any codes), the rest in binary32, rounded once. K < 131072; T and N < 2^22. */
+int soi_int8_linear(const int8_t* x, const float* x_scale, const int8_t* Wq, const float* w_scale,
+                    const uint16_t* residual, uint16_t* y, int64_t T, int64_t N, int64_t K, void* stream);
+/* h [T, N] = fp16(silu(g) u), g and u the products of x with gate_Wq and up_Wq [N, K] in binary32, neither rounded first. */
+int soi_int8_gate_up(const int8_t* x, const float* x_scale, const int8_t* gate_Wq, const float* gate_scale,
+                     const int8_t* up_Wq, const float* up_scale, uint16_t* h, int64_t T, int64_t N, int64_t K,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2129,6 +2129,119 @@ torch::Tensor prompt_attention(torch::Tensor q, torch::Tensor k, torch::Tensor v
     return o;
 }
 
+namespace {
+
+const uint16_t* h16_or_null(const OptTensor& t) { return t ? h16(*t) : nullptr; }
+
+// rows [T, H] of binary16, any distance apart
+void need_rows(const torch::Tensor& t, const torch::Tensor& dev, const char* n, const char* arg) {
+    TORCH_CHECK(t.is_cuda() && t.scalar_type() == torch::kFloat16 && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) &&
+                    (t.size(0) <= 1 || t.stride(0) >= t.size(1)),
+                n, "(", arg, "): must be a 2D float16 CUDA tensor with contiguous rows that do not overlap");
+    TORCH_CHECK(t.device() == dev.device(), n, "(", arg, "): all tensors must be on one device");
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> int8_rows(const torch::Tensor& x, const OptTensor& residual,
+                                                                  const OptTensor& weight, double eps, const char* n) {
+    need_rows(x, x, n, "x");
+    const int64_t T = x.size(0), H = x.size(1);
+    if (residual) {
+        need_rows(*residual, x, n, "residual");
+        TORCH_CHECK(residual->sizes() == x.sizes(), n, "(residual): must have x's shape");
+    }
+    if (weight) {
+        need(*weight, torch::kFloat16, x, n, "weight");
+        TORCH_CHECK(weight->dim() == 1 && weight->size(0) == H, n, "(weight): must be [hidden]");
+    }
+    const at::DeviceGuard guard(x.device());
+    auto q = torch::empty({T, H}, x.options().dtype(torch::kInt8));
+    auto scale = torch::empty({T}, x.options().dtype(torch::kFloat32));
+    torch::Tensor sum = residual ? torch::empty({T, H}, x.options()) : torch::Tensor();
+    check_status(soi_int8_rows(h16(x), x.stride(0), h16_or_null(residual), residual ? residual->stride(0) : 0,
+                               h16_or_null(weight), eps, T, H, q.data_ptr<int8_t>(), scale.data_ptr<float>(),
+                               residual ? h16m(sum) : nullptr, cur_stream(x)),
+                 n);
+    return {q, scale, sum};
+}
+
+// one scale a row: [rows] or [rows, 1]
+void need_scale(const torch::Tensor& s, int64_t rows, const torch::Tensor& dev, const char* n, const char* arg) {
+    need(s, torch::kFloat32, dev, n, arg);
+    TORCH_CHECK(s.numel() == rows && (s.dim() == 1 || (s.dim() == 2 && s.size(1) == 1)), n, "(", arg, "): must be [", rows,
+                "] or [", rows, ", 1]");
+}
+
+void need_int8(const torch::Tensor& t, int64_t K, const torch::Tensor& dev, const char* n, const char* arg) {
+    need(t, torch::kInt8, dev, n, arg);
+    TORCH_CHECK(t.dim() == 2 && (K < 0 || t.size(1) == K), n, "(", arg, "): must be 2D [rows, K] of one K");
+}
+
+torch::Tensor int8_out(const OptTensor& out, int64_t T, int64_t N, const torch::Tensor& x, const char* n) {
+    if (!out) return torch::empty({T, N}, x.options().dtype(torch::kFloat16));
+    need(*out, torch::kFloat16, x, n, "out");
+    TORCH_CHECK(out->dim() == 2 && out->size(0) == T && out->size(1) == N, n, "(out): must be [", T, ", ", N, "]");
+    return *out;
+}
+
+}  // namespace
+
+std::tuple<torch::Tensor, torch::Tensor> quantize_int8(torch::Tensor x, OptTensor weight, double eps) {
+    const auto r = int8_rows(x, c10::nullopt, weight, eps, "quantize_int8");
+    return {std::get<0>(r), std::get<1>(r)};
+}
+
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> add_rmsnorm_int8(torch::Tensor x, torch::Tensor residual,
+                                                                         torch::Tensor weight, double eps) {
+    return int8_rows(x, residual, weight, eps, "add_rmsnorm_int8");
+}
+
+torch::Tensor int8_linear(torch::Tensor x, torch::Tensor x_scale, torch::Tensor Wq, torch::Tensor w_scale, OptTensor residual,
+                          OptTensor out) {
+    const char* n = "int8_linear";
+    need_int8(x, -1, x, n, "x");
+    const int64_t T = x.size(0), K = x.size(1);
+    need_int8(Wq, K, x, n, "Wq");
+    const int64_t N = Wq.size(0);
+    need_scale(x_scale, T, x, n, "x_scale");
+    need_scale(w_scale, N, x, n, "w_scale");
+    const at::DeviceGuard guard(x.device());
+    torch::Tensor y = int8_out(out, T, N, x, n);
+    if (residual) {
+        need(*residual, torch::kFloat16, x, n, "residual");
+        TORCH_CHECK(residual->sizes() == y.sizes(), n, "(residual): must be [", T, ", ", N, "]");
+        if (out && residual->data_ptr() != y.data_ptr()) no_overlap(y, *residual, n, "out and residual");
+    }
+    if (out)
+        for (const auto* t : {&x, &x_scale, &Wq, &w_scale}) no_overlap(y, *t, n, "out and an input");
+    check_status(soi_int8_linear(x.data_ptr<int8_t>(), x_scale.data_ptr<float>(), Wq.data_ptr<int8_t>(),
+                                 w_scale.data_ptr<float>(), h16_or_null(residual), h16m(y), T, N, K, cur_stream(x)),
+                 n);
+    return y;
+}
+
+torch::Tensor int8_gate_up(torch::Tensor x, torch::Tensor x_scale, torch::Tensor gate_Wq, torch::Tensor gate_scale,
+                           torch::Tensor up_Wq, torch::Tensor up_scale, OptTensor out) {
+    const char* n = "int8_gate_up";
+    need_int8(x, -1, x, n, "x");
+    const int64_t T = x.size(0), K = x.size(1);
+    need_int8(gate_Wq, K, x, n, "gate_Wq");
+    need_int8(up_Wq, K, x, n, "up_Wq");
+    const int64_t N = gate_Wq.size(0);
+    TORCH_CHECK(up_Wq.size(0) == N, n, ": gate_Wq and up_Wq must have one shape");
+    need_scale(x_scale, T, x, n, "x_scale");
+    need_scale(gate_scale, N, x, n, "gate_scale");
+    need_scale(up_scale, N, x, n, "up_scale");
+    const at::DeviceGuard guard(x.device());
+    torch::Tensor h = int8_out(out, T, N, x, n);
+    if (out)
+        for (const auto* t : {&x, &x_scale, &gate_Wq, &gate_scale, &up_Wq, &up_scale}) no_overlap(h, *t, n, "out and an input");
+    check_status(soi_int8_gate_up(x.data_ptr<int8_t>(), x_scale.data_ptr<float>(), gate_Wq.data_ptr<int8_t>(),
+                                  gate_scale.data_ptr<float>(), up_Wq.data_ptr<int8_t>(), up_scale.data_ptr<float>(), h16m(h), T,
+                                  N, K, cur_stream(x)),
+                 n);
+    return h;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "soinfer MI355X (gfx950) quantized decode hot path";
     m.def("gemv_w8a16", &gemv_w8a16, "INT8 GEMV");
@@ -2281,4 +2394,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("v"), py::arg("cu_q"), py::arg("cu_k"), py::arg("max_q"), py::arg("scale") = py::none(),
           py::arg("out") = py::none(), py::arg("workspace") = py::none());
     m.def("prompt_attention_workspace_bytes", &prompt_attention_workspace_bytes);
+    m.def("quantize_int8", &quantize_int8, "rows, or their RMSNorm, in 8 bits with a scale for each: (q, scale)", py::arg("x"),
+          py::arg("weight") = py::none(), py::arg("eps") = 1e-6);
+    m.def("add_rmsnorm_int8", &add_rmsnorm_int8, "RMSNorm of x + residual in 8 bits: (q, scale, x + residual)", py::arg("x"),
+          py::arg("residual"), py::arg("weight"), py::arg("eps") = 1e-6);
+    m.def("int8_linear", &int8_linear, "product of 8-bit rows with 8-bit weights, the residual added", py::arg("x"),
+          py::arg("x_scale"), py::arg("Wq"), py::arg("w_scale"), py::arg("residual") = py::none(), py::arg("out") = py::none());
+    m.def("int8_gate_up", &int8_gate_up, "silu(gate) * up of 8-bit rows and weights", py::arg("x"), py::arg("x_scale"),
+          py::arg("gate_Wq"), py::arg("gate_scale"), py::arg("up_Wq"), py::arg("up_scale"), py::arg("out") = py::none());
 }

@@ -88,16 +88,6 @@ __device__ __forceinline__ uint32_t xor_u(uint32_t v) {
     return __builtin_bit_cast(uint32_t, xor_lanes<MASK>(__builtin_bit_cast(float, v)));
 }
 
-// 1 / sqrt(x) to the last bits of binary64: two Newton steps on y (3 - x y^2) / 2 from the hardware's estimate, which for an
-// infinity (0) is already the answer, and would become NaN.
-__device__ __forceinline__ double rsqrt_f64(double x) {
-    const double e = __builtin_amdgcn_rsq(x);
-    double y = e;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
-    return e == 0.0 ? e : y;
-}
-
 // Lane o of a token's hd / 8 holds eight dimensions in two quads, 4 o + 0 .. 3 (x) and hd / 2 + 4 o + 0 .. 3 (y): the pairs
 // of the rotation are one lane's, so an element is widened once for both its products, and a lane needs the cos and sin
 // of four angles only.

@@ -408,6 +408,16 @@ __device__ __forceinline__ void rope_pair(float a, float b, float c, float s, fl
     o2 = fmaf(b, c, a * s);
 }
 
+// 1 / sqrt(x) to the last bits of binary64: two Newton steps on y (3 - x y^2) / 2 from the hardware's estimate, which for an
+// infinity (0) is already the answer, and would become NaN.
+__device__ __forceinline__ double rsqrt_f64(double x) {
+    const double e = __builtin_amdgcn_rsq(x);
+    double y = e;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) y = fma(y * 0.5, fma(-x * y, y, 1.0), y);
+    return e == 0.0 ? e : y;
+}
+
 // silu(t) = t / (1 + exp(-t)) in fp32 (SwiGLU gating, generate.py:178)
 __device__ __forceinline__ float silu_f32(float t) { return t / (1.0f + expf(-t)); }
 

@@ -461,3 +461,38 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     last bits of a row with it) follows from Tq, Tk and NQ. out and workspace (uint8, _C.prompt_attention_workspace_bytes)
     are allocated unless given; a workspace needs no initial value, and calls that overlap need one each."""
     return _C.prompt_attention(q, k, v, cu_q, cu_k, max_q, scale, out, workspace)
+
+
+# ---------------------------------------------------------------------------
+# the linears of several tokens in 8 bits
+# ---------------------------------------------------------------------------
+
+def quantize_int8(x: torch.Tensor, weight: torch.Tensor | None = None,
+                  eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows x [T, H] fp16 (H a multiple of 16 up to 65536, rows any distance apart), or with weight [H] their RMSNorm, in
+    symmetric INT8 with one scale a row: (q int8 [T, H], scale fp32 [T]), value q * scale, scale = max|n| / 127,
+    q = round_half_even(n / scale). The norm is not rounded before it is quantized. A row of zeros has scale 0; one that
+    holds a value that is not finite gets a scale that is not finite and codes 0 (its products are NaN)."""
+    return _C.quantize_int8(x, weight, eps)
+
+
+def add_rmsnorm_int8(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                     eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A layer's input to its projections: h = x + residual (rounded to fp16), and quantize_int8(h, weight, eps), in one
+    pass: (q, scale, h)."""
+    return _C.add_rmsnorm_int8(x, residual, weight, eps)
+
+
+def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, Wq: torch.Tensor, w_scale: torch.Tensor,
+                residual: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [T, N] fp16 = x_scale[t] * w_scale[n] * (x @ Wq^T) (+ residual [T, N] fp16). x [T, K] int8 with x_scale [T] (from
+    quantize_int8), Wq [N, K] int8 with w_scale [N] or [N, 1] (soinfer.quant.formats, per_channel), K a multiple of 16
+    below 131072, any T and N. Integer sums are exact, the rest is fp32, rounded once. out may be residual itself."""
+    return _C.int8_linear(x, x_scale, Wq, w_scale, residual, out)
+
+
+def int8_gate_up(x: torch.Tensor, x_scale: torch.Tensor, gate_Wq: torch.Tensor, gate_scale: torch.Tensor,
+                 up_Wq: torch.Tensor, up_scale: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """h [T, I] fp16 = silu(g) * u, g and u as int8_linear computes them for gate_Wq and up_Wq [I, K], but not rounded
+    first: the gated feed-forward up to its down projection, in one kernel."""
+    return _C.int8_gate_up(x, x_scale, gate_Wq, gate_scale, up_Wq, up_scale, out)
