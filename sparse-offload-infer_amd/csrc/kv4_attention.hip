@@ -258,16 +258,20 @@ __global__ __launch_bounds__(kKv4Waves * kWave, kv4_per_cu(HD)) void kv4_attn_ke
         }
         float up = 0.0f;  // binades by which the base moves for the block's V scales
         auto most_of = [](const u32x4& w) {
-            const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, w.x), __builtin_bit_cast(u16x2, w.y));
-            const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, w.z), __builtin_bit_cast(u16x2, w.w));
+            // (lanes copied to scalars first: a bit cast of a vector's lane was compiled as one of lane 0)
+            const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+            const u16x2 a = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v[0]), __builtin_bit_cast(u16x2, v[1]));
+            const u16x2 b = __builtin_elementwise_max(__builtin_bit_cast(u16x2, v[2]), __builtin_bit_cast(u16x2, v[3]));
             const u16x2 c = __builtin_elementwise_max(a, b);
             return static_cast<uint32_t>(max(c.x, c.y));
         };
         if (ballot(most_of(vs) >= cap) & kVLanes) {  // (wave-uniform): a larger scale than any before, or not a finite one
-            u32x4 w = vs & 0x7fff7fffu;
+            const u32x4 abs = vs & 0x7fff7fffu;
+            const uint32_t lanes[4] = {abs.x, abs.y, abs.z, abs.w};
+            u32x4 w;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const u16x2 b = __builtin_bit_cast(u16x2, w[k]);
+                const u16x2 b = __builtin_bit_cast(u16x2, lanes[k]);
                 w[k] = __builtin_bit_cast(uint32_t, b & (b < (uint16_t)0x7c00));
             }
             const float top = wave_max_bcast(kVLanes >> lane & 1 ? static_cast<float>(most_of(w)) : 0.0f);
