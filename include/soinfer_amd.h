@@ -841,6 +841,32 @@ int soi_int8_gate_up(const int8_t* x, const float* x_scale, const int8_t* gate_W
                      const int8_t* up_Wq, const float* up_scale, uint16_t* h, int64_t T, int64_t N, int64_t K,
                      void* stream);
 
+/* --------------------------------------------------------------------------
+ * The next token of each row of logits [batch, vocab] (binary16, or binary32
+ * with logits_f32; rows `stride` elements apart, any alignment of their type)
+ * from given random numbers u [batch] in [0, 1). No reference counterpart: the
+ * reference takes the argmax (generate.py:446).
+ *   w_i = exp((l_i - max l) / temperature), tokens in order of falling logits,
+ *   the lower index first among equals. top_k > 0 keeps the first k; top_p < 1,
+ *   of these, every token in front of which the weights add up to less than
+ *   top_p times their sum; min_p > 0, of these, the tokens of w >= min_p (the
+ *   first always stays). The token is the first whose weights, added up over
+ *   the kept ones from the front, exceed u times their sum.
+ * Each setting is an array of one value a row or, where that is NULL, the
+ * *_all value. temperature <= 0 (or NaN), and rows that hold a NaN, an
+ * infinity or nothing but -infinity: the first largest logit, NaN above every
+ * number. Logits of -infinity are never drawn. Weights are held in units of
+ * 2^-44 of the largest, sums are exact: a row's token does not depend on the
+ * other rows. vocab <= 524288, batch <= 65535. The workspace is 16-byte
+ * aligned, needs no initial value and may be reused by the next call on the
+ * stream; calls that overlap need one each.
+ * ------------------------------------------------------------------------ */
+size_t soi_sample_tokens_workspace_bytes(int64_t batch, int64_t vocab);
+int soi_sample_tokens(const void* logits, int logits_f32, int64_t stride, int64_t batch, int64_t vocab, const float* u,
+                      const float* temperature, float temperature_all, const int32_t* top_k, int32_t top_k_all,
+                      const float* top_p, float top_p_all, const float* min_p, float min_p_all, int32_t* tokens,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

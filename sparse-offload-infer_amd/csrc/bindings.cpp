@@ -2242,6 +2242,57 @@ torch::Tensor int8_gate_up(torch::Tensor x, torch::Tensor x_scale, torch::Tensor
     return h;
 }
 
+int64_t sample_tokens_workspace_bytes(int64_t B, int64_t V) { return static_cast<int64_t>(soi_sample_tokens_workspace_bytes(B, V)); }
+
+torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u, OptTensor temperature, double temperature_all,
+                            OptTensor top_k, int64_t top_k_all, OptTensor top_p, double top_p_all, OptTensor min_p,
+                            double min_p_all, OptTensor out, OptTensor workspace) {
+    const char* n = "sample_tokens";
+    const bool f32 = logits.scalar_type() == torch::kFloat32;
+    TORCH_CHECK(logits.is_cuda() && (f32 || logits.scalar_type() == torch::kFloat16) && logits.dim() == 2 &&
+                    (logits.size(1) <= 1 || logits.stride(1) == 1) && (logits.size(0) <= 1 || logits.stride(0) >= logits.size(1)),
+                n, "(logits): must be a 2D float16 or float32 CUDA tensor with contiguous rows that do not overlap");
+    const int64_t B = logits.size(0), V = logits.size(1);
+    auto row_values = [&](const OptTensor& t, torch::ScalarType dt, const char* arg) {
+        if (!t) return;
+        need(*t, dt, logits, n, arg);
+        TORCH_CHECK(t->dim() == 1 && t->size(0) == B, n, "(", arg, "): must be [batch]");
+    };
+    row_values(u, torch::kFloat32, "u");
+    row_values(temperature, torch::kFloat32, "temperature");
+    row_values(top_k, torch::kInt32, "top_k");
+    row_values(top_p, torch::kFloat32, "top_p");
+    row_values(min_p, torch::kFloat32, "min_p");
+    TORCH_CHECK(temperature_all >= 0.0, n, ": temperature must not be negative");
+    TORCH_CHECK(top_k_all >= 0 && top_k_all <= INT32_MAX, n, ": top_k must not be negative");
+    TORCH_CHECK(top_p_all > 0.0 && top_p_all <= 1.0, n, ": top_p must be in (0, 1]");
+    TORCH_CHECK(min_p_all >= 0.0 && min_p_all <= 1.0, n, ": min_p must be in [0, 1]");
+    const at::DeviceGuard guard(logits.device());
+    torch::Tensor o = out ? *out : torch::empty({B}, logits.options().dtype(torch::kInt32));
+    if (out) {
+        row_values(out, torch::kInt32, "out");
+        no_overlap(o, logits, n, "out and logits");
+    }
+    if (B == 0) return o;
+    const int64_t bytes = sample_tokens_workspace_bytes(B, V);
+    torch::Tensor ws;
+    if (workspace) {
+        need(*workspace, torch::kUInt8, logits, n, "workspace");
+        ws = *workspace;
+    } else {
+        ws = torch::empty({bytes}, logits.options().dtype(torch::kUInt8));
+    }
+    auto f32_or_null = [](const OptTensor& t) { return t ? t->data_ptr<float>() : nullptr; };
+    check_status(soi_sample_tokens(logits.data_ptr(), f32 ? 1 : 0, logits.stride(0), B, V, u.data_ptr<float>(),
+                                   f32_or_null(temperature), static_cast<float>(temperature_all),
+                                   top_k ? top_k->data_ptr<int32_t>() : nullptr, static_cast<int32_t>(top_k_all),
+                                   f32_or_null(top_p), static_cast<float>(top_p_all), f32_or_null(min_p),
+                                   static_cast<float>(min_p_all), o.data_ptr<int32_t>(), ws.data_ptr<uint8_t>(), ws.numel(),
+                                   cur_stream(logits)),
+                 n);
+    return o;
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.doc() = "soinfer MI355X (gfx950) quantized decode hot path";
     m.def("gemv_w8a16", &gemv_w8a16, "INT8 GEMV");
@@ -2402,4 +2453,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("x_scale"), py::arg("Wq"), py::arg("w_scale"), py::arg("residual") = py::none(), py::arg("out") = py::none());
     m.def("int8_gate_up", &int8_gate_up, "silu(gate) * up of 8-bit rows and weights", py::arg("x"), py::arg("x_scale"),
           py::arg("gate_Wq"), py::arg("gate_scale"), py::arg("up_Wq"), py::arg("up_scale"), py::arg("out") = py::none());
+    m.def("sample_tokens", &sample_tokens, "the next token of each row of logits from given random numbers", py::arg("logits"),
+          py::arg("u"), py::arg("temperature") = py::none(), py::arg("temperature_all") = 1.0, py::arg("top_k") = py::none(),
+          py::arg("top_k_all") = 0, py::arg("top_p") = py::none(), py::arg("top_p_all") = 1.0, py::arg("min_p") = py::none(),
+          py::arg("min_p_all") = 0.0, py::arg("out") = py::none(), py::arg("workspace") = py::none());
+    m.def("sample_tokens_workspace_bytes", &sample_tokens_workspace_bytes);
 }

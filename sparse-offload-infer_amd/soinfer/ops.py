@@ -496,3 +496,27 @@ def int8_gate_up(x: torch.Tensor, x_scale: torch.Tensor, gate_Wq: torch.Tensor, 
     """h [T, I] fp16 = silu(g) * u, g and u as int8_linear computes them for gate_Wq and up_Wq [I, K], but not rounded
     first: the gated feed-forward up to its down projection, in one kernel."""
     return _C.int8_gate_up(x, x_scale, gate_Wq, gate_scale, up_Wq, up_scale, out)
+
+
+# ---------------------------------------------------------------------------
+# the next tokens of several sequences
+# ---------------------------------------------------------------------------
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: float | torch.Tensor = 1.0,
+                  top_k: int | torch.Tensor = 0, top_p: float | torch.Tensor = 1.0, min_p: float | torch.Tensor = 0.0,
+                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row (int32 [B]) of logits [B, V] (fp16 or fp32, rows any distance apart, V up to 524288), drawn by the
+    given random numbers u [B] fp32 in [0, 1). Weights exp((l - max l) / temperature), tokens in order of falling logits,
+    the lower index first among equals: top_k keeps the first k (0: all), top_p of these every token in front of which the
+    weights add up to less than top_p times their sum, min_p of these the tokens of at least min_p times the largest weight;
+    the token is the first whose running sum over the kept ones exceeds u times their sum. Each setting is a number or a
+    tensor with one value a row (fp32, top_k int32; out of range: top_k <= 0, top_p >= 1 and min_p <= 0 cut nothing, top_p <= 0
+    and min_p >= 1 leave the first tokens, NaN cuts nothing). Temperature 0: the first largest logit; so for rows with a NaN (which is
+    above every number) or an infinity, or of nothing but -infinity. Equal calls give equal tokens: a row's does not depend
+    on the others. out and workspace (uint8, _C.sample_tokens_workspace_bytes) are allocated unless given; a workspace needs
+    no initial value, and calls that overlap need one each."""
+    def split(x, off):
+        return (x, off) if isinstance(x, torch.Tensor) else (None, x)
+
+    return _C.sample_tokens(logits, u, *split(temperature, 1.0), *split(top_k, 0), *split(top_p, 1.0), *split(min_p, 0.0),
+                            out, workspace)
