@@ -802,6 +802,22 @@ size_t soi_kv4_decode_attention_workspace_bytes(int64_t batch, int64_t num_q_hea
 int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,
                              int64_t max_len, uint16_t* out, float scale, void* workspace, size_t workspace_bytes,
                              void* stream);
+/* soi_kv4_decode_attention where sequences begin with the same pages: the sequences cu_groups[g] .. cu_groups[g+1] - 1
+ * (int32 [groups + 1], ascending in [0, batch]; offsets that are not make every sequence stand alone) are a group, whose
+ * first shared_lens[b] tokens (int32 [batch]; at most max_shared) are the same in every table row of the group. They are
+ * read and multiplied once for the group, through the row of one of its sequences; the tokens behind them through each
+ * sequence's own row. What counts as shared is the least of min(shared_lens[b], seq_lens[b]) over the group's sequences where
+ * that is at least 64, rounded down to a multiple of 64; the others, and sequences in no group, share nothing. K and V are
+ * rounded to binary16 as soi_kv4_read gives them, weights by 2^-11 of themselves down to 2^-21 of a query's largest in a split,
+ * and to 0 below 2^-32 of it. How contexts are split follows from all lengths, as there. batch and groups at most 2048,
+ * max_shared at most max_len. The workspace is 16-byte aligned, needs no initial value and may be reused by the next call on
+ * the stream; calls that overlap need one each. */
+size_t soi_kv4_shared_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads, int64_t num_kv_heads,
+                                                int64_t head_dim, int64_t max_len, int64_t max_shared);
+int soi_kv4_shared_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,
+                             const int32_t* cu_groups, int64_t groups, const int32_t* shared_lens, int64_t max_len,
+                             int64_t max_shared, uint16_t* out, float scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
 /* Causal attention of packed prompts over binary16 q, k, v (strides in elements; dimensions contiguous). Sequence b has
  * nq = cu_q[b+1] - cu_q[b] <= max_q <= 524280 queries and nk = cu_k[b+1] - cu_k[b] keys; query i sees keys
  * j <= i + nk - nq, and one that sees none gives zeros. head_dim a multiple of 8 up to 256; q, k, v 16-byte aligned with strides of whole 16

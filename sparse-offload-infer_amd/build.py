@@ -32,10 +32,10 @@ ARCH = os.environ.get("SOINFER_HIP_ARCH", "gfx950")
 HIP_SOURCES = ["decoder.hip", "capi.hip", "gemv_int4.hip", "gemv_int8.hip", "topk_select.hip", "dip_descriptors.hip",
                "sparse_down.hip", "decode_attention.hip", "dip_dense_down.hip", "grid_sync.hip", "prompt.hip",
                "prompt_mfma.hip", "prompt_dip.hip", "quantize.hip", "kv4_cache.hip", "kv4_attention.hip",
-               "prompt_attention.hip", "int8_rows.hip", "int8_linear.hip", "sample.hip"]
+               "prompt_attention.hip", "int8_rows.hip", "int8_linear.hip", "sample.hip", "kv4_shared.hip"]
 # Kernels of these may not spill: a version of the decode attention that did came back with a register of Q lost, for a
 # reason that was never found.
-NO_SPILLS = ["kv4_cache.hip", "kv4_attention.hip", "prompt_attention.hip", "int8_linear.hip"]
+NO_SPILLS = ["kv4_cache.hip", "kv4_attention.hip", "prompt_attention.hip", "int8_linear.hip", "kv4_shared.hip"]
 HIP_LIB = SOINFER / "libsoinfer_hip.so"
 EXT_LIB = SOINFER / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 

@@ -2081,6 +2081,51 @@ torch::Tensor kv4_decode_attention(torch::Tensor q, torch::Tensor k_pages, torch
     return o;
 }
 
+int64_t kv4_shared_attention_workspace_bytes(int64_t B, int64_t G, int64_t NQ, int64_t NKV, int64_t head_dim, int64_t max_len,
+                                             int64_t max_shared) {
+    return static_cast<int64_t>(soi_kv4_shared_attention_workspace_bytes(B, G, NQ, NKV, head_dim, max_len, max_shared));
+}
+
+torch::Tensor kv4_shared_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor k_scale, torch::Tensor v_pages,
+                                   torch::Tensor v_scale, torch::Tensor block_table, torch::Tensor seq_lens,
+                                   torch::Tensor cu_groups, torch::Tensor shared_lens, c10::optional<int64_t> max_len,
+                                   c10::optional<int64_t> max_shared, c10::optional<double> scale, OptTensor out,
+                                   OptTensor workspace) {
+    const char* n = "kv4_shared_attention";
+    TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kFloat16 && q.dim() == 3, n,
+                "(q): must be a 3D [batch, num_q_heads, head_dim] float16 CUDA tensor");
+    const soi_kv4_cache c = kv4_cache_of(k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, q, n);
+    const int64_t B = q.size(0), NQ = q.size(1), hd = q.size(2);
+    TORCH_CHECK(B == c.batch && hd == c.head_dim, n, "(q): must be [batch, num_q_heads, head_dim] of the cache's batch and head_dim");
+    TORCH_CHECK(q.stride(2) == 1 && (NQ == 1 || q.stride(1) == hd), n, "(q): the heads of a token must be contiguous");
+    need(cu_groups, torch::kInt32, q, n, "cu_groups");
+    TORCH_CHECK(cu_groups.dim() == 1 && cu_groups.size(0) >= 1, n, "(cu_groups): must be 1D [groups + 1]");
+    need(shared_lens, torch::kInt32, q, n, "shared_lens");
+    TORCH_CHECK(shared_lens.dim() == 1 && shared_lens.size(0) == B, n, "(shared_lens): must be 1D [batch]");
+    const int64_t G = cu_groups.size(0) - 1, cap = c.max_blocks * c.page_size, ml = max_len.value_or(cap);
+    TORCH_CHECK(ml >= 0 && ml <= cap, n, ": max_len must be in [0, ", cap, "], got ", ml);
+    const int64_t ms = max_shared.value_or(ml);
+    TORCH_CHECK(ms >= 0 && ms <= ml, n, ": max_shared must be in [0, ", ml, "], got ", ms);
+    const double sc = scale.value_or(1.0 / std::sqrt(static_cast<double>(hd)));
+    const at::DeviceGuard guard(q.device());
+    torch::Tensor o = out_or_empty(out, {B, NQ, hd}, q, n, "out");
+    if (out) no_overlap(o, q, n, "out and q");
+    if (B == 0) return o;
+    torch::Tensor ws;
+    if (workspace) {
+        need(*workspace, torch::kUInt8, q, n, "workspace");
+        ws = *workspace;
+    } else {
+        ws = torch::empty({kv4_shared_attention_workspace_bytes(B, G, NQ, c.num_kv_heads, hd, ml, ms)},
+                          q.options().dtype(torch::kUInt8));
+    }
+    check_status(soi_kv4_shared_attention(&c, h16(q), q.stride(0), NQ, cu_groups.data_ptr<int32_t>(), G,
+                                          shared_lens.data_ptr<int32_t>(), ml, ms, h16m(o), static_cast<float>(sc),
+                                          ws.data_ptr<uint8_t>(), ws.numel(), cur_stream(q)),
+                 n);
+    return o;
+}
+
 int64_t prompt_attention_workspace_bytes(int64_t Tq, int64_t Tk, int64_t NQ, int64_t head_dim) {
     return static_cast<int64_t>(soi_prompt_attention_workspace_bytes(Tq, Tk, NQ, head_dim));
 }
@@ -2458,4 +2503,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("top_k_all") = 0, py::arg("top_p") = py::none(), py::arg("top_p_all") = 1.0, py::arg("min_p") = py::none(),
           py::arg("min_p_all") = 0.0, py::arg("out") = py::none(), py::arg("workspace") = py::none());
     m.def("sample_tokens_workspace_bytes", &sample_tokens_workspace_bytes);
+    m.def("kv4_shared_attention", &kv4_shared_attention, "kv4_decode_attention of sequences in groups that begin with the same pages",
+          py::arg("q"), py::arg("k_pages"), py::arg("k_scale"), py::arg("v_pages"), py::arg("v_scale"), py::arg("block_table"),
+          py::arg("seq_lens"), py::arg("cu_groups"), py::arg("shared_lens"), py::arg("max_len") = py::none(),
+          py::arg("max_shared") = py::none(), py::arg("scale") = py::none(), py::arg("out") = py::none(),
+          py::arg("workspace") = py::none());
+    m.def("kv4_shared_attention_workspace_bytes", &kv4_shared_attention_workspace_bytes);
 }

@@ -448,6 +448,23 @@ def kv4_decode_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.
                                    workspace)
 
 
+def kv4_shared_attention(q: torch.Tensor, k_pages: torch.Tensor, k_scale: torch.Tensor, v_pages: torch.Tensor,
+                         v_scale: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, cu_groups: torch.Tensor,
+                         shared_lens: torch.Tensor, max_len: int | None = None, max_shared: int | None = None,
+                         scale: float | None = None, out: torch.Tensor | None = None,
+                         workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """kv4_decode_attention where sequences begin with the same pages: those of group g, rows cu_groups[g] ..
+    cu_groups[g + 1] - 1 (int32 [groups + 1], ascending), hold the same first shared_lens[b] tokens (int32 [B]; what a
+    group's sequences name in common counts, in whole 64 tokens; 0: shares nothing). Those are read, unpacked and multiplied
+    once for the group. Every table row names all its pages, the shared ones too. max_len and max_shared bound the lengths
+    (pass the longest the host knows; defaults: all the block table holds). K and V are rounded to fp16 as kv4_read gives
+    them; a sequence's last bits can change with the others' lengths. At most 2048 sequences and groups. workspace (uint8,
+    _C.kv4_shared_attention_workspace_bytes) and out are allocated unless given; a workspace needs no initial value, and calls
+    that overlap need one each."""
+    return _C.kv4_shared_attention(q, k_pages, k_scale, v_pages, v_scale, block_table, seq_lens, cu_groups, shared_lens,
+                                   max_len, max_shared, scale, out, workspace)
+
+
 def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
                      max_q: int, scale: float | None = None, out: torch.Tensor | None = None,
                      workspace: torch.Tensor | None = None) -> torch.Tensor:
