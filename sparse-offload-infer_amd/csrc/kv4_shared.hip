@@ -8,14 +8,20 @@
 // units of one sequence. A first launch of one workgroup lists the units from the lengths (about `want` of equal cost for each
 // KV head), a second one runs them, a third adds up each (sequence, head)'s states.
 //
-// A unit is taken in stages of 128 tokens. The workgroup's four waves unpack a stage's K and V to binary16 in LDS (values
-// q s rounded once, as kv4_read gives them), the next stage's bytes on their way into registers meanwhile. Then each wave
-// takes 32 columns (v_mfma_f32_32x32x16_f16, lanes n = lane & 31, h = lane >> 5), cw of them side by side, 4 / cw waves
-// sharing the stage's tokens:
-//   * S^T = K Q^T: lane (n, h) ends with the scores of column n and tokens 8 (r >> 2) + 4 h + (r & 3), r < 16;
-//   * O^T = V^T P^T takes these, exponentiated, as its B operand as they lie. V is kept as V^T [dimension][token], tokens
-//     in the order that this operand's k slots want (16 j + 4 h + 0 .. 3, + 8 .. 11 side by side: one 16-byte read). The
-//     cache's V units hold four tokens of one dimension, so unpacking writes such rows without a transposition.
+// A unit is taken in stages of 128 tokens. The workgroup's four waves unpack a stage's K and V codes into LDS as binary16
+// integers (exact), the next stage's bytes on their way into registers meanwhile. Then each wave takes 32 columns
+// (v_mfma_f32_32x32x16_f16, lanes n = lane & 31, h = lane >> 5), cw of them side by side, 4 / cw waves sharing the stage's
+// tokens:
+//   * S^T = K Q^T: lane (n, h) ends with the scores of column n and tokens 8 (r >> 2) + 4 h + (r & 3), r < 16; a scale group's
+//     sums are multiplied by its scale in binary32;
+//   * O^T = V^T P^T takes these, exponentiated, as its B operand as they lie, times V's scale, rounded to binary16 once: a set
+//     of weights for each scale group. V is kept as V^T [dimension][token], tokens in the order that this operand's k slots
+//     want (16 j + 4 h + 0 .. 3, + 8 .. 11 side by side: one 16-byte read). The cache's V units hold four tokens of one
+//     dimension, so unpacking writes such rows without a transposition;
+//   * the base of the exponents follows weight times the stage's largest V scale, so the products fill binary16's range
+//     whatever V's size: rounded by 2^-11 of themselves down to 2^-26 of the largest weight times the largest scale that meets
+//     it, 0 below 2^-37 of it. (K and V rounded to binary16 values in LDS would save a third of the vector work, but their
+//     rounding triples the output's error.)
 // 16-byte chunks are XOR-swizzled so that operand reads and the unpacked rows' writes spread over the banks.
 #include "soi_host.h"
 #include "soi_kv4.h"
@@ -31,7 +37,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kShWaves = 4, kShThreads = kShWaves * kWave, kShKeys = 128;
 constexpr int kShRound = 64;                     // shared tokens end on a multiple of this
 constexpr int kShMost = 2048;                    // sequences of a call
-constexpr float kShLow = 7.0f, kShHigh = 15.0f;  // a column's largest weight lies between 2^kShLow and 2^kShHigh
+constexpr float kShLow = 12.0f, kShHigh = 15.0f;  // a column's largest weight times V scale is between 2^kShLow and 2^kShHigh
 constexpr int sh_per_cu(int hd) { return hd == 64 ? 3 : hd == 128 ? 2 : 1; }  // workgroups that a CU holds
 
 struct ShUnit {
@@ -210,11 +216,13 @@ __device__ __forceinline__ int sh_swz_k(int key) {
 template <int HD, int GS>
 __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(const ShArgs a, const Kv4Cache c) {
     constexpr int W = HD / 32, U = HD / 64, G = HD / GS, KK = HD / 16, DT = HD / 32, ROWB = 2 * HD, VROWB = 2 * kShKeys;
-    // K: a thread unpacks KT pieces of 16 bytes, which lie in GK scale groups; V: VT times eight tokens of UU dimension blocks
-    constexpr int PK = HD / 32, KT = kShKeys * PK / kShThreads, GK = (HD == 64 ? 64 : 128) / GS;
-    constexpr int UU = U < 2 ? U : 2, VT = U / UU, GV = 64 * UU / GS < 1 ? 1 : 64 * UU / GS;
+    // K: a thread unpacks KT pieces of 16 bytes, of PK that a token has; V: VT times eight tokens of UU dimension blocks
+    constexpr int PK = HD / 32, KT = kShKeys * PK / kShThreads, UU = U < 2 ? U : 2, VT = U / UU;
+    static_assert(G <= PK && 2 * G <= 16, "a piece of K, and a lane m of V, for each scale");
     __shared__ __attribute__((aligned(1024))) uint8_t s_k[kShKeys * ROWB], s_v[HD * VROWB];
-    __shared__ uint64_t s_valid;  // a byte for each 16 tokens of the stage: they have a page
+    __shared__ __attribute__((aligned(16))) uint16_t s_ks[G][kShKeys], s_vs[G][kShKeys];  // scales, zeros for tokens that are not there
+    __shared__ uint64_t s_valid;   // a byte for each 16 tokens of the stage: they have a page
+    __shared__ uint32_t s_top[2];  // bits of the largest finite V scale, of this stage and the next
     if (static_cast<int>(blockIdx.y) >= ldg(&a.head->units)) return;
     const ShUnit un = a.units[blockIdx.y];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, hh = lane >> 5;
@@ -235,8 +243,8 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
     auto k_key = [&](int t) { return (tid + kShThreads * t) / PK; };
     const int k_p = tid % PK, m = tid & 15, vh = (tid >> 4) & 1, j = tid >> 5;
     u32x4 kraw[KT];
-    uint16_t ksc[KT][GK];
-    u32x2 vraw[VT][2][UU], vsc[VT][2][GV];
+    uint16_t ksc[KT];  // the token's scale of group k_p, if there is one
+    u32x2 vraw[VT][2][UU], vsc;  // lanes m < 2 G: the scales of four tokens, + 8 (m & 1), of group m >> 1
     int kid[KT], vid;
     auto pages = [&](int key0, int (&ki)[KT], int& vi) {
 #pragma unroll
@@ -250,14 +258,12 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
             const int slot = (key0 + k_key(t)) & (c.page - 1);
             const int64_t h = head_of(kid[t]);
             kraw[t] = ldg(reinterpret_cast<const u32x4*>(c.k_pages + (h * c.page + slot) * (HD / 2) + 16 * k_p));
-            const uint16_t* sp = c.k_scale + (h * G + (HD == 256 ? (k_p & 1) * (128 / GS) : 0)) * c.page + slot;
-#pragma unroll
-            for (int e = 0; e < GK; ++e) ksc[t][e] = ldg(sp + e * c.page);
+            ksc[t] = ldg(c.k_scale + (h * G + (k_p < G ? k_p : 0)) * c.page + slot);
         }
         const int slot = (key0 + 16 * j + 4 * vh) & (c.page - 1);
         const int64_t h = head_of(vid);
         const uint8_t* vp = c.v_pages + h * c.page * (HD / 2) + (slot >> 2) * (16 * U * 8) + m * (U * 8);
-        const uint16_t* sp = c.v_scale + h * G * c.page + slot;
+        vsc = ldg(reinterpret_cast<const u32x2*>(c.v_scale + (h * G + (m < 2 * G ? m >> 1 : 0)) * c.page + slot + 8 * (m & 1)));
 #pragma unroll
         for (int t = 0; t < VT; ++t)
 #pragma unroll
@@ -269,54 +275,48 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
                     vraw[t][x][0] = u32x2{r.x, r.y};
                     vraw[t][x][1] = u32x2{r.z, r.w};
                 }
-#pragma unroll
-                for (int e = 0; e < GV; ++e)
-                    vsc[t][x][e] = ldg(reinterpret_cast<const u32x2*>(sp + (128 * t / GS + e) * c.page + 8 * x));
             }
     };
-    // Values q s rounded to binary16. Tokens that are not there (past the unit, or without a page) are zeros: their scales may
-    // be anything.
-    auto unpack = [&](int key0) {
+    // Tokens that are not there (past the unit, or without a page) get scales 0: theirs may be anything.
+    auto unpack = [&](int key0, int odd) {
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
             const int key = k_key(t);
             const bool live = kid[t] >= 0 && key0 + key < un.key1;
+            if (k_p < G) s_ks[k_p][key] = live ? ksc[t] : 0;
             uint8_t* row = s_k + key * ROWB;
+            const uint32_t word[4] = {kraw[t].x, kraw[t].y, kraw[t].z, kraw[t].w};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int w = 4 * k_p + x, i = HD == 256 ? 4 * (k_p & 1) + x : w % W, g = w / W;  // word W g + i: chunk 4 i + g
-                const f16 s = __builtin_bit_cast(f16, static_cast<uint16_t>(live ? ksc[t][(HD == 64 ? 32 * i : 32 * x) / GS] : 0));
-                const f16x2 s2 = {s, s};
                 f16x2 v[4];
-                const uint32_t word[4] = {kraw[t].x, kraw[t].y, kraw[t].z, kraw[t].w};
                 dequant_int4x8_bitfield(word[x], v);
-                const f16x2 r[4] = {v[0] * s2, v[1] * s2, v[2] * s2, v[3] * s2};
-                const f16x8 o = {r[0].x, r[0].y, r[1].x, r[1].y, r[2].x, r[2].y, r[3].x, r[3].y};
+                const f16x8 o = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
                 *reinterpret_cast<f16x8*>(row + (((4 * i + g) ^ sh_swz_k<HD>(key)) << 4)) = o;
             }
         }
         const int left = vid < 0 ? 0 : un.key1 - key0 - 16 * j - 4 * vh;  // live tokens from the thread's first on
         if ((tid & 31) == 0) reinterpret_cast<uint8_t*>(&s_valid)[j] = vid >= 0;
+        if (m < 2 * G) {
+            uint32_t w[2] = {vsc.x, vsc.y}, most = 0;
 #pragma unroll
-        for (int t = 0; t < VT; ++t) {
-            f16x2 sc[2][2][GV];  // of the quad's two pairs of tokens
+            for (int y = 0; y < 2; ++y) {
+                const int there = left - 8 * (m & 1) - 2 * y;
+                w[y] = there > 1 ? w[y] : there == 1 ? w[y] & 0xffffu : 0u;
+                const uint32_t lo = w[y] & 0x7fffu, hi = w[y] >> 16 & 0x7fffu;
+                most = lo < 0x7c00u && lo > most ? lo : most;
+                most = hi < 0x7c00u && hi > most ? hi : most;
+            }
+            *reinterpret_cast<u32x2*>(&s_vs[m >> 1][16 * j + 4 * vh + 8 * (m & 1)]) = u32x2{w[0], w[1]};
+            atomicMax(&s_top[odd], most);
+        }
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
-#pragma unroll
-                for (int e = 0; e < GV; ++e) {
-                    uint32_t w[2] = {vsc[t][x][e].x, vsc[t][x][e].y};
-#pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        const int there = left - 8 * x - 2 * y;
-                        w[y] = there > 1 ? w[y] : there == 1 ? w[y] & 0xffffu : 0u;
-                        sc[x][y][e] = as_f16x2(w[y]);
-                    }
-                }
+        for (int t = 0; t < VT; ++t)
 #pragma unroll
             for (int u = 0; u < UU; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {  // dimension 64 (UU t + u) + 16 k + m
-                    const int dim = 64 * (UU * t + u) + 16 * k + m, e = (64 * u + 16 * k) / GS;
+                    const int dim = 64 * (UU * t + u) + 16 * k + m;
                     f16x2 v[2][2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
@@ -326,16 +326,14 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
                             const f16x2 bias = {(f16)-1032.0f, (f16)-1032.0f}, bias16 = {(f16)-72.0f, (f16)-72.0f};
                             const f16x2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
                             const uint32_t y8 = k < 2 ? w[y] : w[y] >> 8;
-                            const f16x2 q = k & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(y8, 0x00f000f0u, 0x64806480u)),
-                                                                              sixteenth, bias16)
-                                                  : as_f16x2(and_xor(y8, 0x000f000fu, 0x64086408u)) + bias;
-                            v[x][y] = q * sc[x][y][e];
+                            v[x][y] = k & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(y8, 0x00f000f0u, 0x64806480u)), sixteenth,
+                                                                        bias16)
+                                            : as_f16x2(and_xor(y8, 0x000f000fu, 0x64086408u)) + bias;
                         }
                     }
                     const f16x8 o = {v[0][0].x, v[0][0].y, v[0][1].x, v[0][1].y, v[1][0].x, v[1][0].y, v[1][1].x, v[1][1].y};
                     *reinterpret_cast<f16x8*>(s_v + dim * VROWB + (((2 * j + vh) ^ (dim & 15)) << 4)) = o;
                 }
-        }
     };
 
     f32x16 acc[DT];
@@ -344,31 +342,46 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
     float base = kNegBig, l = 0.0f;
-    auto products = [&](int key0, int sub, bool whole, uint64_t valid) {
-        f32x16 z;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    // scale_top: binades from the stage's largest V scale up to 1
+    auto products = [&](int key0, int sub, bool whole, uint64_t valid, float scale_top) {
+        const int at = 32 * sub + 4 * hh;  // the lane's first token, the others 8 (r >> 2) + (r & 3) further
+        float z[16];
         const uint8_t* row = s_k + (32 * sub + n) * ROWB;
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) {
-            const f16x8 kf = *reinterpret_cast<const f16x8*>(row + (((2 * kk + hh) ^ sh_swz_k<HD>(n)) << 4));
-            z = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[kk], z, 0, 0, 0);
+        for (int g = 0; g < G; ++g) {
+            f32x16 sum;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
+#pragma unroll
+            for (int kk = g * (GS / 16); kk < (g + 1) * (GS / 16); ++kk) {
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(row + (((2 * kk + hh) ^ sh_swz_k<HD>(n)) << 4));
+                sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[kk], sum, 0, 0, 0);
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const u32x2 sc = *reinterpret_cast<const u32x2*>(&s_ks[g][at + 8 * x]);
+                const f16x2 lo = as_f16x2(sc.x), hi = as_f16x2(sc.y);
+                const f16 s4[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    z[4 * x + e] = fmaf(sum[4 * x + e], static_cast<float>(s4[e]), g ? z[4 * x + e] : 0.0f);
+            }
+            if (HD == 256) __builtin_amdgcn_sched_barrier(0);  // (all groups at once would spill)
         }
         if (!whole) {
-            const int left = un.key1 - key0 - 32 * sub - 4 * hh;
+            const int left = un.key1 - key0 - at;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                const int key = 8 * (r >> 2) + (r & 3);  // from 32 sub + 4 hh
-                const bool live = key < left && ((valid >> (16 * sub + 8 * (r >> 3))) & 1);
+                const bool live = 8 * (r >> 2) + (r & 3) < left && ((valid >> (16 * sub + 8 * (r >> 3))) & 1);
                 z[r] = live ? z[r] : -__builtin_inff();
             }
         }
         float top = z[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, z[r]);
-        top = fmaxf(top, xor_lanes<32>(top)) * a.scale_log2;
-        // the base rises only where a weight would pass 2^kShHigh, to where it is 2^kShLow; a column does not depend on its
-        // neighbours
+        top = fmaf(fmaxf(top, xor_lanes<32>(top)), a.scale_log2, -scale_top);
+        // the base rises only where a product would pass 2^kShHigh, to where the largest is 2^kShLow; a column does not depend
+        // on its neighbours
         if (ballot(top > base + kShHigh)) {
             const float up = top > base + kShHigh ? top - kShLow : base, w = fast_exp2(base - up);
             base = up;
@@ -378,33 +391,47 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= w;
         }
-        f16x8 pb[2];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) pb[x][e] = static_cast<f16>(fast_exp2(fmaf(z[8 * x + e], a.scale_log2, -base)));
-            // the sum is that of the weights the products use
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) l = dot2(f16x2{pb[x][e], pb[x][e + 1]}, f16x2{(f16)1.0f, (f16)1.0f}, l);
+        for (int r = 0; r < 16; ++r) {
+            z[r] = fast_exp2(fmaf(z[r], a.scale_log2, -base));
+            l += z[r];
         }
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-            const uint8_t* vrow = s_v + (32 * d + n) * VROWB;
+        for (int g = 0; g < G; ++g) {
+            f16x8 pb[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const f16x8 vf = *reinterpret_cast<const f16x8*>(vrow + (((4 * sub + 2 * x + hh) ^ (n & 15)) << 4));
-                acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[x], acc[d], 0, 0, 0);
+            for (int x = 0; x < 4; ++x) {
+                const u32x2 sc = *reinterpret_cast<const u32x2*>(&s_vs[g][at + 8 * x]);
+                const f16x2 lo = as_f16x2(sc.x), hi = as_f16x2(sc.y);
+                const f16 s4[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // (fma, not a product: one mixed-precision instruction)
+                    pb[x >> 1][4 * (x & 1) + e] = static_cast<f16>(fmaf(z[4 * x + e], static_cast<float>(s4[e]), 0.0f));
             }
+#pragma unroll
+            for (int d = g * (GS / 32); d < (g + 1) * (GS / 32); ++d) {
+                const uint8_t* vrow = s_v + (32 * d + n) * VROWB;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const f16x8 vf = *reinterpret_cast<const f16x8*>(vrow + (((4 * sub + 2 * x + hh) ^ (n & 15)) << 4));
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[x], acc[d], 0, 0, 0);
+                }
+            }
+            if (HD == 256) __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     pages(un.key0, kid, vid);
     fetch(un.key0);
-    for (int key0 = un.key0; key0 < un.key1; key0 += kShKeys) {
+    if (tid < 2) s_top[tid] = 0;
+    sh_meet();
+    int odd = 0;
+    for (int key0 = un.key0; key0 < un.key1; key0 += kShKeys, odd ^= 1) {
         int next_kid[KT], next_vid;
         pages(key0 + kShKeys, next_kid, next_vid);
         if (key0 > un.key0) sh_meet();  // the stage before is read
-        unpack(key0);
+        unpack(key0, odd);
+        if (tid == 0) s_top[odd ^ 1] = 0;
 #pragma unroll
         for (int t = 0; t < KT; ++t) kid[t] = next_kid[t];
         vid = next_vid;
@@ -412,9 +439,10 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
         sh_meet();
         const uint64_t valid = s_valid;
         const bool whole = key0 + kShKeys <= un.key1 && valid == 0x0101010101010101ull;
+        const float scale_top = 14.0f - static_cast<float>(s_top[odd] >> 10);  // (the exponent's bits: scales below 2^(bits - 14))
         if (wcols > 0)
             for (int sub = kwave; sub < kShKeys / 32; sub += kw)
-                if (key0 + 32 * sub < un.key1) products(key0, sub, whole, valid);
+                if (key0 + 32 * sub < un.key1) products(key0, sub, whole, valid, scale_top);
     }
     if (n >= wcols) return;  // (no barrier from here on)
     l += xor_lanes<32>(l);
