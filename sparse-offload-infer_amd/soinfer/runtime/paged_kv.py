@@ -2,7 +2,7 @@
 
 PagedKV4 owns the pages of every layer, hands them out to sequences, and turns "these sequences get so many new tokens"
 into the block table, lengths and offsets that the operators take (soinfer.ops.kv4_append, kv4_read,
-kv4_decode_attention, prompt_attention). No reference counterpart: the reference keeps one sequence's binary16 cache of
+kv4_decode_attention, kv4_shared_attention, prompt_attention). No reference counterpart: the reference keeps one sequence's binary16 cache of
 a fixed length per layer (python/soinfer/runtime/generate.py:276-310).
 
     cache = PagedKV4(layers, pages, NKV, hd, max_len=4096)
@@ -12,6 +12,9 @@ a fixed length per layer (python/soinfer/runtime/generate.py:276-310).
     out = cache.prompt(layer, step, q, k, v)                 # causal attention of the packed prompts
     step = cache.step({a: 1, b: 1})                          # a decode step
     out = cache.attend(layer, step, cache.append(layer, step, qkv, qn, kn, cos, sin, NQ))
+    c = cache.fork(a)                                        # begins with a's whole pages, which it does not copy
+
+Sequences next to each other in a decode step that share pages are attended to together: their common pages are read once.
 
 One page number stands for the same page in every layer, so a step's tables serve them all.
 """
@@ -37,6 +40,9 @@ class Step:
     tokens: int                 # rows of all sequences
     max_new: int
     max_len: int
+    cu_groups: torch.Tensor | None = None    # int32 [groups + 1]: sequences next to each other that share pages,
+    shared_lens: torch.Tensor | None = None  # int32 [B]: and the tokens these hold (None, None: no sequences do)
+    max_shared: int = 0
 
 
 class PagedKV4:
@@ -65,6 +71,7 @@ class PagedKV4:
         self.v_scale = pages((head_dim // group_size, page_size), torch.float16)
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
+        self._users: dict[int, int] = {}  # of pages that more than one sequence holds
         self._lens: dict[int, int] = {}
         self._next = 0
 
@@ -84,11 +91,49 @@ class PagedKV4:
         self._pages[s], self._lens[s] = [], 0
         return s
 
+    def fork(self, sequence: int, tokens: int | None = None) -> int:
+        """A new sequence that begins as `sequence` does: with the whole pages among its first `tokens` tokens (default: all it
+        has), which both hold from now on. length() says how many tokens these are; the rest is for the caller to append."""
+        have = self._lens[sequence]
+        tokens = have if tokens is None else tokens
+        if not 0 <= tokens <= have:
+            raise ValueError(f"PagedKV4.fork: sequence {sequence} holds {have} tokens, not {tokens}")
+        pages = self._pages[sequence][:tokens // self.page_size]
+        s = self.add()
+        self._pages[s], self._lens[s] = list(pages), len(pages) * self.page_size
+        for p in pages:
+            self._users[p] = self._users.get(p, 1) + 1
+        return s
+
     def free(self, sequence: int) -> None:
-        """Gives a sequence's pages back. Work already on the stream still reads them; the pages are written again only by
-        later appends on it."""
-        self._free.extend(reversed(self._pages.pop(sequence)))
+        """Gives a sequence's pages back, those that no other holds. Work already on the stream still reads them; the pages are
+        written again only by later appends on it."""
+        for p in reversed(self._pages.pop(sequence)):
+            users = self._users.pop(p, 1) - 1
+            if users > 1:
+                self._users[p] = users
+            elif users == 0:
+                self._free.append(p)
         del self._lens[sequence]
+
+    def _groups(self, seqs: tuple[int, ...], table: np.ndarray) -> tuple[list[int], list[int]]:
+        """Sequences next to each other that begin with the same pages: (offsets of the groups, shared tokens of each sequence).
+        A sequence joins the group before it where that saves page reads, though the group then shares fewer pages."""
+        held = np.array([len(self._pages[s]) for s in seqs])
+        apart = table[1:] != table[:-1]
+        apart |= np.arange(table.shape[1]) >= np.minimum(held[1:], held[:-1])[:, None]
+        common = np.where(apart.any(1), apart.argmax(1), table.shape[1]).tolist()  # pages that each has with the one before it
+        cu, shared, size, pages = [0], [], 1, int(held[0])
+        for i, n in enumerate(common, 1):
+            n = min(n, pages)
+            if n and size * n >= (size - 1) * pages:
+                size, pages = size + 1, n
+                continue
+            shared += [pages * self.page_size if size > 1 else 0] * size
+            cu.append(i)
+            size, pages = 1, int(held[i])
+        shared += [pages * self.page_size if size > 1 else 0] * size
+        return cu + [len(seqs)], shared
 
     def step(self, new: dict[int, int]) -> Step:
         """Room for `new` tokens of each sequence (0: attend or read only). Raises RuntimeError, and changes nothing, where
@@ -114,10 +159,17 @@ class PagedKV4:
         for i, s in enumerate(seqs):
             table[i, :len(self._pages[s])] = self._pages[s]
         cu = np.concatenate([[0], np.cumsum(list(new.values()))]).astype(np.int32)
-        # one copy for the three tables
-        flat = torch.from_numpy(np.concatenate([table.ravel(), np.asarray(lens, np.int32), cu])).to(self.device)
-        t, ln, c = flat.split([table.size, len(seqs), len(seqs) + 1])
-        return Step(seqs, tuple(new.values()), lens, t.view(table.shape), ln, c, int(cu[-1]), max(new.values()), max(lens))
+        groups, shared = self._groups(seqs, table) if self._users else ([], [])
+        if not any(shared):
+            groups, shared = [], []
+        # one copy for the tables
+        flat = torch.from_numpy(np.concatenate([table.ravel(), np.asarray(lens, np.int32), cu, np.asarray(groups, np.int32),
+                                                np.asarray(shared, np.int32)])).to(self.device)
+        t, ln, c, gr, sh = flat.split([table.size, len(seqs), len(seqs) + 1, len(groups), len(shared)])
+        step = Step(seqs, tuple(new.values()), lens, t.view(table.shape), ln, c, int(cu[-1]), max(new.values()), max(lens))
+        if groups:
+            step.cu_groups, step.shared_lens, step.max_shared = gr, sh, max(shared)
+        return step
 
     # ---- the operators --------------------------------------------------------------------------
 
@@ -154,7 +206,11 @@ class PagedKV4:
         return k, v, cu_k
 
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float | None = None) -> torch.Tensor:
-        """ops.kv4_decode_attention: one query token of each sequence, q [B, NQ, hd], over its cached tokens."""
+        """ops.kv4_decode_attention: one query token of each sequence, q [B, NQ, hd], over its cached tokens. Where sequences
+        next to each other share pages, ops.kv4_shared_attention (up to its 2048 sequences)."""
+        if step.cu_groups is not None and len(step.sequences) <= 2048:
+            return ops.kv4_shared_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.cu_groups,
+                                            step.shared_lens, step.max_len, min(step.max_shared, step.max_len), scale)
         return ops.kv4_decode_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.max_len, scale)
 
     def prompt(self, layer: int, step: Step, q: torch.Tensor, k: torch.Tensor | None = None, v: torch.Tensor | None = None,
