@@ -8,7 +8,7 @@
 // units of one sequence. A first launch of one workgroup lists the units from the lengths (about `want` of equal cost for each
 // KV head), a second one runs them, a third adds up each (sequence, head)'s states.
 //
-// A unit is taken in stages of 128 tokens. The workgroup's four waves unpack a stage's K and V codes into LDS as binary16
+// A unit is taken in stages of 64 tokens. The workgroup's four waves unpack a stage's K and V codes into LDS as binary16
 // integers (exact), the next stage's bytes on their way into registers meanwhile. Then each wave takes 32 columns
 // (v_mfma_f32_32x32x16_f16, lanes n = lane & 31, h = lane >> 5), cw of them side by side, 4 / cw waves sharing the stage's
 // tokens:
@@ -33,18 +33,19 @@ namespace soi {
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kShWaves = 4, kShThreads = kShWaves * kWave, kShKeys = 128;
+constexpr int kShWaves = 4, kShThreads = kShWaves * kWave, kShKeys = 64;
 constexpr int kShRound = 64;                     // shared tokens end on a multiple of this
 constexpr int kShMost = 2048;                    // sequences of a call
 constexpr float kShLow = 12.0f, kShHigh = 15.0f;  // a column's largest weight times V scale is between 2^kShLow and 2^kShHigh
-constexpr int sh_per_cu(int hd) { return hd == 64 ? 3 : hd == 128 ? 2 : 1; }  // workgroups that a CU holds
+// workgroups that a CU's registers hold
+constexpr int sh_per_cu(int hd, int gs) { return hd == 64 ? 4 : hd == 256 ? 1 : gs == 32 ? 2 : 3; }
 
 struct ShUnit {
     int row, key0, key1;    // tokens key0 .. key1 - 1 of page table row `row`
     int seq0, col0, ncols;  // columns col0 .. col0 + ncols - 1 of the sequences from seq0 on
-    int state, step;        // state of its first column, the next wave's share of the tokens `step` further
-    int cw, pad[3];         // waves side by side
+    int state, cw;          // state of its first column; waves side by side
 };
 struct ShSeq {                    // the states of a sequence's head r of a KV head:
     int pre, pre_step, pre_n;     // pre + i pre_step + r, i < pre_n, over the shared tokens
@@ -69,23 +70,23 @@ struct ShArgs {
 };
 
 // What a stage costs a wave, roughly (in units of ten cycles): unpacking its part, and cw rounds of 32 tokens.
-__device__ __forceinline__ int sh_cost(int cw) { return 110 + 80 * cw; }
+__device__ __forceinline__ int sh_cost(int cw) { return 60 + 90 * (cw == 4 ? 2 : 1); }
 
-constexpr int kShPlan = 1024;  // threads of the plan
-template <class N>
-__device__ __forceinline__ N sh_scan(N v, N* s_part, N& all) {  // exclusive over the threads, and the sum
+template <int NT>
+__device__ __forceinline__ int64_t sh_scan(int64_t v, int64_t* s_part, int64_t& all) {  // exclusive over the threads, and the sum
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    N x = v;
+    int64_t x = v;
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {
-        const N y = __shfl_up(x, o);
+        const int64_t y = __shfl_up(x, o);
         x += lane >= o ? y : 0;
     }
     if (lane == 63) s_part[wave] = x;
     __syncthreads();
-    N base = 0;
+    int64_t base = 0;
     all = 0;
-    for (int w = 0; w < kShPlan / kWave; ++w) {
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) {
         base += w < wave ? s_part[w] : 0;
         all += s_part[w];
     }
@@ -94,109 +95,122 @@ __device__ __forceinline__ N sh_scan(N v, N* s_part, N& all) {  // exclusive ove
 }
 
 // The units of a call, and where each sequence's states are. A group shares what all its sequences that share anything have
-// in common, so that a unit's columns all see all its tokens; sequences outside every group share nothing.
-__global__ __launch_bounds__(kShPlan) void kv4_shared_plan_kernel(const ShArgs a, const Kv4Cache c) {
-    // of each group: first sequence, shared tokens, the first sequence that shares them, its first unit and state
-    __shared__ int s_cu[kShMost + 1], s_keys[kShMost], s_row[kShMost], s_unit[kShMost], s_state[kShMost];
-    __shared__ int s_part[kShPlan / kWave];
-    __shared__ int64_t s_part64[kShPlan / kWave];
+// in common, so that a unit's columns all see all its tokens; sequences outside every group share nothing. NT: a thread for
+// each sequence and group, where 1024 are enough.
+template <int NT>
+__global__ __launch_bounds__(NT) void kv4_shared_plan_kernel(const ShArgs a, const Kv4Cache c) {
+    // of each group: first sequence, shared tokens, the first sequence that shares them, its first unit and state; of each
+    // sequence: its length, its group (none: kNone) if it shares anything
+    constexpr int kMost = NT < 1024 ? NT : kShMost, kNone = 0xffff;
+    __shared__ int s_cu[kMost + 1], s_keys[kMost], s_row[kMost], s_unit[kMost], s_state[kMost], s_len[kMost];
+    __shared__ uint16_t s_group[kMost];
+    __shared__ int64_t s_part[NT / kWave];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, B = c.B, rep = a.rep;
-    for (int g = tid; g <= a.G; g += kShPlan) s_cu[g] = ldg(a.cu + g);
-    for (int g = tid; g < a.G; g += kShPlan) s_keys[g] = s_row[g] = 0x7fffffff;
+    for (int g = tid; g <= a.G; g += NT) s_cu[g] = ldg(a.cu + g);
+    for (int g = tid; g < a.G; g += NT) s_keys[g] = s_row[g] = 0x7fffffff;
+    int shared[kMost / NT];
+#pragma unroll
+    for (int i = 0; i < kMost / NT; ++i) {
+        const int b = tid + i * NT;
+        if (b < B) {
+            int L = ldg(c.lens + b), n = ldg(a.shared + b);
+            L = L < 0 ? 0 : L < a.max_len ? L : a.max_len;
+            n = n < a.max_shared ? n : a.max_shared;
+            n = n < L ? n : L;
+            shared[i] = n < kShRound ? 0 : n / kShRound * kShRound;
+            s_len[b] = L;
+        }
+    }
     __syncthreads();
     int bad = 0;
-    for (int g = tid; g <= a.G; g += kShPlan) bad |= s_cu[g] < (g ? s_cu[g - 1] : 0) || s_cu[g] > B;
+    for (int g = tid; g <= a.G; g += NT) bad |= s_cu[g] < (g ? s_cu[g - 1] : 0) || s_cu[g] > B;
     const int G = __syncthreads_or(bad) ? 0 : a.G;  // offsets that are none: nobody shares anything
-    auto length = [&](int b) {
-        const int L = ldg(c.lens + b);
-        return L < 0 ? 0 : L < a.max_len ? L : a.max_len;
-    };
-    auto group_of = [&](int b) {  // -1: none
-        int lo = 0, hi = G;       // the last g < G with cu[g] <= b
+#pragma unroll
+    for (int i = 0; i < kMost / NT; ++i) {
+        const int b = tid + i * NT;
+        if (b >= B) continue;
+        int lo = 0, hi = G;  // the last g < G with cu[g] <= b
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (s_cu[mid] <= b) lo = mid;
             else hi = mid;
         }
-        return G > 0 && s_cu[lo] <= b && b < s_cu[lo + 1] ? lo : -1;
-    };
-    auto shares = [&](int b, int L) {
-        int n = ldg(a.shared + b);
-        n = n < a.max_shared ? n : a.max_shared;
-        n = n < L ? n : L;
-        return n < kShRound ? 0 : n / kShRound * kShRound;
-    };
-    for (int b = tid; b < B; b += kShPlan) {
-        const int g = group_of(b), n = shares(b, length(b));
-        if (g >= 0 && n > 0) {
-            atomicMin(&s_keys[g], n);
-            atomicMin(&s_row[g], b);
+        const bool in = G > 0 && s_cu[lo] <= b && b < s_cu[lo + 1] && shared[i] > 0;
+        s_group[b] = static_cast<uint16_t>(in ? lo : kNone);
+        if (in) {
+            atomicMin(&s_keys[lo], shared[i]);
+            atomicMin(&s_row[lo], b);
         }
     }
     __syncthreads();
-    const int width = 32 * a.cw, own_tiles = (rep + 31) / 32, pre_kw = kShWaves / a.cw;
+    const int width = 32 * a.cw, own_tiles = (rep + 31) / 32;
     auto stages = [](int keys) { return (keys + kShKeys - 1) / kShKeys; };
     auto keys_of = [&](int g) { return s_row[g] == 0x7fffffff ? 0 : s_keys[g]; };
     auto columns = [&](int g) { return (s_cu[g + 1] - s_cu[g]) * rep; };
     auto tiles = [&](int g) { return (columns(g) + width - 1) / width; };
+    auto start_of = [&](int b) { return s_group[b] == kNone ? 0 : keys_of(s_group[b]); };
     int64_t cost = 0, total;
-    for (int g = tid; g < G; g += kShPlan) cost += static_cast<int64_t>(tiles(g)) * stages(keys_of(g)) * sh_cost(a.cw);
-    for (int b = tid; b < B; b += kShPlan) {
-        const int L = length(b), g = group_of(b);
-        cost += static_cast<int64_t>(own_tiles) * stages(L - (g >= 0 && shares(b, L) > 0 ? keys_of(g) : 0)) * sh_cost(1);
-    }
-    sh_scan(cost, s_part64, total);
+    for (int g = tid; g < G; g += NT) cost += static_cast<int64_t>(tiles(g)) * stages(keys_of(g)) * sh_cost(a.cw);
+    for (int b = tid; b < B; b += NT) cost += static_cast<int64_t>(own_tiles) * stages(s_len[b] - start_of(b)) * sh_cost(1);
+    sh_scan<NT>(cost, s_part, total);
     auto per_unit = [&](int of) {  // stages of a unit, each of cost `of`
-        const int64_t d = static_cast<int64_t>(a.want) * of, n = (total + d - 1) / d;
+        const uint64_t d = static_cast<uint64_t>(a.want) * of, t = static_cast<uint64_t>(total);
+        const uint64_t n = (t | d) >> 32 ? (t + d - 1) / d : (static_cast<uint32_t>(t) + static_cast<uint32_t>(d) - 1) / static_cast<uint32_t>(d);
         return static_cast<int>(n < 1 ? 1 : n);
     };
     const int pre_per = per_unit(sh_cost(a.cw)), own_per = per_unit(sh_cost(1));
     auto splits = [&](int keys, int per) { return (stages(keys) + per - 1) / per; };
-    int unit0 = 0, state0 = 0;
-    for (int g0 = 0; g0 < G; g0 += kShPlan) {
+    auto both = [](int units, int64_t states) { return states << 24 | units; };  // (at most 65535 units, 2^31 states)
+    int64_t at = 0;
+    for (int g0 = 0; g0 < G; g0 += NT) {
         const int g = g0 + tid, ns = g < G ? splits(keys_of(g), pre_per) : 0;
-        int units, states;
-        const int u = unit0 + sh_scan(ns ? tiles(g) * ns : 0, s_part, units);
-        const int s = state0 + sh_scan(ns ? columns(g) * ns * pre_kw : 0, s_part, states);
+        int64_t all;
+        const int64_t x = at + sh_scan<NT>(ns ? both(tiles(g) * ns, static_cast<int64_t>(columns(g)) * ns) : 0, s_part, all);
         if (g < G) {
-            s_unit[g] = u;
-            s_state[g] = s;
+            s_unit[g] = static_cast<int>(x & 0xffffff);
+            s_state[g] = static_cast<int>(x >> 24);
         }
-        unit0 += units;
-        state0 += states;
+        at += all;
     }
     __syncthreads();
-    for (int g = wave; g < G; g += kShPlan / kWave) {  // a wave lists a group's units
+    for (int g = wave; g < G; g += NT / kWave) {  // a wave lists a group's units
         const int keys = keys_of(g), ns = splits(keys, pre_per), cols = columns(g), n = ns ? tiles(g) * ns : 0;
         for (int i = lane; i < n; i += kWave) {
             const int t = i / ns, k = i - t * ns, k0 = k * pre_per * kShKeys, k1 = k0 + pre_per * kShKeys;
             const int left = cols - t * width;
             if (s_unit[g] + i < a.most_units)
                 a.units[s_unit[g] + i] = ShUnit{s_row[g], k0, k1 < keys ? k1 : keys, s_cu[g], t * width, left < width ? left : width,
-                                                s_state[g] + k * pre_kw * cols + t * width, cols, a.cw, {0, 0, 0}};
+                                                s_state[g] + k * cols + t * width, a.cw};
         }
     }
-    for (int b0 = 0; b0 < B; b0 += kShPlan) {
-        const int b = b0 + tid, L = b < B ? length(b) : 0, g = b < B ? group_of(b) : -1;
-        const int start = g >= 0 && shares(b, L) > 0 ? keys_of(g) : 0, ns = splits(L - start, own_per);
-        int units, states;
-        int u = unit0 + sh_scan(ns * own_tiles, s_part, units);
-        const int s = state0 + sh_scan(ns * kShWaves * rep, s_part, states);
-        unit0 += units;
-        state0 += states;
+    for (int b0 = 0; b0 < B; b0 += NT) {
+        const int b = b0 + tid, L = b < B ? s_len[b] : 0, start = b < B ? start_of(b) : 0, ns = splits(L - start, own_per);
+        int64_t all;
+        const int64_t x = at + sh_scan<NT>(both(ns * own_tiles, static_cast<int64_t>(ns) * rep), s_part, all);
+        at += all;
         if (b >= B) continue;
+        int u = static_cast<int>(x & 0xffffff);
+        const int s = static_cast<int>(x >> 24);
         for (int t = 0; t < own_tiles; ++t)
             for (int k = 0; k < ns; ++k, ++u) {
                 const int k0 = start + k * own_per * kShKeys, k1 = k0 + own_per * kShKeys, left = rep - 32 * t;
                 if (u < a.most_units)
-                    a.units[u] = ShUnit{b, k0, k1 < L ? k1 : L, b, 32 * t, left < 32 ? left : 32,
-                                        s + k * kShWaves * rep + 32 * t, rep, 1, {0, 0, 0}};
+                    a.units[u] = ShUnit{b, k0, k1 < L ? k1 : L, b, 32 * t, left < 32 ? left : 32, s + k * rep + 32 * t, 1};
             }
-        const int cols = start ? columns(g) : 0;
-        a.seqs[b] = ShSeq{start ? s_state[g] + (b - s_cu[g]) * rep : 0, cols, start ? splits(start, pre_per) * pre_kw : 0,
-                          s, ns * kShWaves, {0, 0, 0}};
+        const int g = start ? s_group[b] : 0, cols = start ? columns(g) : 0;
+        a.seqs[b] = ShSeq{start ? s_state[g] + (b - s_cu[g]) * rep : 0, cols, start ? splits(start, pre_per) : 0, s, ns, {0, 0, 0}};
     }
-    if (tid == 0) a.head->units = unit0 < a.most_units ? unit0 : a.most_units;
+    if (tid == 0) {
+        const int units = static_cast<int>(at & 0xffffff);
+        a.head->units = units < a.most_units ? units : a.most_units;
+    }
+}
+
+// an index that the compiler does not compute ahead of the loop and keep (addresses that differ in a few bits would take more
+// registers than there are)
+__device__ __forceinline__ int sh_here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 
 // the waves' LDS writes are done, and all reads before; loads into registers stay in flight
@@ -207,26 +221,42 @@ __device__ __forceinline__ void sh_meet() {
     asm volatile("" ::: "memory");
 }
 
-// physical 16-byte chunk of chunk c of a K row (HD / 8 chunks), and of a V row (16 chunks: the stage's tokens)
-template <int HD>
-__device__ __forceinline__ int sh_swz_k(int key) {
-    return HD == 64 ? (key >> 1) & 7 : key & 15;
+// (a lo(s), b hi(s)) as binary16, each product rounded once
+__device__ __forceinline__ uint32_t times_f16(float a, float b, uint32_t s) {
+    const f16x2 w = as_f16x2(s);  // (fma, not a product: one mixed-precision instruction)
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(fmaf(a, static_cast<float>(w.x), 0.0f)),
+                                              static_cast<f16>(fmaf(b, static_cast<float>(w.y), 0.0f))});
 }
 
-template <int HD, int GS>
-__global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(const ShArgs a, const Kv4Cache c) {
+// physical 16-byte chunk of chunk c: c ^ swizzle, of a K row (HD / 8 chunks) and of a V row (8 chunks: the stage's tokens)
+template <int HD>
+__device__ __forceinline__ int sh_swz_k(int key) {
+    return HD == 64 ? (key >> 1) & 7 : (key & 3) << 2 | ((key >> 2) & 3);
+}
+__device__ __forceinline__ int sh_swz_v(int dim) { return (dim >> 1) & 7; }
+
+// BIG: pages of at least a stage, so a stage lies in one page, and its addresses are wave-uniform but for the lane's offset.
+template <int HD, int GS, bool BIG>
+__global__ __launch_bounds__(kShThreads, sh_per_cu(HD, GS)) void kv4_shared_kernel(const ShArgs a, const Kv4Cache c) {
     constexpr int W = HD / 32, U = HD / 64, G = HD / GS, KK = HD / 16, DT = HD / 32, ROWB = 2 * HD, VROWB = 2 * kShKeys;
-    // K: a thread unpacks KT pieces of 16 bytes, of PK that a token has; V: VT times eight tokens of UU dimension blocks
-    constexpr int PK = HD / 32, KT = kShKeys * PK / kShThreads, UU = U < 2 ? U : 2, VT = U / UU;
+    // K: KT pieces of 16 bytes, of PK that a token has, a thread; V: eight tokens of UU blocks of 64 dimensions a thread. Heads
+    // of 64 have enough for half the threads: the first half unpacks V, the second K.
+    constexpr int PK = HD / 32, KT = HD == 256 ? 2 : 1, UU = HD == 256 ? 2 : 1;
     static_assert(G <= PK && 2 * G <= 16, "a piece of K, and a lane m of V, for each scale");
-    __shared__ __attribute__((aligned(1024))) uint8_t s_k[kShKeys * ROWB], s_v[HD * VROWB];
-    __shared__ __attribute__((aligned(16))) uint16_t s_ks[G][kShKeys], s_vs[G][kShKeys];  // scales, zeros for tokens that are not there
-    __shared__ uint64_t s_valid;   // a byte for each 16 tokens of the stage: they have a page
-    __shared__ uint32_t s_top[2];  // bits of the largest finite V scale, of this stage and the next
-    if (static_cast<int>(blockIdx.y) >= ldg(&a.head->units)) return;
-    const ShUnit un = a.units[blockIdx.y];
+    __shared__ __attribute__((aligned(1024))) uint8_t s_kv[kShKeys * ROWB + HD * VROWB];
+    uint8_t *const s_k = s_kv, *const s_v = s_kv + kShKeys * ROWB;
+    // scales, zeros for tokens that are not there; K's times scale_log2
+    __shared__ __attribute__((aligned(16))) float s_ks[G][kShKeys];
+    __shared__ __attribute__((aligned(16))) uint16_t s_vs[G][kShKeys];
+    __shared__ uint32_t s_valid;   // a byte for each 16 tokens of the stage: they have a page
+    __shared__ __attribute__((aligned(8))) float s_top[2][2];  // bits of the largest finite V scale, by two waves, two stages
+    __shared__ f32x2 s_state[2][32];  // (base, weight) of a wave's columns
+    const int units = ldg(&a.head->units);
+    const ShUnit un = a.units[blockIdx.y];  // (read whether there is one or not: one round trip)
+    if (static_cast<int>(blockIdx.y) >= units) return;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 31, hh = lane >> 5;
-    const int kvh = blockIdx.x, cwave = wave % un.cw, kwave = wave / un.cw, kw = kShWaves / un.cw;
+    const int kvh = blockIdx.x, cwave = wave % un.cw, kwave = wave / un.cw;
+    const int kw = un.cw == 4 ? 1 : 2;  // waves that share a stage's tokens (cw 1 leaves two that only unpack)
     const int wcols = un.ncols - 32 * cwave;  // columns of this wave
     const int col = un.col0 + 32 * cwave + (n < wcols ? n : 0);
 
@@ -239,101 +269,151 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
     }
 
     // The stage's bytes in registers. K piece t: token k_key(t), words 4 k_p .. + 3. V: tokens 16 j + 4 vh + 0 .. 3 and + 8 .. 11,
-    // dimensions 16 x + m.
-    auto k_key = [&](int t) { return (tid + kShThreads * t) / PK; };
-    const int k_p = tid % PK, m = tid & 15, vh = (tid >> 4) & 1, j = tid >> 5;
+    // dimensions 64 (v_u + u) + 16 k + m.
+    const bool has_k = HD > 64 || tid >= kShThreads / 2, has_v = HD > 64 || tid < kShThreads / 2;  // (the same for a wave)
+    struct Part {
+        uint32_t id, k_p, m, vh, j, v_u;
+        __device__ __forceinline__ Part()
+            : id(static_cast<uint32_t>(sh_here(static_cast<int>(threadIdx.x)))), k_p(id % PK), m(id & 15), vh((id >> 4) & 1), j((id >> 5) & 3),
+              v_u(HD > 64 ? UU * (id >> 7) : 0) {}
+        __device__ __forceinline__ int k_key(int t) const {
+            return ((HD > 64 ? id : id & (kShThreads / 2 - 1)) + kShThreads * t) / PK;
+        }
+    };
     u32x4 kraw[KT];
     uint16_t ksc[KT];  // the token's scale of group k_p, if there is one
-    u32x2 vraw[VT][2][UU], vsc;  // lanes m < 2 G: the scales of four tokens, + 8 (m & 1), of group m >> 1
-    int kid[KT], vid;
-    auto pages = [&](int key0, int (&ki)[KT], int& vi) {
-#pragma unroll
-        for (int t = 0; t < KT; ++t) ki[t] = key0 < un.key1 ? kv4_page(c, un.row, key0 + k_key(t)) : -1;
-        vi = key0 < un.key1 ? kv4_page(c, un.row, key0 + 16 * j) : -1;
+    u32x2 vraw[2][UU], vsc;  // lanes m < 2 G: the scales of four tokens, + 8 (m & 1), of group m >> 1
+    constexpr int NID = BIG ? 1 : KT + 1;  // page table entries of a stage: its one page, or the K pieces' and V's
+    int ids[NID];                          // pages, -1: none
+    // The entries as the table has them, without a branch: nothing waits for them here.
+    const int32_t* table = c.table + static_cast<int64_t>(un.row) * c.max_blocks;
+    auto entry = [&](int pos) {
+        const int blk = pos >> c.page_shift;
+        return ldg(table + (blk < c.max_blocks ? blk : 0));
     };
-    auto head_of = [&](int id) { return static_cast<int64_t>(id < 0 ? 0 : id) * c.NKV + kvh; };
-    auto fetch = [&](int key0) {
+    auto page = [&](int pos, int id) { return pos >> c.page_shift < c.max_blocks && id >= 0 && id < c.P ? id : -1; };
+    auto pages = [&](int key0, int (&e)[NID]) {
+        if constexpr (BIG) {
+            e[0] = entry(key0);
+        } else {
+            const Part p;
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-            const int slot = (key0 + k_key(t)) & (c.page - 1);
-            const int64_t h = head_of(kid[t]);
-            kraw[t] = ldg(reinterpret_cast<const u32x4*>(c.k_pages + (h * c.page + slot) * (HD / 2) + 16 * k_p));
-            ksc[t] = ldg(c.k_scale + (h * G + (k_p < G ? k_p : 0)) * c.page + slot);
+            for (int t = 0; t < KT; ++t) e[t] = entry(key0 + p.k_key(t));
+            e[KT] = entry(key0 + 16 * p.j);
         }
-        const int slot = (key0 + 16 * j + 4 * vh) & (c.page - 1);
-        const int64_t h = head_of(vid);
-        const uint8_t* vp = c.v_pages + h * c.page * (HD / 2) + (slot >> 2) * (16 * U * 8) + m * (U * 8);
-        vsc = ldg(reinterpret_cast<const u32x2*>(c.v_scale + (h * G + (m < 2 * G ? m >> 1 : 0)) * c.page + slot + 8 * (m & 1)));
+    };
+    auto check = [&](int key0, const int (&e)[NID]) {
+        if constexpr (BIG) {
+            ids[0] = page(key0, __builtin_amdgcn_readfirstlane(e[0]));
+        } else {
+            const Part p;
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
+            for (int t = 0; t < KT; ++t) ids[t] = page(key0 + p.k_key(t), e[t]);
+            ids[KT] = page(key0 + 16 * p.j, e[KT]);
+        }
+    };
+    // (page, head) of an entry; every one of them takes 256 bytes or more, so their number has 31 bits
+    auto head_of = [&](int id) { return static_cast<uint32_t>(id < 0 ? 0 : id) * static_cast<uint32_t>(c.NKV) + kvh; };
+    const uint32_t page_bytes = c.page * (HD / 2), scale_count = G * c.page;
+    auto fetch = [&](int key0) {
+        const Part p;
+        const int lead = key0 & (c.page - 1);  // BIG: the stage's first slot
+        if (has_k) {
+#pragma unroll
+            for (int t = 0; t < KT; ++t) {
+                const uint64_t h = head_of(ids[BIG ? 0 : t]);
+                const uint32_t slot = BIG ? p.k_key(t) : (key0 + p.k_key(t)) & (c.page - 1), g = p.k_p < G ? p.k_p : 0;
+                const uint8_t* kp = c.k_pages + (h * page_bytes + (BIG ? lead * (HD / 2) : 0));
+                const uint16_t* sp = c.k_scale + (h * scale_count + (BIG ? lead : 0));
+                kraw[t] = ldg(reinterpret_cast<const u32x4*>(kp + (slot * (HD / 2) + 16 * p.k_p)));
+                ksc[t] = ldg(sp + (g * c.page + slot));
+            }
+        }
+        if (has_v) {
+            const uint64_t h = head_of(ids[NID - 1]);
+            const uint32_t first = 16 * p.j + 4 * p.vh, slot = BIG ? first : (key0 + first) & (c.page - 1);
+            const uint8_t* vp = c.v_pages + (h * page_bytes + (BIG ? lead * (HD / 2) : 0));
+            const uint16_t* sp = c.v_scale + (h * scale_count + (BIG ? lead : 0));
+            const uint32_t off = (slot >> 2) * (16 * U * 8) + (p.m * U + p.v_u) * 8;
+            vsc = ldg(reinterpret_cast<const u32x2*>(sp + ((p.m < 2 * G ? p.m >> 1 : 0) * c.page + slot + 8 * (p.m & 1))));
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 if constexpr (UU == 1) {
-                    vraw[t][x][0] = ldg(reinterpret_cast<const u32x2*>(vp + x * 2 * (16 * U * 8)));
+                    vraw[x][0] = ldg(reinterpret_cast<const u32x2*>(vp + (off + x * 2 * (16 * U * 8))));
                 } else {
-                    const u32x4 r = ldg(reinterpret_cast<const u32x4*>(vp + x * 2 * (16 * U * 8) + 16 * t));
-                    vraw[t][x][0] = u32x2{r.x, r.y};
-                    vraw[t][x][1] = u32x2{r.z, r.w};
+                    const u32x4 r = ldg(reinterpret_cast<const u32x4*>(vp + (off + x * 2 * (16 * U * 8))));
+                    vraw[x][0] = u32x2{r.x, r.y};
+                    vraw[x][1] = u32x2{r.z, r.w};
                 }
             }
+        }
     };
     // Tokens that are not there (past the unit, or without a page) get scales 0: theirs may be anything.
-    auto unpack = [&](int key0, int odd) {
+    auto unpack_k = [&](int key0, bool whole) {
+        const Part p;
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
-            const int key = k_key(t);
-            const bool live = kid[t] >= 0 && key0 + key < un.key1;
-            if (k_p < G) s_ks[k_p][key] = live ? ksc[t] : 0;
-            uint8_t* row = s_k + key * ROWB;
+            const int key = p.k_key(t);
+            float ks = f16_bits_to_f32(ksc[t]) * a.scale_log2;
+            if (!whole) ks = ids[BIG ? 0 : t] >= 0 && key0 + key < un.key1 ? ks : 0.0f;
+            if (p.k_p < G) s_ks[p.k_p][key] = ks;
+            const int row = sh_here(key * ROWB);
             const uint32_t word[4] = {kraw[t].x, kraw[t].y, kraw[t].z, kraw[t].w};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const int w = 4 * k_p + x, i = HD == 256 ? 4 * (k_p & 1) + x : w % W, g = w / W;  // word W g + i: chunk 4 i + g
+                const int w = 4 * p.k_p + x, i = HD == 256 ? 4 * (p.k_p & 1) + x : w % W, g = w / W;  // word W g + i: chunk 4 i + g
                 f16x2 v[4];
                 dequant_int4x8_bitfield(word[x], v);
                 const f16x8 o = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
-                *reinterpret_cast<f16x8*>(row + (((4 * i + g) ^ sh_swz_k<HD>(key)) << 4)) = o;
+                *reinterpret_cast<f16x8*>(s_k + row + (((4 * i + g) ^ sh_swz_k<HD>(key)) << 4)) = o;
             }
         }
-        const int left = vid < 0 ? 0 : un.key1 - key0 - 16 * j - 4 * vh;  // live tokens from the thread's first on
-        if ((tid & 31) == 0) reinterpret_cast<uint8_t*>(&s_valid)[j] = vid >= 0;
-        if (m < 2 * G) {
-            uint32_t w[2] = {vsc.x, vsc.y}, most = 0;
+    };
+    auto unpack_v = [&](int key0, int odd, bool whole) {
+        const Part p;
+        const int m = p.m, vh = p.vh, j = p.j, v_u = p.v_u;
+        if (!BIG && (tid & 31) == 0) reinterpret_cast<uint8_t*>(&s_valid)[j] = ids[NID - 1] >= 0;
+        if (wave < 2) {  // (waves of v_u 0: the scales are theirs)
+            uint32_t w[2] = {vsc.x, vsc.y};
+            if (!whole) {
+                const int left = ids[NID - 1] < 0 ? 0 : un.key1 - key0 - 16 * j - 4 * vh - 8 * (m & 1);  // tokens that are there
+                w[0] = left > 1 ? w[0] : left == 1 ? w[0] & 0xffffu : 0u;
+                w[1] = left > 3 ? w[1] : left == 3 ? w[1] & 0xffffu : 0u;
+            }
+            if (m < 2 * G) *reinterpret_cast<u32x2*>(&s_vs[m >> 1][16 * j + 4 * vh + 8 * (m & 1)]) = u32x2{w[0], w[1]};
+            // (lanes past 2 G repeat group 0's first scales)
+            u16x2 t[2];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const int there = left - 8 * (m & 1) - 2 * y;
-                w[y] = there > 1 ? w[y] : there == 1 ? w[y] & 0xffffu : 0u;
-                const uint32_t lo = w[y] & 0x7fffu, hi = w[y] >> 16 & 0x7fffu;
-                most = lo < 0x7c00u && lo > most ? lo : most;
-                most = hi < 0x7c00u && hi > most ? hi : most;
+                const u16x2 v = __builtin_bit_cast(u16x2, w[y] & 0x7fff7fffu);
+                t[y] = v & (v < (uint16_t)0x7c00);
             }
-            *reinterpret_cast<u32x2*>(&s_vs[m >> 1][16 * j + 4 * vh + 8 * (m & 1)]) = u32x2{w[0], w[1]};
-            atomicMax(&s_top[odd], most);
+            const u16x2 most = __builtin_elementwise_max(t[0], t[1]);
+            const float wave_top = wave_max_bcast(static_cast<float>(max(most.x, most.y)));
+            if (lane == 0) s_top[odd][wave] = wave_top;
         }
 #pragma unroll
-        for (int t = 0; t < VT; ++t)
+        for (int u = 0; u < UU; ++u)
 #pragma unroll
-            for (int u = 0; u < UU; ++u)
+            for (int k = 0; k < 4; ++k) {
+                const int dim = 64 * (v_u + u) + 16 * k + m;
+                f16x2 v[2][2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {  // dimension 64 (UU t + u) + 16 k + m
-                    const int dim = 64 * (UU * t + u) + 16 * k + m;
-                    f16x2 v[2][2];
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t w[2] = {vraw[x][u].x, vraw[x][u].y};  // tokens (0, 1), (2, 3)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t w[2] = {vraw[t][x][u].x, vraw[t][x][u].y};  // tokens (0, 1), (2, 3)
-#pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const f16x2 bias = {(f16)-1032.0f, (f16)-1032.0f}, bias16 = {(f16)-72.0f, (f16)-72.0f};
-                            const f16x2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
-                            const uint32_t y8 = k < 2 ? w[y] : w[y] >> 8;
-                            v[x][y] = k & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(y8, 0x00f000f0u, 0x64806480u)), sixteenth,
-                                                                        bias16)
-                                            : as_f16x2(and_xor(y8, 0x000f000fu, 0x64086408u)) + bias;
-                        }
+                    for (int y = 0; y < 2; ++y) {
+                        const f16x2 bias = {(f16)-1032.0f, (f16)-1032.0f}, bias16 = {(f16)-72.0f, (f16)-72.0f};
+                        const f16x2 sixteenth = {(f16)0.0625f, (f16)0.0625f};
+                        const uint32_t y8 = k < 2 ? w[y] : w[y] >> 8;
+                        v[x][y] = k & 1 ? __builtin_elementwise_fma(as_f16x2(and_xor(y8, 0x00f000f0u, 0x64806480u)), sixteenth,
+                                                                    bias16)
+                                        : as_f16x2(and_xor(y8, 0x000f000fu, 0x64086408u)) + bias;
                     }
-                    const f16x8 o = {v[0][0].x, v[0][0].y, v[0][1].x, v[0][1].y, v[1][0].x, v[1][0].y, v[1][1].x, v[1][1].y};
-                    *reinterpret_cast<f16x8*>(s_v + dim * VROWB + (((2 * j + vh) ^ (dim & 15)) << 4)) = o;
                 }
+                const f16x8 o = {v[0][0].x, v[0][0].y, v[0][1].x, v[0][1].y, v[1][0].x, v[1][0].y, v[1][1].x, v[1][1].y};
+                *reinterpret_cast<f16x8*>(s_v + dim * VROWB + (((2 * j + vh) ^ sh_swz_v(dim)) << 4)) = o;
+            }
     };
 
     f32x16 acc[DT];
@@ -341,12 +421,13 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[d][r] = 0.0f;
-    float base = kNegBig, l = 0.0f;
+    float base = 0.0f, l = 0.0f;
+    bool fresh = true;  // no token yet
     // scale_top: binades from the stage's largest V scale up to 1
-    auto products = [&](int key0, int sub, bool whole, uint64_t valid, float scale_top) {
-        const int at = 32 * sub + 4 * hh;  // the lane's first token, the others 8 (r >> 2) + (r & 3) further
-        float z[16];
-        const uint8_t* row = s_k + (32 * sub + n) * ROWB;
+    auto products = [&](int key0, int sub, bool whole, uint32_t valid, float scale_top) {
+        const int at = sh_here(32 * sub + 4 * hh);  // the lane's first token, the others 8 (r >> 2) + (r & 3) further
+        float z[16];                                // score in binades, less the base
+        const int k_at = sh_here((32 * sub + n) * ROWB + ((hh ^ sh_swz_k<HD>(n)) << 4));  // K's chunk hh, 2 kk + hh: bits flipped
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             f32x16 sum;
@@ -354,19 +435,17 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
             for (int r = 0; r < 16; ++r) sum[r] = 0.0f;
 #pragma unroll
             for (int kk = g * (GS / 16); kk < (g + 1) * (GS / 16); ++kk) {
-                const f16x8 kf = *reinterpret_cast<const f16x8*>(row + (((2 * kk + hh) ^ sh_swz_k<HD>(n)) << 4));
+                const f16x8 kf = *reinterpret_cast<const f16x8*>(s_k + (k_at ^ (kk << 5)));
                 sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[kk], sum, 0, 0, 0);
+                if ((kk & 3) == 3) __builtin_amdgcn_sched_barrier(0);
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const u32x2 sc = *reinterpret_cast<const u32x2*>(&s_ks[g][at + 8 * x]);
-                const f16x2 lo = as_f16x2(sc.x), hi = as_f16x2(sc.y);
-                const f16 s4[4] = {lo.x, lo.y, hi.x, hi.y};
+                const f32x4 sc = *reinterpret_cast<const f32x4*>(&s_ks[g][at + 8 * x]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    z[4 * x + e] = fmaf(sum[4 * x + e], static_cast<float>(s4[e]), g ? z[4 * x + e] : 0.0f);
+                for (int e = 0; e < 4; ++e) z[4 * x + e] = fmaf(sum[4 * x + e], sc[e], g ? z[4 * x + e] : -base);
             }
-            if (HD == 256) __builtin_amdgcn_sched_barrier(0);  // (all groups at once would spill)
+            __builtin_amdgcn_sched_barrier(0);  // (all groups at once would spill)
         }
         if (!whole) {
             const int left = un.key1 - key0 - at;
@@ -379,74 +458,108 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD)) void kv4_shared_kernel(c
         float top = z[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, z[r]);
-        top = fmaf(fmaxf(top, xor_lanes<32>(top)), a.scale_log2, -scale_top);
-        // the base rises only where a product would pass 2^kShHigh, to where the largest is 2^kShLow; a column does not depend
-        // on its neighbours
-        if (ballot(top > base + kShHigh)) {
-            const float up = top > base + kShHigh ? top - kShLow : base, w = fast_exp2(base - up);
-            base = up;
+        top = fmaxf(top, xor_lanes<32>(top)) - scale_top;
+        // the base rises only where a product would pass 2^kShHigh, to where the largest is 2^kShLow (and is set so by the first
+        // token that is there); a column does not depend on its neighbours
+        const bool raise = top > kShHigh || (fresh && top > -__builtin_inff());
+        if (ballot(raise)) {
+            const float by = raise ? top - kShLow : 0.0f, w = fresh ? 0.0f : fast_exp2(-by);
+            fresh = fresh && !raise;
+            base += by;
             l *= w;
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[d][r] *= w;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z[r] -= by;
         }
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            z[r] = fast_exp2(fmaf(z[r], a.scale_log2, -base));
+            z[r] = fast_exp2(z[r]);
             l += z[r];
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            f16x8 pb[2];
+            u32x4 pb[2];
+            const int v_at = sh_here(n * VROWB + (((4 * sub + hh) ^ sh_swz_v(n)) << 4));
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const u32x2 sc = *reinterpret_cast<const u32x2*>(&s_vs[g][at + 8 * x]);
-                const f16x2 lo = as_f16x2(sc.x), hi = as_f16x2(sc.y);
-                const f16 s4[4] = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-                for (int e = 0; e < 4; ++e)  // (fma, not a product: one mixed-precision instruction)
-                    pb[x >> 1][4 * (x & 1) + e] = static_cast<f16>(fmaf(z[4 * x + e], static_cast<float>(s4[e]), 0.0f));
+                pb[x >> 1][2 * (x & 1)] = times_f16(z[4 * x], z[4 * x + 1], sc.x);
+                pb[x >> 1][2 * (x & 1) + 1] = times_f16(z[4 * x + 2], z[4 * x + 3], sc.y);
             }
 #pragma unroll
             for (int d = g * (GS / 32); d < (g + 1) * (GS / 32); ++d) {
-                const uint8_t* vrow = s_v + (32 * d + n) * VROWB;
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const f16x8 vf = *reinterpret_cast<const f16x8*>(vrow + (((4 * sub + 2 * x + hh) ^ (n & 15)) << 4));
-                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pb[x], acc[d], 0, 0, 0);
+                    const f16x8 vf = *reinterpret_cast<const f16x8*>(s_v + (v_at ^ (x << 5)) + 32 * d * VROWB);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, __builtin_bit_cast(f16x8, pb[x]), acc[d], 0, 0, 0);
                 }
             }
-            if (HD == 256) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    pages(un.key0, kid, vid);
+    int next[NID];
+    pages(un.key0, next);
+    check(un.key0, next);
+    pages(un.key0 + kShKeys, next);
     fetch(un.key0);
-    if (tid < 2) s_top[tid] = 0;
-    sh_meet();
     int odd = 0;
     for (int key0 = un.key0; key0 < un.key1; key0 += kShKeys, odd ^= 1) {
-        int next_kid[KT], next_vid;
-        pages(key0 + kShKeys, next_kid, next_vid);
         if (key0 > un.key0) sh_meet();  // the stage before is read
-        unpack(key0, odd);
-        if (tid == 0) s_top[odd ^ 1] = 0;
-#pragma unroll
-        for (int t = 0; t < KT; ++t) kid[t] = next_kid[t];
-        vid = next_vid;
-        if (key0 + kShKeys < un.key1) fetch(key0 + kShKeys);
+        const bool inside = key0 + kShKeys <= un.key1, there = BIG && ids[0] >= 0;
+        if (has_k) unpack_k(key0, inside && there);
+        if (has_v) unpack_v(key0, odd, inside && there);
+        if (key0 + kShKeys < un.key1) {
+            check(key0 + kShKeys, next);
+            fetch(key0 + kShKeys);
+            pages(key0 + 2 * kShKeys, next);
+        }
         sh_meet();
-        const uint64_t valid = s_valid;
-        const bool whole = key0 + kShKeys <= un.key1 && valid == 0x0101010101010101ull;
-        const float scale_top = 14.0f - static_cast<float>(s_top[odd] >> 10);  // (the exponent's bits: scales below 2^(bits - 14))
-        if (wcols > 0)
-            for (int sub = kwave; sub < kShKeys / 32; sub += kw)
-                if (key0 + 32 * sub < un.key1) products(key0, sub, whole, valid, scale_top);
+        const uint32_t valid = BIG ? (there ? 0x01010101u : 0u) : s_valid;
+        const bool whole = inside && valid == 0x01010101u;
+        const f32x2 tops = *reinterpret_cast<const f32x2*>(s_top[odd]);
+        const int top_bits = static_cast<int>(fmaxf(tops.x, tops.y));
+        const float scale_top = 14.0f - static_cast<float>(top_bits >> 10);  // (the exponent's bits: scales below 2^(bits - 14))
+        if (wcols <= 0 || kwave >= kw) continue;
+        const int subs = min(kShKeys / 32, (un.key1 - key0 + 31) >> 5);
+        for (int sub = kwave; sub < subs; sub += kw) products(key0, sub, whole, valid, scale_top);
     }
-    if (n >= wcols) return;  // (no barrier from here on)
+    if (fresh) base = kNegBig;
     l += xor_lanes<32>(l);
-    float* st = a.part + (static_cast<int64_t>(kvh) * a.states + un.state + kwave * un.step + 32 * cwave + n) * (HD + 4);
+    // the second of two waves that share the unit's tokens hands its state to the first through LDS, where K and V were
+    if (kw > 1) {
+        static_assert(2 * 32 * HD * 4 <= kShKeys * ROWB + HD * VROWB, "room for two waves' states");
+        uint8_t* st = s_kv + (cwave * 32 + n) * HD * 4;
+        sh_meet();
+        if (kwave == 1) {
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    *reinterpret_cast<f32x4*>(st + (((8 * d + 2 * x + hh) ^ (n & 15)) << 4)) =
+                        f32x4{acc[d][4 * x], acc[d][4 * x + 1], acc[d][4 * x + 2], acc[d][4 * x + 3]};
+            if (hh == 0) s_state[cwave][n] = f32x2{base, l};
+        }
+        sh_meet();
+        if (kwave > 0) return;
+        const f32x2 bl = s_state[cwave][n];
+        const float top = fmaxf(base, bl.x), w0 = fast_exp2(base - top), w1 = fast_exp2(bl.x - top);
+        base = top;
+        l = fmaf(l, w0, bl.y * w1);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const f32x4 v = *reinterpret_cast<const f32x4*>(st + (((8 * d + 2 * x + hh) ^ (n & 15)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[d][4 * x + e] = fmaf(acc[d][4 * x + e], w0, v[e] * w1);
+            }
+    }
+    if (n >= wcols) return;
+    float* st = a.part + (static_cast<int64_t>(kvh) * a.states + un.state + 32 * cwave + n) * (HD + 4);
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -470,28 +583,34 @@ __global__ __launch_bounds__(256) void kv4_shared_combine_kernel(const ShArgs a)
         const int at = i < s.pre_n ? s.pre + i * s.pre_step + r : s.own + (i - s.pre_n) * a.rep + r;
         return part + static_cast<int64_t>(at) * (HD + 4);
     };
-    float M = kNegBig;
-    for (int i = lane; i < ns; i += kWave) M = fmaxf(M, ldg(state(i) + HD));
+    // the first states' sums are requested with the (base, weight) pairs: up to kFirst states are two round trips
+    constexpr int kFirst = 16;
+    auto pair = [&](int i) { return i < ns ? ldg(reinterpret_cast<const f32x2*>(state(i) + HD)) : f32x2{kNegBig, 0.0f}; };
+    float x[kFirst][E];
+    auto load = [&](int i0) {
+#pragma unroll
+        for (int k = 0; k < kFirst; ++k)
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[k][e] = i0 + k < ns ? ldg(state(i0 + k) + 64 * e + lane) : 0.0f;
+    };
+    const f32x2 first = pair(lane);
+    load(0);
+    float M = first.x;
+    for (int i = lane + kWave; i < ns; i += kWave) M = fmaxf(M, ldg(state(i) + HD));
     M = wave_max_bcast(M);
     float l = 0.0f, v[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = 0.0f;
     for (int i0 = 0; i0 < ns; i0 += kWave) {
-        f32x2 ml = {kNegBig, 0.0f};
-        if (i0 + lane < ns) ml = ldg(reinterpret_cast<const f32x2*>(state(i0 + lane) + HD));
+        const f32x2 ml = i0 ? pair(i0 + lane) : first;
         const float w = fast_exp2(ml.x - M);
         l = fmaf(ml.y, w, l);
-        const int here = ns - i0 < kWave ? ns - i0 : kWave;
-        for (int i = 0; i < here; i += 4) {
-            float x[4][E];
+        for (int i = i0; i < ns && i < i0 + kWave; i += kFirst) {
+            if (i) load(i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int e = 0; e < E; ++e) x[k][e] = ldg(state(i0 + (i + k < here ? i + k : i)) + 64 * e + lane);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (i + k >= here) break;
-                const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i + k));
+            for (int k = 0; k < kFirst; ++k) {
+                if (i + k >= ns) break;
+                const float wk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i - i0 + k));
 #pragma unroll
                 for (int e = 0; e < E; ++e) v[e] = fmaf(x[k][e], wk, v[e]);
             }
@@ -503,6 +622,8 @@ __global__ __launch_bounds__(256) void kv4_shared_combine_kernel(const ShArgs a)
         stg(a.out + (static_cast<int64_t>(b) * a.NQ + h) * HD + 64 * e + lane, f32_to_f16_bits(l == 0.0f ? 0.0f : v[e] / l));
 }
 
+// Units aimed at: two workgroups to a CU (one for heads of 256). 64 sequences of up to 512 tokens behind 8192 shared ones, 32 /
+// 8 heads of 128, with 1 / 2 / 4 / 8: 55 / 37 / 45 / 45 us for the units and 6 / 8 / 14 / 26 us to add up their states.
 // The most units and states there can be. Each of the plan's splits but a tile's last costs at least a unit's share, so there
 // are at most `want` units more than tiles.
 struct ShSizes {
@@ -510,7 +631,7 @@ struct ShSizes {
     ShSizes(int64_t B, int64_t G, int64_t NQ, int64_t NKV, int64_t hd, int64_t max_len, int64_t max_shared) {
         const int64_t rep = NQ / NKV, per_group = ceil_div64(B * rep, G < 1 ? 1 : G);
         cw = per_group > 64 ? 4 : per_group > 32 ? 2 : 1;
-        want = ceil_div64(256 * sh_per_cu(static_cast<int>(hd)), NKV);
+        want = ceil_div64(256 * (hd == 256 ? 1 : 2), NKV);
         const int64_t pre_tiles = B * rep / (32 * cw) + G, own_tiles = B * ceil_div64(rep, 32);
         auto units_of = [&](int64_t tiles, int64_t keys) {
             const int64_t most = tiles * ceil_div64(keys, kShKeys);
@@ -518,7 +639,7 @@ struct ShSizes {
         };
         const int64_t pre = units_of(pre_tiles, max_shared), own = units_of(own_tiles, max_len);
         units = pre + own;
-        states = pre * 32 * kShWaves + own * kShWaves * (rep < 32 ? rep : 32);
+        states = pre * 32 * cw + own * (rep < 32 ? rep : 32);
     }
     size_t bytes(int64_t B, int64_t NKV, int64_t hd) const {
         return sizeof(ShHead) + units * sizeof(ShUnit) + B * sizeof(ShSeq) + static_cast<size_t>(NKV) * states * (hd + 4) * 4;
@@ -590,10 +711,17 @@ extern "C" int soi_kv4_shared_attention(const soi_kv4_cache* cache, const uint16
     a.scale_log2 = scale * kLog2e;
     const Kv4Cache c = kv4_device(cache);
     hipStream_t s = as_stream(stream);
-    hipLaunchKernelGGL(kv4_shared_plan_kernel, dim3(1), dim3(kShPlan), 0, s, a, c);
+    if (B <= 256 && groups <= 256) hipLaunchKernelGGL(kv4_shared_plan_kernel<256>, dim3(1), dim3(256), 0, s, a, c);
+    else hipLaunchKernelGGL(kv4_shared_plan_kernel<1024>, dim3(1), dim3(1024), 0, s, a, c);
     if (sz.units > 0) {
         const dim3 grid(static_cast<unsigned>(NKV), static_cast<unsigned>(sz.units));
-#define SOI_X(H, G) hipLaunchKernelGGL((kv4_shared_kernel<H, G>), grid, dim3(kShThreads), 0, s, a, c)
+#define SOI_X(H, G)                                                                                              \
+    do {                                                                                                         \
+        if (cache->page_size >= kShKeys)                                                                         \
+            hipLaunchKernelGGL((kv4_shared_kernel<H, G, true>), grid, dim3(kShThreads), 0, s, a, c);             \
+        else                                                                                                     \
+            hipLaunchKernelGGL((kv4_shared_kernel<H, G, false>), grid, dim3(kShThreads), 0, s, a, c);            \
+    } while (0)
         SOI_KV4_SHAPES(SOI_X);
 #undef SOI_X
     }
