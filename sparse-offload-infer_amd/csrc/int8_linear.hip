@@ -26,51 +26,69 @@ struct I8Args {
     const uint16_t* res;
     uint16_t* y;
     int T, N, K;
-    int ks;    // few rows: the waves of a workgroup that share a row of weights
-    int quad;  // the outputs of four neighbouring n, and what is read with them, lie on whole 8 or 16 bytes
+    int wide;  // 1: the outputs of four neighbouring n, and what is read with them, lie on whole 8 or 16 bytes; 2: eight outputs on 16
 };
 
-// Output n .. n + 3 of token t from their sums (g, and u where GATED).
+// silu with the hardware's exponential and reciprocal (2^-22 each, next to a rounding to 2^-11): the library's exponential and
+// an exact quotient took a third of gate_up's time at 8192 rows.
+__device__ __forceinline__ float i8_silu(float g) {
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.4426950408889634f));
+}
+
+// The weights' scales of outputs n .. n + 3.
 template <bool GATED>
-__device__ __forceinline__ void i8_values(const I8Args& a, int t, int n, const i32x4& g, const i32x4& u, float (&v)[4]) {
-    const float sx = ldg(a.sx + t);
-    float sg[4], su[4];
-    if (a.quad) {
-        const f32x4 s = ldg(reinterpret_cast<const f32x4*>(a.sw + n));
+struct I8Scales {
+    float g[4], u[GATED ? 4 : 1];
+};
+template <bool GATED>
+__device__ __forceinline__ I8Scales<GATED> i8_scales(const I8Args& a, int n) {
+    I8Scales<GATED> s;
+    auto four = [&](const float* p, float* o) {
+        if (a.wide) {
+            const f32x4 v = ldg(reinterpret_cast<const f32x4*>(p + n));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sg[e] = s[e];
-        if constexpr (GATED) {
-            const f32x4 r = ldg(reinterpret_cast<const f32x4*>(a.sw2 + n));
+            for (int e = 0; e < 4; ++e) o[e] = v[e];
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) su[e] = r[e];
+            for (int e = 0; e < 4; ++e) o[e] = ldg(p + (n + e < a.N ? n + e : a.N - 1));
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = n + e < a.N ? n + e : a.N - 1;
-            sg[e] = ldg(a.sw + i);
-            if constexpr (GATED) su[e] = ldg(a.sw2 + i);
-        }
-    }
+    };
+    four(a.sw, s.g);
+    if constexpr (GATED) four(a.sw2, s.u);
+    return s;
+}
+
+// Four outputs of a token with scale sx from their sums (g, and u where GATED).
+template <bool GATED>
+__device__ __forceinline__ void i8_values(float sx, const I8Scales<GATED>& s, const i32x4& g, const i32x4& u, float (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        v[e] = static_cast<float>(g[e]) * sg[e] * sx;
-        if constexpr (GATED) v[e] = silu_f32(v[e]) * (static_cast<float>(u[e]) * su[e] * sx);
+        v[e] = static_cast<float>(g[e]) * s.g[e] * sx;
+        if constexpr (GATED) v[e] = i8_silu(v[e]) * (static_cast<float>(u[e]) * s.u[e] * sx);
     }
 }
 
-// stores them, the residual added
-__device__ __forceinline__ void i8_store(const I8Args& a, int t, int n, float (&v)[4]) {
+// two outputs; rounded to binary32 first in every kernel, so that a row's bits do not follow from the tile it is in
+__device__ __forceinline__ float i8_pack(float a, float b) {
+    asm("" : "+v"(a), "+v"(b));
+    return __builtin_bit_cast(float, f16x2{static_cast<f16>(a), static_cast<f16>(b)});
+}
+
+// the residual of outputs n .. n + 3, where they are wide
+__device__ __forceinline__ void i8_add(const I8Args& a, int t, int n, float (&v)[4]) {
+    const u32x2 r = ldg(reinterpret_cast<const u32x2*>(a.res + static_cast<int64_t>(t) * a.N + n));
+    const f16x2 lo = as_f16x2(r.x), hi = as_f16x2(r.y);
+    v[0] += static_cast<float>(lo.x);
+    v[1] += static_cast<float>(lo.y);
+    v[2] += static_cast<float>(hi.x);
+    v[3] += static_cast<float>(hi.y);
+}
+
+// the residual added, and the outputs stored
+__device__ __forceinline__ void i8_finish(const I8Args& a, int t, int n, float (&v)[4]) {
     const int64_t at = static_cast<int64_t>(t) * a.N + n;
-    if (a.quad) {
-        if (a.res) {
-            const u32x2 r = ldg(reinterpret_cast<const u32x2*>(a.res + at));
-            const f16x2 lo = as_f16x2(r.x), hi = as_f16x2(r.y);
-            v[0] += static_cast<float>(lo.x);
-            v[1] += static_cast<float>(lo.y);
-            v[2] += static_cast<float>(hi.x);
-            v[3] += static_cast<float>(hi.y);
-        }
+    if (a.wide) {
+        if (a.res) i8_add(a, t, n, v);
         stg(reinterpret_cast<u32x2*>(a.y + at), u32x2{pack_f16x2(v[0], v[1]), pack_f16x2(v[2], v[3])});
         return;
     }
@@ -80,106 +98,17 @@ __device__ __forceinline__ void i8_store(const I8Args& a, int t, int n, float (&
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: the weights' bytes bound it, so they go straight from memory to the matrix cores, each once. A wave has R tiles
-// of 16 weight rows (GATED: half of them of either matrix) against C tiles of 16 activation rows, whose bytes come from the
-// caches; `ks` waves of a workgroup split K and add their sums up through LDS.
+// Many rows: tiles of BN weight rows x BT activation rows, STEP bytes of K a stage, NBUF stages in LDS. A stage goes from
+// memory into LDS without passing through registers, NBUF - 1 stages ahead; 16-byte chunks are XOR-swizzled on the way, so that
+// the operand reads of 32 rows spread over the banks.
 // ---------------------------------------------------------------------------
-constexpr int kFewWaves = 8;
-
-template <int R, int C, bool GATED>
-__global__ __launch_bounds__(kFewWaves * kWave) void int8_few_kernel(const I8Args a) {
-    constexpr int U = 4, RN = GATED ? R / 2 : R;  // 64-byte steps in flight; tiles of n
-    __shared__ i32x4 s_sum[kFewWaves][R * C][kWave];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
-    const int part = wave % a.ks, team = wave / a.ks, teams = kFewWaves / a.ks;
-    const int n0 = (static_cast<int>(blockIdx.x) * teams + team) * 16 * RN, t0 = static_cast<int>(blockIdx.y) * 16 * C;
-    const int8_t *wp[R], *xp[C];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int n = n0 + 16 * (GATED ? r >> 1 : r) + col;
-        const int8_t* base = GATED && (r & 1) ? a.w2 : a.w;
-        wp[r] = base + static_cast<int64_t>(n < a.N ? n : a.N - 1) * a.K + 16 * g;
-    }
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-        const int t = t0 + 16 * c + col;
-        xp[c] = a.x + static_cast<int64_t>(t < a.T ? t : a.T - 1) * a.K + 16 * g;
-    }
-    i32x4 acc[R][C];
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int c = 0; c < C; ++c) acc[r][c] = i32x4{0, 0, 0, 0};
-    auto step = [&](int k, auto WHOLE) {
-        u32x4 w[R][U], x[C][U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = WHOLE || k + 64 * u + 16 * g < a.K;
-            const auto* zero = reinterpret_cast<const int8_t*>(g_zero16);
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-                w[r][u] = ldg_stream(reinterpret_cast<const u32x4*>(in ? wp[r] + k + 64 * u : zero));
-#pragma unroll
-            for (int c = 0; c < C; ++c) x[c][u] = ldg(reinterpret_cast<const u32x4*>(in ? xp[c] + k + 64 * u : zero));
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int c = 0; c < C; ++c)
-                    acc[r][c] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w[r][u]),
-                                                                      __builtin_bit_cast(i32x4, x[c][u]), acc[r][c], 0, 0, 0);
-    };
-    if (n0 < a.N)
-        for (int k = part * 64 * U; k < a.K; k += a.ks * 64 * U) {
-            if (k + 64 * U <= a.K) step(k, std::true_type{});
-            else step(k, std::false_type{});
-        }
-    // tile (r, c) of a lane: token 16 c + col, outputs 16 r + 4 g + 0 .. 3
-    auto finish = [&](int tile, const i32x4& s0, const i32x4& s1) {  // tile: of n and t
-        const int t = t0 + 16 * (tile % C) + col, n = n0 + 16 * (tile / C) + 4 * g;
-        if (t < a.T && n < a.N) {
-            float v[4];
-            i8_values<GATED>(a, t, n, s0, s1, v);
-            i8_store(a, t, n, v);
-        }
-    };
-    if (a.ks == 1) {
-#pragma unroll
-        for (int r = 0; r < RN; ++r)
-#pragma unroll
-            for (int c = 0; c < C; ++c) finish(r * C + c, acc[GATED ? 2 * r : r][c], acc[GATED ? 2 * r + 1 : r][c]);
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int c = 0; c < C; ++c) s_sum[wave][r * C + c][lane] = acc[r][c];
-    __syncthreads();
-    auto total = [&](int i) {
-        i32x4 s = s_sum[team * a.ks][i][lane];
-        for (int k = 1; k < a.ks; ++k) s += s_sum[team * a.ks + k][i][lane];
-        return s;
-    };
-    for (int tile = part; tile < RN * C; tile += a.ks) {
-        if constexpr (GATED) finish(tile, total(2 * (tile / C) * C + tile % C), total((2 * (tile / C) + 1) * C + tile % C));
-        else finish(tile, total(tile), i32x4{0, 0, 0, 0});
-    }
+template <int STEP>
+__device__ __forceinline__ int i8_swz(int row) {
+    return STEP == 128 ? (row >> 1) & 7 : (row >> 2) & 3;
 }
 
-// ---------------------------------------------------------------------------
-// Many rows: tiles of BN weight rows x BT activation rows, kI8Step bytes of K a stage, two stages in LDS. A stage goes from
-// memory into LDS without passing through registers, during the products of the stage before; 16-byte chunks are XOR-swizzled
-// on the way, so that the operand reads of 32 rows spread over the banks.
-// ---------------------------------------------------------------------------
-constexpr int kI8Step = 128;
-
-__device__ __forceinline__ int i8_swz(int row) { return (row >> 1) & 7; }
-
-// 1 KB pieces (8 rows of a stage) into LDS: lane offsets `off` from `base`, zeros from `bytes` on. In asm because the compiler
-// would let every LDS read wait for the loads in flight (the kernel waits for them itself, at the barrier). m0 holds the LDS
+// 1 KB pieces of a stage into LDS: lane offsets `off` from `base`, zeros from `bytes` on. In asm because the compiler would
+// let every LDS read wait for the loads in flight (the kernel waits for them itself, at the barrier). m0 holds the LDS
 // address; with the s_nop the load is 5 wait states behind whatever wrote the descriptor's registers.
 template <int LOADS>
 __device__ __forceinline__ void i8_load(const int8_t* base, int bytes, const uint32_t (&off)[LOADS], uint32_t lds) {
@@ -195,12 +124,14 @@ __device__ __forceinline__ void i8_load(const int8_t* base, int bytes, const uin
 }
 
 // WN x WT waves, each with NI x TI tiles of 32 x 32. GATED: odd 32-row strips of the weights' tile are the second matrix's.
-template <int WN, int WT, int NI, int TI, bool GATED, int OCC>
+template <int WN, int WT, int NI, int TI, int STEP, int NBUF, bool GATED, int OCC>
 __global__ __launch_bounds__(WN * WT * kWave, OCC) void int8_many_kernel(const I8Args a, int ntiles, int ttiles) {
-    constexpr int NW = WN * WT, BN = 32 * WN * NI, BT = 32 * WT * TI, STAGE = (BN + BT) * kI8Step;
-    constexpr int WL = BN / 8 / NW, XL = BT / 8 / NW;  // 1 KB loads of a wave and stage
-    static_assert(BN % (8 * NW) == 0 && BT % (8 * NW) == 0, "whole loads per wave");
-    __shared__ __attribute__((aligned(1024))) uint8_t s_tile[2][STAGE];
+    constexpr int NW = WN * WT, BN = 32 * WN * NI, BT = 32 * WT * TI, STAGE = (BN + BT) * STEP, CH = STEP / 16, RL = 1024 / STEP;
+    constexpr int WL = BN / RL / NW, XL = BT / RL / NW;  // 1 KB loads of a wave and stage, RL rows each
+    static_assert(BN % (RL * NW) == 0 && BT % (RL * NW) == 0, "whole loads per wave");
+    constexpr int SL = 32 / RL;  // loads of a strip
+    static_assert(!GATED || SL % WL == 0 || WL % (2 * SL) == 0, "a wave's loads of weights are parts of a strip, or pairs of them");
+    __shared__ __attribute__((aligned(1024))) uint8_t s_tile[NBUF * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wn = wave % WN, wt = wave / WN, m = lane & 31, hh = lane >> 5;
     // Workgroups go to the XCDs in turn: each XCD takes a contiguous part of the tiles, and walks it in blocks of 4 token tiles
@@ -216,54 +147,60 @@ __global__ __launch_bounds__(WN * WT * kWave, OCC) void int8_many_kernel(const I
     const int high = min(GT, ttiles - band * GT);
     const int n0 = (in / high) * (GATED ? BN / 2 : BN), t0 = (band * GT + in % high) * BT;
 
-    // The lane's chunk of each load: row 8 i + lane / 8 of the wave's part, physical chunk lane % 8. Rows past the matrix are
-    // past the descriptor's end; GATED: a wave's loads of a strip stay inside one matrix.
+    // The lane's chunk of each load: row RL i + lane / CH of the wave's part, physical chunk lane % CH. Rows past the matrix are
+    // past the descriptor's end.
     uint32_t wo[WL], xo[XL];
-    const int c8 = lane & 7;
+    auto chunk = [&](int r) { return 16 * ((lane & (CH - 1)) ^ i8_swz<STEP>(r)); };
+    auto row_of = [&](int i) { return i * RL + lane / CH; };
 #pragma unroll
     for (int i = 0; i < WL; ++i) {
-        const int r = (wave * WL + i) * 8 + (lane >> 3);
-        const int row = GATED ? (r >> 6) * 32 + (r & 31) : r;
-        wo[i] = static_cast<uint32_t>(row) * a.K + 16 * (c8 ^ i8_swz(r));
+        const int r = row_of(wave * WL + i);
+        wo[i] = static_cast<uint32_t>(GATED ? (r >> 6) * 32 + (r & 31) : r) * a.K + chunk(r);
     }
 #pragma unroll
     for (int i = 0; i < XL; ++i) {
-        const int r = (wave * XL + i) * 8 + (lane >> 3);
-        xo[i] = static_cast<uint32_t>(r) * a.K + 16 * (c8 ^ i8_swz(r));
+        const int r = row_of(wave * XL + i);
+        xo[i] = static_cast<uint32_t>(r) * a.K + chunk(r);
     }
-    static_assert(!GATED || WL == 4 || WL % 8 == 0, "a wave's loads of weights are whole strips");
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)&s_tile[0][0]));
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)&s_tile[0]));
     const int64_t wrows = min(a.N - n0, GATED ? BN / 2 : BN), xrows = min(a.T - t0, BT);
     const int8_t* wb = a.w + static_cast<int64_t>(n0) * a.K;
     const int8_t* wb2 = GATED ? a.w2 + static_cast<int64_t>(n0) * a.K : nullptr;
     const int8_t* xb = a.x + static_cast<int64_t>(t0) * a.K;
     const int wend = static_cast<int>(wrows * a.K), xend = static_cast<int>(xrows * a.K);
-    auto load = [&](int k0, uint32_t lds) {
-        const int left = a.K - k0;
-        uint32_t w[WL], x[XL];
-        const bool tail = left < kI8Step;  // chunks past the row's end would be the next row's
+    int at = 0;         // the next stage's first byte of a row
+    uint32_t into = 0;  // and its place in LDS
+    auto load = [&] {
+        const int left = a.K - at;
+        const int wbytes = left > 0 ? wend - at : 0, xbytes = left > 0 ? xend - at : 0;  // (nothing past the last stage)
+        const uint32_t lds = lds0 + into;
+        auto issue = [&](const uint32_t (&w)[WL], const uint32_t (&x)[XL]) {
+            if constexpr (!GATED || WL <= SL) {
+                const bool second = GATED && (wave * WL / SL) & 1;
+                i8_load<WL>((second ? wb2 : wb) + at, wbytes, w, lds + wave * WL * 1024);
+            } else {
 #pragma unroll
-        for (int i = 0; i < WL; ++i) {
-            const int r = (wave * WL + i) * 8 + (lane >> 3);
-            w[i] = tail && 16 * (c8 ^ i8_swz(r)) >= left ? 0xfffffff0u : wo[i];
-        }
+                for (int i = 0; i < WL; i += SL) {
+                    uint32_t o[SL];
 #pragma unroll
-        for (int i = 0; i < XL; ++i) {
-            const int r = (wave * XL + i) * 8 + (lane >> 3);
-            x[i] = tail && 16 * (c8 ^ i8_swz(r)) >= left ? 0xfffffff0u : xo[i];
-        }
-        if constexpr (GATED && WL == 4) {
-            i8_load<WL>((wave & 1 ? wb2 : wb) + k0, wend - k0, w, lds + wave * WL * 1024);
-        } else if constexpr (GATED) {
-#pragma unroll
-            for (int i = 0; i < WL; i += 4) {
-                const uint32_t o[4] = {w[i], w[i + 1], w[i + 2], w[i + 3]};
-                i8_load<4>((i & 4 ? wb2 : wb) + k0, wend - k0, o, lds + (wave * WL + i) * 1024);
+                    for (int e = 0; e < SL; ++e) o[e] = w[i + e];
+                    i8_load<SL>((i / SL & 1 ? wb2 : wb) + at, wbytes, o, lds + (wave * WL + i) * 1024);
+                }
             }
-        } else {
-            i8_load<WL>(wb + k0, wend - k0, w, lds + wave * WL * 1024);
+            i8_load<XL>(xb + at, xbytes, x, lds + BN * STEP + wave * XL * 1024);
+        };
+        if (left >= STEP || left <= 0) {
+            issue(wo, xo);
+        } else {  // chunks past the row's end would be the next row's
+            uint32_t w[WL], x[XL];
+#pragma unroll
+            for (int i = 0; i < WL; ++i) w[i] = chunk(row_of(wave * WL + i)) >= left ? 0xfffffff0u : wo[i];
+#pragma unroll
+            for (int i = 0; i < XL; ++i) x[i] = chunk(row_of(wave * XL + i)) >= left ? 0xfffffff0u : xo[i];
+            issue(w, x);
         }
-        i8_load<XL>(xb + k0, xend - k0, x, lds + BN * kI8Step + wave * XL * 1024);
+        at += STEP;
+        into = into == (NBUF - 1) * STAGE ? 0 : into + STAGE;
     };
 
     i32x16 acc[NI][TI];
@@ -273,87 +210,251 @@ __global__ __launch_bounds__(WN * WT * kWave, OCC) void int8_many_kernel(const I
         for (int j = 0; j < TI; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-    const uint32_t w_at = lds0 + (wn * NI * 32 + m) * kI8Step + ((hh ^ i8_swz(m)) << 4);
-    const uint32_t x_at = lds0 + BN * kI8Step + (wt * TI * 32 + m) * kI8Step + ((hh ^ i8_swz(m)) << 4);
-    load(0, lds0);
-    uint32_t cur = 0;
-    for (int k0 = 0; k0 < a.K; k0 += kI8Step) {
-        // every wave's loads of this stage have landed, and its reads of the other buffer are done
+    const uint32_t w_at = lds0 + (wn * NI * 32 + m) * STEP + ((hh ^ i8_swz<STEP>(m)) << 4);
+    const uint32_t x_at = lds0 + BN * STEP + (wt * TI * 32 + m) * STEP + ((hh ^ i8_swz<STEP>(m)) << 4);
+    // Operands of a 32-byte step are read while the step before is multiplied. The barrier between two stages lies in front of
+    // the last products of the first one, which hide it, and the reads behind it.
+    constexpr int KK = STEP / 32, kFlight = (NBUF - 2) * (WL + XL);
+    i32x4 wf[2][NI], xf[2][TI];
+    auto read = [&](int kk, uint32_t cur) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+            wf[kk & 1][i] = __builtin_bit_cast(i32x4, *(const lds_u32x4*)((lds_u8*)((w_at ^ (kk << 5)) + cur) + i * 32 * STEP));
+#pragma unroll
+        for (int j = 0; j < TI; ++j)
+            xf[kk & 1][j] = __builtin_bit_cast(i32x4, *(const lds_u32x4*)((lds_u8*)((x_at ^ (kk << 5)) + cur) + j * 32 * STEP));
+    };
+    auto multiply = [&](int kk) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < TI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[kk & 1][i], xf[kk & 1][j], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // this wave's loads of the next stage have landed, and its reads are done; after the barrier everyone's
+    auto meet = [] {
         asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_waitcnt(0x0070 | (kFlight & 15) | (kFlight >> 4) << 14);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k0 + kI8Step < a.K) load(k0 + kI8Step, lds0 + (cur ^ STAGE));
+    };
 #pragma unroll
-        for (int kk = 0; kk < kI8Step / 32; ++kk) {
+    for (int i = 0; i < NBUF - 1; ++i) load();
+    uint32_t cur = 0;
+    meet();
+    load();  // (into the last buffer, which nothing has used)
+    read(0, cur);
+    for (int k0 = 0; k0 < a.K; k0 += STEP) {
+#pragma unroll
+        for (int kk = 0; kk < KK - 1; ++kk) {
+            read(kk + 1, cur);
+            multiply(kk);
+        }
+        meet();
+        load();  // into this stage's buffer
+        cur = cur == (NBUF - 1) * STAGE ? 0 : cur + STAGE;
+        read(0, cur);
+        multiply(KK - 1);
+    }
+    // lane (m, hh): token m of a tile, outputs 8 q + 4 hh + 0 .. 3 of its 32
+    constexpr int NO = GATED ? NI / 2 : NI;
+    float sx[TI];
+#pragma unroll
+    for (int j = 0; j < TI; ++j) {
+        const int t = t0 + (wt * TI + j) * 32 + m;
+        sx[j] = ldg(a.sx + (t < a.T ? t : a.T - 1));
+    }
+    auto quad = [](const i32x16& s, int q) { return i32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]}; };
+    if (a.wide == 2) {
+        // Lanes m and m + 32 change a quad for a quad, so that each stores eight outputs side by side (N is a multiple of 8: what
+        // is past it is never stored).
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+                const int n = n0 + (wn * NO + i) * 32 + 8 * q;
+                __builtin_amdgcn_sched_barrier(0);  // (all outputs at once would spill)
+                if (n >= a.N) continue;
+                I8Scales<GATED> sc[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) sc[x] = i8_scales<GATED>(a, min(n + 8 * x, a.N - 8) + 4 * hh);
+#pragma unroll
+                for (int j = 0; j < TI; ++j) {
+                    const int t = t0 + (wt * TI + j) * 32 + m;
+                    if (t >= a.T) continue;  // (lanes m and m + 32 alike)
+                    float o[4];
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float v[4];
+                        i8_values<GATED>(sx[j], sc[x], quad(acc[GATED ? 2 * i : i][j], q + x), quad(acc[GATED ? 2 * i + 1 : i][j], q + x), v);
+                        if (!GATED && a.res && n + 8 * x < a.N) i8_add(a, t, n + 8 * x + 4 * hh, v);
+                        o[2 * x] = i8_pack(v[0], v[1]);
+                        o[2 * x + 1] = i8_pack(v[2], v[3]);
+                    }
+                    swap32(o[0], o[2]);  // the lower lanes have quad q of 8 q + 0 .. 7 now, the upper ones quad q + 1
+                    swap32(o[1], o[3]);
+                    const u32x4 w = {__builtin_bit_cast(uint32_t, o[0]), __builtin_bit_cast(uint32_t, o[1]),
+                                     __builtin_bit_cast(uint32_t, o[2]), __builtin_bit_cast(uint32_t, o[3])};
+                    if (n + 8 * hh < a.N) stg(reinterpret_cast<u32x4*>(a.y + static_cast<int64_t>(t) * a.N + n + 8 * hh), w);
+                }
+            }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int j = 0; j < TI; ++j) {
+            const int t = t0 + (wt * TI + j) * 32 + m;
+            __builtin_amdgcn_sched_barrier(0);
+            if (t >= a.T) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int n = n0 + (wn * NO + i) * 32 + 8 * q + 4 * hh;
+                if (n >= a.N) continue;
+                float v[4];
+                i8_values<GATED>(sx[j], i8_scales<GATED>(a, n), quad(acc[GATED ? 2 * i : i][j], q), quad(acc[GATED ? 2 * i + 1 : i][j], q), v);
+                i8_finish(a, t, n, v);
+            }
+        }
+}
+
+// ---------------------------------------------------------------------------
+// Few tiles (few rows, or few outputs): a tile of 32 NI weight rows (GATED: half of them of either matrix) x 32 TI activation
+// rows is a workgroup's whose eight waves share K, 64 bytes at a time in turn. A wave stages its own slices in LDS, the next one
+// on its way during a slice's products, and waits for nobody until the waves' sums are added up.
+// ---------------------------------------------------------------------------
+constexpr int kFewWaves = 8;
+
+template <int NI, int TI, bool GATED>
+__global__ __launch_bounds__(kFewWaves * kWave, 2) void int8_few_kernel(const I8Args a) {
+    constexpr int STEP = 64, WR = 32 * NI, XR = 32 * TI, STAGE = (WR + XR) * STEP, WL = 2 * NI, XL = 2 * TI, BN = GATED ? WR / 2 : WR;
+    __shared__ __attribute__((aligned(1024))) uint8_t s_tile[kFewWaves * 2 * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = lane & 31, hh = lane >> 5;
+    const int n0 = static_cast<int>(blockIdx.x) * BN, t0 = static_cast<int>(blockIdx.y) * XR;
+    // the lane's row and chunk of each 1 KB load of 16 rows
+    auto chunk = [&](int i) { return 16 * ((lane & 3) ^ i8_swz<STEP>(16 * i + (lane >> 2))); };
+    uint32_t wo[WL], xo[XL];
+#pragma unroll
+    for (int i = 0; i < WL; ++i) wo[i] = static_cast<uint32_t>((16 * i + (lane >> 2)) % BN) * a.K + chunk(i);
+#pragma unroll
+    for (int i = 0; i < XL; ++i) xo[i] = static_cast<uint32_t>(16 * i + (lane >> 2)) * a.K + chunk(i);
+    const int wend = min(a.N - n0, BN) * a.K, xend = min(a.T - t0, XR) * a.K;
+    const int8_t* wb = a.w + static_cast<int64_t>(n0) * a.K;
+    const int8_t* wb2 = GATED ? a.w2 + static_cast<int64_t>(n0) * a.K : wb;
+    const int8_t* xb = a.x + static_cast<int64_t>(t0) * a.K;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8*)&s_tile[0])) + wave * 2 * STAGE;
+    auto load = [&](int k, uint32_t lds) {  // the slice from byte k on; nothing past the rows' end, which would be the next row's
+        const int left = a.K - k, at = left > 0 ? k : 0;
+        uint32_t w[2][WL / 2], x[XL];
+#pragma unroll
+        for (int i = 0; i < WL; ++i) w[i / (WL / 2)][i % (WL / 2)] = chunk(i) < left ? wo[i] : 0xfffffff0u;
+#pragma unroll
+        for (int i = 0; i < XL; ++i) x[i] = chunk(i) < left ? xo[i] : 0xfffffff0u;
+        i8_load<WL / 2>(wb + at, wend - at, w[0], lds);
+        i8_load<WL / 2>(wb2 + at, wend - at, w[1], lds + WL / 2 * 1024);
+        i8_load<XL>(xb + at, xend - at, x, lds + WR * STEP);
+    };
+    i32x16 acc[NI][TI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < TI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    const uint32_t w_at = lds0 + m * STEP + ((hh ^ i8_swz<STEP>(m)) << 4), x_at = w_at + WR * STEP;
+    load(wave * STEP, lds0);
+    uint32_t cur = 0;
+    for (int k = wave * STEP; k < a.K; k += kFewWaves * STEP) {
+        load(k + kFewWaves * STEP, lds0 + (cur ? 0 : STAGE));
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (WL + XL));  // this slice has landed; the next one's loads are in flight
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int kk = 0; kk < STEP / 32; ++kk) {
             i32x4 wf[NI], xf[TI];
 #pragma unroll
             for (int i = 0; i < NI; ++i)
-                wf[i] = __builtin_bit_cast(
-                    i32x4, *(const lds_u32x4*)((lds_u8*)((w_at ^ (kk << 5)) + cur) + i * 32 * kI8Step));
+                wf[i] = __builtin_bit_cast(i32x4, *(const lds_u32x4*)((lds_u8*)((w_at ^ (kk << 5)) + cur) + i * 32 * STEP));
 #pragma unroll
             for (int j = 0; j < TI; ++j)
-                xf[j] = __builtin_bit_cast(
-                    i32x4, *(const lds_u32x4*)((lds_u8*)((x_at ^ (kk << 5)) + cur) + j * 32 * kI8Step));
+                xf[j] = __builtin_bit_cast(i32x4, *(const lds_u32x4*)((lds_u8*)((x_at ^ (kk << 5)) + cur) + j * 32 * STEP));
 #pragma unroll
             for (int i = 0; i < NI; ++i)
 #pragma unroll
                 for (int j = 0; j < TI; ++j)
                     acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(wf[i], xf[j], acc[i][j], 0, 0, 0);
         }
-        cur ^= STAGE;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // the slice is read before its place is loaded again
+        asm volatile("" ::: "memory");
+        cur = cur ? 0 : STAGE;
     }
-    // lane (m, hh): token m of a tile, outputs 8 q + 4 hh + 0 .. 3 of its 32
-    constexpr int NO = GATED ? NI / 2 : NI;
+    // The waves' sums, [wave][token][four outputs] with a token's quads swizzled, in the same LDS once no load is in flight.
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    constexpr int Q = WR / 4;  // quads of a token
+    static_assert(kFewWaves * XR * Q * 16 <= sizeof(s_tile), "room for the sums");
+    i32x4* sums = reinterpret_cast<i32x4*>(s_tile);
 #pragma unroll
-    for (int i = 0; i < NO; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < TI; ++j) {
-            const int t = t0 + (wt * TI + j) * 32 + m;
-            if (t >= a.T) continue;
+        for (int j = 0; j < TI; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int n = n0 + (wn * NO + i) * 32 + 8 * q + 4 * hh;
-                if (n >= a.N) continue;
-                const i32x16 &x0 = acc[GATED ? 2 * i : i][j], &x1 = acc[GATED ? 2 * i + 1 : i][j];
-                float v[4];
-                i8_values<GATED>(a, t, n, i32x4{x0[4 * q], x0[4 * q + 1], x0[4 * q + 2], x0[4 * q + 3]},
-                                 i32x4{x1[4 * q], x1[4 * q + 1], x1[4 * q + 2], x1[4 * q + 3]}, v);
-                i8_store(a, t, n, v);
-            }
-        }
+            for (int q = 0; q < 4; ++q)
+                sums[(wave * XR + 32 * j + m) * Q + ((8 * i + 2 * q + hh) ^ (m & (Q - 1)))] =
+                    i32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+    __syncthreads();
+    for (int x = threadIdx.x; x < XR * BN / 4; x += kFewWaves * kWave) {
+        const int row = x / (BN / 4), c = x % (BN / 4), t = t0 + row, n = n0 + 4 * c;
+        if (t >= a.T || n >= a.N) continue;
+        auto total = [&](int quad) {
+            i32x4 s = sums[row * Q + (quad ^ (row & (Q - 1)))];
+#pragma unroll
+            for (int k = 1; k < kFewWaves; ++k) s += sums[(k * XR + row) * Q + (quad ^ (row & (Q - 1)))];
+            return s;
+        };
+        float v[4];
+        i8_values<GATED>(ldg(a.sx + t), i8_scales<GATED>(a, n), total(c), GATED ? total(BN / 4 + c) : i32x4{0, 0, 0, 0}, v);
+        i8_finish(a, t, n, v);
+    }
 }
 
 template <bool GATED>
 static void int8_launch(I8Args a, hipStream_t st) {
     const int64_t T = a.T, N = a.N;
-    if (T <= 64) {
-        // as many waves share a row of weights as keep the CUs in waves
-#define SOI_F(R, C)                                                                                                     \
-    do {                                                                                                                \
-        const int64_t tiles = ceil_div64(N, 16 * (GATED ? R / 2 : R));                                                  \
-        a.ks = tiles >= 4096 ? 1 : tiles >= 2048 ? 2 : tiles >= 1024 ? 4 : 8;                                           \
-        const unsigned gx = static_cast<unsigned>(ceil_div64(tiles, kFewWaves / a.ks));                                 \
-        hipLaunchKernelGGL((int8_few_kernel<R, C, GATED>), dim3(gx, static_cast<unsigned>(ceil_div64(T, 16 * C))),      \
-                           dim3(kFewWaves * kWave), 0, st, a);                                                          \
-    } while (0)
-        if (T <= 16) SOI_F(2, 1);
-        else if (T <= 32) SOI_F(2, 2);
-        else if (T <= 48) SOI_F(2, 3);
-        else SOI_F(2, 4);
-#undef SOI_F
-        return;
-    }
-#define SOI_M(WN, WT, NI, TI, OCC)                                                                                           \
+#define SOI_M(WN, WT, NI, TI, STEP, NBUF, OCC)                                                                               \
     do {                                                                                                                     \
         const int64_t bn = 32 * WN * NI / (GATED ? 2 : 1), bt = 32 * WT * TI;                                                \
         const int64_t nt = ceil_div64(N, bn), tt = ceil_div64(T, bt);                                                        \
-        hipLaunchKernelGGL((int8_many_kernel<WN, WT, NI, TI, GATED, OCC>), dim3(static_cast<unsigned>(nt * tt)),             \
+        hipLaunchKernelGGL((int8_many_kernel<WN, WT, NI, TI, STEP, NBUF, GATED, OCC>), dim3(static_cast<unsigned>(nt * tt)), \
                            dim3(WN * WT * kWave), 0, st, a, static_cast<int>(nt), static_cast<int>(tt));                     \
     } while (0)
+#define SOI_F(NI, TI)                                                                                                \
+    hipLaunchKernelGGL((int8_few_kernel<NI, TI, GATED>),                                                             \
+                       dim3(static_cast<unsigned>(ceil_div64(N, 32 * NI / (GATED ? 2 : 1))),                         \
+                            static_cast<unsigned>(ceil_div64(T, 32 * TI))),                                          \
+                       dim3(kFewWaves * kWave), 0, st, a)
     const int64_t n_all = GATED ? 2 * N : N;
-    if (ceil_div64(n_all, 256) * ceil_div64(T, 256) >= 256) SOI_M(2, 4, 4, 2, 2);
-    else SOI_M(2, 2, 2, 2, 2);
+    auto tiles = [&](int64_t n, int64_t t) { return ceil_div64(n_all, n) * ceil_div64(T, t); };
+    // Workgroups that share K among their waves, of the smallest tiles while these fit the CUs once; rows up to 32 are one tile,
+    // and bound by the weights' bytes, however many outputs there are. Larger tiles read less from LDS and the caches: 64 x 64 up
+    // to two rounds of the CUs, then 128 x 128, whose workgroup keeps K to itself, and 256 x 256 where those fill their last
+    // round. us at 2048 -> 4096 (linear, 64 / 128 / 256 / 400 / 1000 rows): 32 x 32 5.5 / 6.1 / 9.7 / 14.8 / -, 64 x 32 5.6 / 5.7 / 9.3 /
+    // 16.1 / -, 64 x 64 7.1 / 7.0 / 7.2 / 12.2 / 23.4, 128 x 128 14.2 / 14.5 / 14.6 / 14.5 / 16.4. 2048 -> 151936, 1 / 32 / 48 rows:
+    // 49 / 68 / 125, 60 / 70 / 130, 66 / 76 / 82, 60 / 66 / 73. 2048 -> 2 x 6144 (gate_up), 2048 / 8192 rows: 128 x 128 57 / 240,
+    // 256 x 256 65 / 227; 6144 -> 8192, 8192 rows: 443, 407.
+    const int64_t big = tiles(256, 256), rounds = ceil_div64(big, 256);
+    if (tiles(32, 32) <= 256) SOI_F(1, 1);
+    else if (tiles(64, 32) <= 256) SOI_F(2, 1);
+    else if (T <= 32) SOI_F(1, 1);
+    else if (tiles(64, 64) <= 512) SOI_F(2, 2);
+    else if (big < 256 || 5 * big < 4 * 256 * rounds) SOI_M(2, 2, 2, 2, 128, 2, 2);
+    else if constexpr (GATED) SOI_M(4, 2, 2, 4, 64, 4, 2);
+    else SOI_M(2, 4, 4, 2, 64, 4, 2);
+#undef SOI_F
 #undef SOI_M
 }
 
@@ -368,6 +469,12 @@ static int int8_check(const char* what, const int8_t* x, const float* x_scale, c
     return SOI_OK;
 }
 
+static int int8_wide(int64_t N, const float* s0, const float* s1, const uint16_t* y, const uint16_t* res) {
+    if (N % 4 || !aligned16(s0) || !aligned16(s1) || ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(res)) & 7))
+        return 0;
+    return N % 8 == 0 && aligned16(y) ? 2 : 1;
+}
+
 }  // namespace soi
 
 using namespace soi;
@@ -377,9 +484,9 @@ extern "C" int soi_int8_linear(const int8_t* x, const float* x_scale, const int8
     const char* what = "soi_int8_linear";
     const int st = int8_check(what, x, x_scale, Wq, w_scale, y, T, N, K);
     if (st || T == 0) return st;
-    const bool quad = N % 4 == 0 && aligned16(w_scale) && ((reinterpret_cast<uintptr_t>(y) | reinterpret_cast<uintptr_t>(residual)) & 7) == 0;
+    const int wide = int8_wide(N, w_scale, w_scale, y, residual);
     const I8Args a{x, Wq, nullptr, x_scale, w_scale, nullptr, residual, y, static_cast<int>(T), static_cast<int>(N),
-                   static_cast<int>(K), 1, quad};
+                   static_cast<int>(K), wide};
     int8_launch<false>(a, as_stream(stream));
     return launch_status(what);
 }
@@ -392,9 +499,9 @@ extern "C" int soi_int8_gate_up(const int8_t* x, const float* x_scale, const int
     if (st || T == 0) return st;
     st = int8_check(what, x, x_scale, up_Wq, up_scale, h, T, N, K);
     if (st) return st;
-    const bool quad = N % 4 == 0 && aligned16(gate_scale) && aligned16(up_scale) && (reinterpret_cast<uintptr_t>(h) & 7) == 0;
+    const int wide = int8_wide(N, gate_scale, up_scale, h, nullptr);
     const I8Args a{x, gate_Wq, up_Wq, x_scale, gate_scale, up_scale, nullptr, h, static_cast<int>(T), static_cast<int>(N),
-                   static_cast<int>(K), 1, quad};
+                   static_cast<int>(K), wide};
     int8_launch<true>(a, as_stream(stream));
     return launch_status(what);
 }

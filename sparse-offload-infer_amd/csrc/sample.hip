@@ -11,9 +11,9 @@
 //
 // No sort of the row. Its weights go into kBins bins of equal width in z (a histogram in LDS of each chunk, added up in
 // memory); the running sums over the bins say which bins the k-th token, the p border, the min_p border and the drawn token
-// can lie in; only the tokens of those few bins are collected, sorted (a few hundred), and looked at one by one. Rows with a
+// can lie in; only the tokens of those few bins (a few hundred) are collected, and searched by radix passes in LDS. Rows with a
 // top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole.
-// Bins that hold more than kList tokens (many equal logits) are searched by radix passes over the row instead.
+// Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
 //
 // Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for few rows and by the three passes
 // over the logits, the binary64 exponentials of the second and its LDS atomics for many.
@@ -71,32 +71,49 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
 __device__ __forceinline__ uint32_t place_key(uint64_t c) { return ~static_cast<uint32_t>(c >> kIdxBits); }
 __device__ __forceinline__ int place_index(uint64_t c) { return static_cast<int>(c & ((1u << kIdxBits) - 1)); }
 
-// Calls f(key, index) for the logits i of [lo, hi) that thread `tid` of kThreads has.
-template <class LT, class F>
-__device__ __forceinline__ void each_logit(const SampleArgs& a, int row, int lo, int hi, int tid, F f) {
-    const LT* p = static_cast<const LT*>(a.logits) + row * a.stride;
-    for (int i = lo + tid * kPiece; i < hi; i += kChunk) {
-        float v[kPiece];
-        if (i + kPiece <= a.V) {
-            if constexpr (sizeof(LT) == 2) {
-                const u32x4 r = ldg_any(p + i);
+// Eight logits i .. i + 7 (those past the row: -infinity).
+struct Piece {
+    float v[kPiece];
+};
+template <class LT>
+__device__ __forceinline__ Piece load_piece(const SampleArgs& a, int row, int i) {
+    const LT* p = static_cast<const LT*>(a.logits) + row * a.stride + i;
+    Piece x;
+    if (i + kPiece <= a.V) {
+        // (lanes copied to scalars first: a bit cast of a vector's lane was compiled as one of lane 0)
+        if constexpr (sizeof(LT) == 2) {
+            const u32x4 r = ldg_any(p);
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-                for (int e = 0; e < kPiece; ++e) v[e] = f16_bits_to_f32(static_cast<uint16_t>(r[e >> 1] >> (16 * (e & 1))));
-            } else {
-                const u32x4 r0 = ldg_any(p + i), r1 = ldg_any(p + i + 4);
-                // (lanes copied to scalars first: a bit cast of a vector's lane was compiled as one of lane 0)
-                const uint32_t w[kPiece] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
-#pragma unroll
-                for (int e = 0; e < kPiece; ++e) v[e] = __builtin_bit_cast(float, w[e]);
-            }
-#pragma unroll
-            for (int e = 0; e < kPiece; ++e) f(key_of(v[e]), i + e);
+            for (int e = 0; e < kPiece; ++e) x.v[e] = f16_bits_to_f32(static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1))));
         } else {
-            for (int e = i; e < a.V; ++e) {
-                if constexpr (sizeof(LT) == 2) f(key_of(f16_bits_to_f32(ldg(p + e))), e);
-                else f(key_of(ldg(p + e)), e);
-            }
+            const u32x4 r0 = ldg_any(p), r1 = ldg_any(p + 4);
+            const uint32_t w[kPiece] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) x.v[e] = __builtin_bit_cast(float, w[e]);
         }
+        return x;
+    }
+#pragma unroll
+    for (int e = 0; e < kPiece; ++e) {
+        x.v[e] = -__builtin_inff();
+        if (i + e < a.V) {
+            if constexpr (sizeof(LT) == 2) x.v[e] = f16_bits_to_f32(ldg(p + e));
+            else x.v[e] = ldg(p + e);
+        }
+    }
+    return x;
+}
+
+// Calls f(logit, index) for the logits of [lo, hi) that thread `tid` of kThreads has (and for -infinity past the row's end);
+// first: its first piece, requested before.
+template <class LT, class F>
+__device__ __forceinline__ void each_logit(const SampleArgs& a, int row, int lo, int hi, int tid, Piece first, F f) {
+    for (int i = lo + tid * kPiece; i < hi; i += kChunk) {
+        const Piece x = first;
+        if (i + kChunk < hi) first = load_piece<LT>(a, row, i + kChunk);
+#pragma unroll
+        for (int e = 0; e < kPiece; ++e) f(x.v[e], i + e);
     }
 }
 
@@ -111,9 +128,12 @@ __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleA
         stg(&w->count[tid], 0u);
         if (tid == 0) stg(&w->listed, 0u);
     }
+    const int lo = chunk * a.chunk, hi = min(a.V, lo + a.chunk);
     uint64_t top = 0;
     uint32_t low = 0xffffffffu;
-    each_logit<LT>(a, row, chunk * a.chunk, min(a.V, (chunk + 1) * a.chunk), tid, [&](uint32_t key, int i) {
+    each_logit<LT>(a, row, lo, hi, tid, load_piece<LT>(a, row, lo + tid * kPiece), [&](float v, int i) {
+        if (i >= a.V) return;
+        const uint32_t key = key_of(v);
         const uint64_t t = static_cast<uint64_t>(key) << 32 | ~static_cast<uint32_t>(i);
         top = t > top ? t : top;
         low = key > kKeyNegInf && key < low ? key : low;
@@ -150,11 +170,10 @@ struct SamplePlan {
     double p;                           // 1: no top-p
     int k;                              // 0: no top-k
     bool by_count;                      // the tokens down to the k-th are all collected
-    __device__ __forceinline__ double z(uint32_t key) const { return (max - static_cast<double>(value_of(key))) * inv_t; }
-    __device__ __forceinline__ bool counts(uint32_t key, double z) const { return key > kKeyNegInf && z <= z_limit; }
-    __device__ __forceinline__ int bin(double z) const {
-        const double b = z * per_z;
-        return b < kBins - 1 ? static_cast<int>(b) : kBins - 1;
+    __device__ __forceinline__ double z(float v) const { return (max - static_cast<double>(v)) * inv_t; }
+    __device__ __forceinline__ bool counts(double z) const { return z <= z_limit; }  // (-infinity: z is infinite or NaN)
+    __device__ __forceinline__ int bin(double z) const {  // of a z that counts
+        return static_cast<int>(fmin(z * per_z, kBins - 1.0));
     }
 };
 
@@ -191,7 +210,7 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
     s.min_z = mp > 0.0f ? (mp < 1.0f ? -log(static_cast<double>(mp)) : 0.0) : __builtin_inf();
     // without top-p, what min-p drops does not count for anything
     s.z_limit = s.p == 1.0 && s.min_z < kZMost ? s.min_z : kZMost;
-    const double most = s.z(low), span = most < s.z_limit ? most : s.z_limit;
+    const double most = s.z(value_of(low)), span = most < s.z_limit ? most : s.z_limit;
     s.per_z = span > 1e-290 ? kBins / span : 0.0;
     s.by_count = s.k > 0 && s.k <= kMostK;
     return s;
@@ -223,20 +242,25 @@ template <class LT>
 __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a) {
     __shared__ uint64_t s_weight[kBins];
     __shared__ uint32_t s_count[kBins];
-    const int tid = threadIdx.x, row = blockIdx.y, chunk = blockIdx.x;
-    const SamplePlan s = sample_plan(a, row);
-    if (s.greedy) return;
+    const int tid = threadIdx.x, row = blockIdx.y, chunk = blockIdx.x, lo = chunk * a.chunk, hi = min(a.V, lo + a.chunk);
+    const Piece first = load_piece<LT>(a, row, lo + tid * kPiece);
     s_weight[tid] = 0;
     s_count[tid] = 0;
+    const SamplePlan s = sample_plan(a, row);
+    if (s.greedy) return;
     __syncthreads();
-    const bool weights = !s.by_count, counts = s.k > 0;
-    each_logit<LT>(a, row, chunk * a.chunk, min(a.V, (chunk + 1) * a.chunk), tid, [&](uint32_t key, int) {
-        const double z = s.z(key);
-        if (!s.counts(key, z)) return;
-        const int b = s.bin(z);
-        if (weights) atomicAdd(reinterpret_cast<unsigned long long*>(&s_weight[b]), weight_of(z));
-        if (counts) atomicAdd(&s_count[b], 1u);
-    });
+    auto pass = [&](auto WEIGHTS, auto COUNTS) {
+        each_logit<LT>(a, row, lo, hi, tid, first, [&](float v, int) {
+            const double z = s.z(v);
+            if (!s.counts(z)) return;
+            const int b = s.bin(z);
+            if (WEIGHTS) atomicAdd(reinterpret_cast<unsigned long long*>(&s_weight[b]), weight_of(z));
+            if (COUNTS) atomicAdd(&s_count[b], 1u);
+        });
+    };
+    if (s.by_count) pass(std::false_type{}, std::true_type{});
+    else if (s.k > 0) pass(std::true_type{}, std::true_type{});
+    else pass(std::true_type{}, std::false_type{});
     __syncthreads();
     SampleRow* w = a.rows + row;
     if (s_weight[tid]) atomicAdd(reinterpret_cast<unsigned long long*>(&w->weight[tid]), s_weight[tid]);
@@ -270,17 +294,13 @@ struct SampleShared {
     uint64_t part[kThreads / kWave];
     uint32_t part32[kThreads / kWave];
     uint64_t before, to;  // answers
-    int at;
+    unsigned long long least, most;
+    int at, n;
 };
 
-__device__ __forceinline__ SampleBins sample_bins(const SampleArgs& a, int row, SampleShared& sh) {
-    const SampleRow* w = a.rows + row;
-    SampleBins b;
-    b.weight = ldg(&w->weight[threadIdx.x]);
-    b.count = ldg(&w->count[threadIdx.x]);
+__device__ __forceinline__ void sum_bins(SampleBins& b, SampleShared& sh) {
     b.to_weight = scan_threads(b.weight, sh.part);
     b.to_count = scan_threads(b.count, sh.part32);
-    return b;
 }
 
 // A bin, with the weights in front of it and with it.
@@ -345,15 +365,26 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(const SampleAr
     __shared__ uint8_t s_wanted[kBins];
     __shared__ uint64_t s_list[kList];
     __shared__ uint32_t s_n, s_at;
-    const int tid = threadIdx.x, row = blockIdx.y, chunk = blockIdx.x;
+    __shared__ int s_lo, s_hi;
+    const int tid = threadIdx.x, row = blockIdx.y, chunk = blockIdx.x, lo_i = chunk * a.chunk, hi_i = min(a.V, lo_i + a.chunk);
+    SampleRow* w = a.rows + row;
+    const Piece first = load_piece<LT>(a, row, lo_i + tid * kPiece);
+    SampleBins b;
+    b.weight = ldg(&w->weight[tid]);
+    b.count = ldg(&w->count[tid]);
+    const float u = ldg(a.u + row);
     const SamplePlan s = sample_plan(a, row);
     if (s.greedy) return;
-    const SampleBins b = sample_bins(a, row, sh);
+    sum_bins(b, sh);
     if (tid == kBins - 1) {
         s_at = b.to_count;
         sh.to = b.to_weight;
     }
-    if (tid == 0) s_n = 0;
+    if (tid == 0) {
+        s_n = 0;
+        s_lo = kBins;
+        s_hi = -1;
+    }
     __syncthreads();
     const uint32_t all_count = s_at;
     uint64_t all_lo = sh.to, all_hi = sh.to;
@@ -384,20 +415,28 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(const SampleAr
             lo = m.before < lo ? m.before : lo;
             hi = m.to < hi ? m.to : hi;
         }
-        const float u = ldg(a.u + row);
         const BinAt x = bin_of_weight(b, u_border(u, lo), sh), y = bin_of_weight(b, u_border(u, hi), sh);
         wanted |= tid >= x.bin && tid <= y.bin;
     }
     s_wanted[tid] = wanted;
+    {  // the first and the last of them: most tokens are past it
+        const uint64_t any = ballot(wanted);
+        if (any && (tid & 63) == 0) {
+            atomicMin(&s_lo, tid + __builtin_ctzll(any));
+            atomicMax(&s_hi, tid + 63 - __builtin_clzll(any));
+        }
+    }
     __syncthreads();
-    each_logit<LT>(a, row, chunk * a.chunk, min(a.V, (chunk + 1) * a.chunk), tid, [&](uint32_t key, int i) {
-        const double z = s.z(key);
-        if (!s.counts(key, z) || !s_wanted[s.bin(z)]) return;
+    const int b_lo = s_lo, b_hi = s_hi;
+    each_logit<LT>(a, row, lo_i, hi_i, tid, first, [&](float v, int i) {
+        const double z = s.z(v);
+        if (!s.counts(z)) return;
+        const int bin = s.bin(z);
+        if (bin < b_lo || bin > b_hi || !s_wanted[bin]) return;
         const uint32_t n = atomicAdd(&s_n, 1u);
-        if (n < kList) s_list[n] = place_of(key, i);
+        if (n < kList) s_list[n] = place_of(key_of(v), i);
     });
     __syncthreads();
-    SampleRow* w = a.rows + row;
     if (tid == 0) s_at = s_n ? atomicAdd(&w->listed, s_n) : 0;
     __syncthreads();
     const uint32_t n = s_n < kList ? s_n : kList, at = s_at;
@@ -415,93 +454,129 @@ struct Found {
     int index;
 };
 
-// The collected tokens in order, with the running sums of their weights.
-struct Sorted {
+// The collected tokens, or, where a segment holds more of them than the list, the row's.
+struct Listed {
     const SamplePlan& s;
-    SampleShared& sh;
-    const uint64_t *place, *sum;  // [n] in LDS
+    const uint64_t *place, *weight;  // [n] in LDS
     int n;
-    __device__ __forceinline__ int bin(int i) const { return s.bin(s.z(place_key(place[i]))); }
-    // position of the segment's first token
-    __device__ __forceinline__ int start(const Segment& g) const {
-        if (threadIdx.x == 0) sh.at = n;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads)
-            if (bin(i) >= g.lo && (i == 0 || bin(i - 1) < g.lo)) sh.at = i;
-        __syncthreads();
-        const int r = sh.at;
-        __syncthreads();
-        return r;
-    }
-    __device__ __forceinline__ uint64_t until(int i) const { return i > 0 ? sum[i - 1] : 0; }
-    // the running sum with the segment's j-th token (from 1)
-    __device__ __forceinline__ uint64_t nth(const Segment& g, uint64_t j) const {
-        const int first = start(g), i = first + static_cast<int>(j);
-        return g.before + until(i < n ? i : n) - until(first);
-    }
-    // the first token with which the running sum reaches x
-    __device__ __forceinline__ Found reach(const Segment& g, uint64_t x) const {
-        const uint64_t base = until(start(g));
-        if (threadIdx.x == 0) {
-            sh.at = 0;
-            sh.to = g.before;
-        }
-        __syncthreads();
+    template <class F>
+    __device__ __forceinline__ void each(const Segment& g, F f) const {
         for (int i = threadIdx.x; i < n; i += kThreads) {
-            const int b = bin(i);
-            if (b < g.lo || b > g.hi) continue;
-            const uint64_t to = g.before + sum[i] - base, before = g.before + until(i) - base;
-            if (to >= x && before < x) {
-                sh.at = place_index(place[i]);
-                sh.to = to;
-            }
+            const double z = s.z(value_of(place_key(place[i])));
+            const int b = s.bin(z);
+            if (b >= g.lo && b <= g.hi) f(place[i], z, [&] { return weight[i]; });
+        }
+    }
+};
+template <class LT>
+struct InRow {
+    const SampleArgs& a;
+    const SamplePlan& s;
+    int row;
+    template <class F>
+    __device__ __forceinline__ void each(const Segment& g, F f) const {
+        each_logit<LT>(a, row, 0, a.V, threadIdx.x, load_piece<LT>(a, row, threadIdx.x * kPiece), [&](float v, int i) {
+            const double z = s.z(v);
+            if (!s.counts(z)) return;
+            const int b = s.bin(z);
+            if (b >= g.lo && b <= g.hi) f(place_of(key_of(v), i), z, [&] { return weight_of(z); });
+        });
+    }
+};
+
+// Finds tokens of a segment: their place, ten bits at a time, by histograms of what the segment's tokens weigh and count, until
+// one token is left where the sum crosses.
+template <class Source>
+struct Search {
+    const Source& q;
+    SampleShared& sh;
+    uint64_t* hist;    // [kBins] in LDS
+    uint32_t* counts;  // likewise
+    // the first token with which the running sum (or, by_count, the number of tokens) of the segment reaches x >= 1
+    __device__ __forceinline__ Found find(const Segment& g, uint64_t x, bool by_count) const {
+        const int tid = threadIdx.x;
+        // the segment's range of places
+        uint64_t least = ~uint64_t(0), most = 0;
+        q.each(g, [&](uint64_t c, double, auto) {
+            least = c < least ? c : least;
+            most = c > most ? c : most;
+        });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const uint64_t l = __shfl_xor(least, o), m = __shfl_xor(most, o);
+            least = l < least ? l : least;
+            most = m > most ? m : most;
+        }
+        if (tid == 0) {
+            sh.least = ~0ull;
+            sh.most = 0;
         }
         __syncthreads();
-        const Found r{sh.to, sh.at};
+        if ((tid & 63) == 0) {
+            atomicMin(&sh.least, least);
+            atomicMax(&sh.most, most);
+        }
+        __syncthreads();
+        uint64_t lo = sh.least, before = 0;
+        const uint64_t range = sh.most >= lo ? sh.most - lo : 0;
+        int shift = 0;
+        while (range >> shift >= kBins) shift += 10;
+        for (;; shift = shift > 10 ? shift - 10 : 0) {
+            hist[tid] = 0;
+            counts[tid] = 0;
+            __syncthreads();
+            q.each(g, [&](uint64_t c, double, auto weight) {
+                const uint64_t d = (c - lo) >> shift;
+                if (c < lo || d >= kBins) return;
+                atomicAdd(reinterpret_cast<unsigned long long*>(&hist[d]), weight());
+                atomicAdd(&counts[d], 1u);
+            });
+            __syncthreads();
+            const uint64_t w = hist[tid], to_w = scan_threads(w, sh.part);
+            const uint32_t n = counts[tid], to_n = scan_threads(n, sh.part32);
+            const uint64_t own = by_count ? n : w, to = by_count ? to_n : to_w;
+            if (tid == 0) {
+                sh.at = kBins - 1;
+                sh.before = sh.to = 0;
+                sh.n = 0;
+            }
+            __syncthreads();
+            if (to >= x && to - own < x) {
+                sh.at = tid;
+                sh.before = to_w - w;
+                sh.to = to - own;
+                sh.n = static_cast<int>(n);
+            }
+            __syncthreads();
+            const uint64_t bin = static_cast<uint64_t>(sh.at);
+            const int left = sh.n;
+            before += sh.before;
+            x -= sh.to;
+            lo += bin << shift;
+            __syncthreads();
+            if (left <= 1 || shift == 0) break;
+        }
+        // the token itself: of the places lo .. lo + 2^shift - 1, of which one is taken
+        if (tid == 0) {
+            sh.at = 0;
+            sh.to = 0;
+        }
+        __syncthreads();
+        q.each(g, [&](uint64_t c, double, auto weight) {
+            if (c < lo || (c - lo) >> shift) return;
+            sh.at = place_index(c);
+            sh.to = weight();
+        });
+        __syncthreads();
+        const Found r{g.before + before + sh.to, sh.at};
         __syncthreads();
         return r;
     }
     // the running sum with the segment's last token of z <= z_max
     __device__ __forceinline__ uint64_t within(const Segment& g, double z_max) const {
-        const uint64_t base = until(start(g));
-        if (threadIdx.x == 0) sh.to = g.before;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kThreads) {
-            const double z = s.z(place_key(place[i]));
-            const int b = s.bin(z);
-            if (b < g.lo || b > g.hi || z > z_max) continue;
-            const int nb = i + 1 < n ? bin(i + 1) : kBins;
-            if (nb > g.hi || s.z(place_key(place[i + 1])) > z_max) sh.to = g.before + sum[i] - base;
-        }
-        __syncthreads();
-        const uint64_t r = sh.to;
-        __syncthreads();
-        return r;
-    }
-};
-
-// The same answers from passes over the row, where a segment holds more tokens than the list: the place is found ten bits at a
-// time by histograms of what the segment's tokens weigh (or count).
-template <class LT>
-struct Searched {
-    const SampleArgs& a;
-    const SamplePlan& s;
-    SampleShared& sh;
-    uint64_t* hist;  // [kBins] in LDS
-    int row;
-    template <class F>
-    __device__ __forceinline__ void each(const Segment& g, F f) const {
-        each_logit<LT>(a, row, 0, a.V, threadIdx.x, [&](uint32_t key, int i) {
-            const double z = s.z(key);
-            if (!s.counts(key, z)) return;
-            const int b = s.bin(z);
-            if (b >= g.lo && b <= g.hi) f(key, i, z);
-        });
-    }
-    __device__ __forceinline__ uint64_t total(const Segment& g, uint64_t last, double z_max) const {
         uint64_t w = 0;
-        each(g, [&](uint32_t key, int i, double z) {
-            if (place_of(key, i) <= last && z <= z_max) w += weight_of(z);
+        q.each(g, [&](uint64_t, double z, auto weight) {
+            if (z <= z_max) w += weight();
         });
         w = scan_threads(w, sh.part);
         if (threadIdx.x == kThreads - 1) sh.to = w;
@@ -510,43 +585,6 @@ struct Searched {
         __syncthreads();
         return r;
     }
-    // the place of the first token with which the sum from the segment's start reaches x (1 <= x)
-    __device__ __forceinline__ uint64_t place(const Segment& g, uint64_t x, bool by_count) const {
-        uint64_t lo = 0;
-        for (int shift = 32 + kIdxBits - 10;; shift = shift > 10 ? shift - 10 : 0) {
-            hist[threadIdx.x] = 0;
-            __syncthreads();
-            each(g, [&](uint32_t key, int i, double z) {
-                const uint64_t d = place_of(key, i) - lo;
-                if (place_of(key, i) >= lo && d >> shift < kBins)
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&hist[d >> shift]), by_count ? 1ull : weight_of(z));
-            });
-            __syncthreads();
-            const uint64_t own = hist[threadIdx.x], to = scan_threads(own, sh.part);
-            if (threadIdx.x == 0) {
-                sh.at = kBins - 1;
-                sh.before = 0;
-            }
-            __syncthreads();
-            if (to >= x && to - own < x) {
-                sh.at = threadIdx.x;
-                sh.before = to - own;
-            }
-            __syncthreads();
-            lo += static_cast<uint64_t>(sh.at) << shift;
-            x -= sh.before;
-            __syncthreads();
-            if (shift == 0) return lo;
-        }
-    }
-    __device__ __forceinline__ uint64_t nth(const Segment& g, uint64_t j) const {
-        return total(g, place(g, j, true), __builtin_inf());
-    }
-    __device__ __forceinline__ Found reach(const Segment& g, uint64_t x) const {
-        const uint64_t c = place(g, x - g.before, false);
-        return {total(g, c, __builtin_inf()), place_index(c)};
-    }
-    __device__ __forceinline__ uint64_t within(const Segment& g, double z_max) const { return total(g, ~uint64_t(0), z_max); }
 };
 
 template <class Q>
@@ -556,90 +594,87 @@ __device__ __forceinline__ int sample_decide(const SamplePlan& s, const SampleBi
         sh.at = static_cast<int>(b.to_count);
     }
     __syncthreads();
-    uint64_t kept = sh.to;
+    uint64_t kept = sh.to;  // the sum of the weights that are left
     const int count = sh.at;
     __syncthreads();
-    Segment g{0, kBins - 1, 0};  // by_count: everything that was collected
-    if (s.by_count) {
-        const int k = s.k < count ? s.k : count;
-        const BinAt c = bin_of_count(b, k, sh);
-        g.hi = c.bin;
-        kept = q.nth(g, k);
-    } else if (s.k > 0 && s.k < count) {
-        const BinAt c = bin_of_count(b, s.k, sh), w = bin_at(b, c.bin, sh);
-        if (c.to == static_cast<uint64_t>(s.k)) kept = w.to;
-        else kept = q.nth(Segment{c.bin, c.bin, w.before}, s.k - c.before);
-    }
-    auto segment = [&](uint64_t x) {  // where the running sum reaches x
-        if (s.by_count) return g;
-        const BinAt w = bin_of_weight(b, x, sh);
-        return Segment{w.bin, w.bin, w.before};
-    };
-    if (s.p < 1.0) {
-        const uint64_t x = p_border(s.p, kept);
-        kept = q.reach(segment(x), x).to;
-    }
-    if (s.min_z < s.z_limit) {
-        Segment m = g;
-        if (!s.by_count) {
-            const BinAt w = bin_at(b, s.bin(s.min_z), sh);
-            m = Segment{w.bin, w.bin, w.before};
+    Segment all{0, kBins - 1, 0};  // by_count: everything that was collected
+    int index = 0;
+    for (int rule = 0; rule < 3; ++rule) {  // top-k, top-p, the draw
+        Segment g = all;
+        uint64_t x;
+        if (rule == 0) {
+            if (s.k == 0 || (!s.by_count && s.k >= count)) continue;
+            x = s.k < count ? s.k : count;
+            const BinAt c = bin_of_count(b, static_cast<uint32_t>(x), sh);
+            if (s.by_count) {
+                all.hi = g.hi = c.bin;
+            } else {
+                const BinAt w = bin_at(b, c.bin, sh);
+                kept = w.to;
+                if (c.to == x) continue;
+                g = Segment{c.bin, c.bin, w.before};
+                x -= c.before;
+            }
+        } else {
+            if (rule == 1 && s.p >= 1.0) continue;
+            if (rule == 2 && s.min_z < s.z_limit) {
+                if (!s.by_count) {
+                    const BinAt w = bin_at(b, s.bin(s.min_z), sh);
+                    g = Segment{w.bin, w.bin, w.before};
+                }
+                if (g.before < kept) {
+                    const uint64_t most = q.within(g, s.min_z);
+                    kept = most < kept ? most : kept;
+                }
+            }
+            x = rule == 1 ? p_border(s.p, kept) : u_border(u, kept);
+            if (!s.by_count) {
+                const BinAt w = bin_of_weight(b, x, sh);
+                g = Segment{w.bin, w.bin, w.before};
+            }
+            x -= g.before;
         }
-        if (m.before < kept) {
-            const uint64_t most = q.within(m, s.min_z);
-            kept = most < kept ? most : kept;
-        }
+        const Found f = q.find(g, x, rule == 0);
+        if (rule < 2) kept = f.to;
+        index = f.index;
     }
-    const uint64_t x = u_border(u, kept);
-    return q.reach(segment(x), x).index;
+    return index;
 }
 
 template <class LT>
 __global__ __launch_bounds__(kThreads) void sample_decide_kernel(const SampleArgs a) {
     __shared__ SampleShared sh;
-    __shared__ uint64_t s_place[kList], s_sum[kList];
+    __shared__ uint64_t s_place[kList], s_weight[kList], s_hist[kBins];
+    __shared__ uint32_t s_count[kBins];
     const int tid = threadIdx.x, row = blockIdx.x;
+    const SampleRow* w = a.rows + row;
+    // everything is requested before the first of it is needed (what the launches before left out is whatever was there)
+    SampleBins b;
+    b.weight = ldg(&w->weight[tid]);
+    b.count = ldg(&w->count[tid]);
+    uint64_t place = ldg(&w->list[tid]);
+    const uint32_t listed = ldg(&w->listed);
+    const float u = ldg(a.u + row);
     const SamplePlan s = sample_plan(a, row);
     if (s.greedy) {
         if (tid == 0) stg(a.tokens + row, s.first);
         return;
     }
-    const SampleBins b = sample_bins(a, row, sh);
-    const SampleRow* w = a.rows + row;
-    const uint32_t listed = ldg(&w->listed);
-    const float u = ldg(a.u + row);
+    sum_bins(b, sh);
     int token;
     if (listed <= kList) {
         const int n = static_cast<int>(listed);
-        int size = 2;
-        while (size < n) size <<= 1;
-        for (int i = tid; i < size; i += kThreads) s_place[i] = i < n ? ldg(&w->list[i]) : ~uint64_t(0);
-        __syncthreads();
-        for (int k = 2; k <= size; k <<= 1)  // bitonic
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                for (int t = tid; t < size / 2; t += kThreads) {
-                    const int i = 2 * t - (t & (j - 1)), o = i + j;
-                    const uint64_t x = s_place[i], y = s_place[o];
-                    if ((x > y) == ((i & k) == 0)) {
-                        s_place[i] = y;
-                        s_place[o] = x;
-                    }
-                }
-                __syncthreads();
-            }
-        uint64_t base = 0;
-        for (int i0 = 0; i0 < n; i0 += kThreads) {  // running sums
-            const int i = i0 + tid;
-            const uint64_t v = scan_threads(i < n ? weight_of(s.z(place_key(s_place[i]))) : uint64_t(0), sh.part) + base;
-            if (i < n) s_sum[i] = v;
-            if (tid == kThreads - 1) sh.to = v;
-            __syncthreads();
-            base = sh.to;
-            __syncthreads();
+        for (int i = tid; i < n; i += kThreads) {
+            if (i >= kThreads) place = ldg(&w->list[i]);
+            s_place[i] = place;
+            s_weight[i] = weight_of(s.z(value_of(place_key(place))));
         }
-        token = sample_decide(s, b, u, Sorted{s, sh, s_place, s_sum, n}, sh);
+        __syncthreads();
+        const Listed q{s, s_place, s_weight, n};
+        token = sample_decide(s, b, u, Search<Listed>{q, sh, s_hist, s_count}, sh);
     } else {
-        token = sample_decide(s, b, u, Searched<LT>{a, s, sh, s_place, row}, sh);
+        const InRow<LT> q{a, s, row};
+        token = sample_decide(s, b, u, Search<InRow<LT>>{q, sh, s_hist, s_count}, sh);
     }
     if (tid == 0) stg(a.tokens + row, token);
 }

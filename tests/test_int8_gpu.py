@@ -133,7 +133,8 @@ def check_gate_up(h, x, xs, ws, ss):
 SHAPES = [(1, 16, 1), (1, 2048, 4096), (2, 48, 17), (5, 2048, 130), (16, 272, 64), (17, 6144, 333), (31, 80, 1000),
           (33, 1024, 2050), (48, 640, 20001), (49, 144, 36), (64, 2064, 4100), (64, 256, 70000), (65, 128, 128),
           (65, 16, 3), (100, 2048, 1000), (129, 400, 257), (256, 6144, 512), (300, 144, 6145), (777, 2048, 4096),
-          (1025, 208, 4099), (2049, 1040, 8200), (4096, 112, 5000)]
+          (1025, 208, 4099), (2049, 1040, 8200), (4096, 112, 5000), (4000, 112, 4050), (4000, 208, 2040), (3850, 80, 4090),
+          (200, 48, 2072), (40, 6144, 2040)]
 
 
 @pytest.mark.parametrize("T,K,N", SHAPES)
