@@ -117,6 +117,32 @@ __device__ __forceinline__ void each_logit(const SampleArgs& a, int row, int lo,
     }
 }
 
+// Inclusive sums over a wave's lanes, and the largest of them in every lane.
+template <int CTRL, int ROWS, class N>
+__device__ __forceinline__ N lane_move(N v) {  // zeros where nothing comes from
+    if constexpr (sizeof(N) == 8) {
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), CTRL, ROWS, 0xf, false);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+    } else {
+        return static_cast<N>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+    }
+}
+template <class N, class Op>
+__device__ __forceinline__ N wave_run(N v, Op op) {
+    v = op(v, lane_move<0x111, 0xf>(v));
+    v = op(v, lane_move<0x112, 0xf>(v));
+    v = op(v, lane_move<0x114, 0xf>(v));
+    v = op(v, lane_move<0x118, 0xf>(v));
+    v = op(v, lane_move<0x142, 0xa>(v));
+    v = op(v, lane_move<0x143, 0xc>(v));
+    return v;
+}
+// The largest of the lanes, valid in lane 63.
+__device__ __forceinline__ uint64_t wave_top(uint64_t v) {
+    return wave_run(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+}
+
 template <class LT>
 __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleArgs a) {
     __shared__ uint64_t s_top[kThreads / kWave];
@@ -138,23 +164,18 @@ __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleA
         top = t > top ? t : top;
         low = key > kKeyNegInf && key < low ? key : low;
     });
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t t = __shfl_xor(top, o);
-        const uint32_t l = __shfl_xor(low, o);
-        top = t > top ? t : top;
-        low = l < low ? l : low;
-    }
-    if (lane == 0) {
+    top = wave_top(top);
+    low = ~static_cast<uint32_t>(wave_top(~low));
+    if (lane == 63) {
         s_top[wave] = top;
         s_low[wave] = low;
     }
     __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < kThreads / kWave; ++w) {
-            top = s_top[w] > top ? s_top[w] : top;
-            low = s_low[w] < low ? s_low[w] : low;
-        }
+    if (wave == 0) {
+        top = wave_top(lane < kThreads / kWave ? s_top[lane] : 0);
+        low = ~static_cast<uint32_t>(wave_top(lane < kThreads / kWave ? ~s_low[lane] : 0));
+    }
+    if (tid == 63) {
         SamplePart* p = a.parts + static_cast<int64_t>(row) * a.chunks + chunk;
         stg(&p->top, top);
         stg(&p->low, low);
@@ -188,13 +209,12 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
         top = t > top ? t : top;
         low = l < low ? l : low;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t t = __shfl_xor(top, o);
-        const uint32_t l = __shfl_xor(low, o);
-        top = t > top ? t : top;
-        low = l < low ? l : low;
-    }
+    auto last = [](uint64_t v) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+    };
+    top = last(wave_top(top));
+    low = ~static_cast<uint32_t>(last(wave_top(~low)));
     const float T = a.temperature ? ldg(a.temperature + row) : a.temperature_all;
     const float tp = a.top_p ? ldg(a.top_p + row) : a.top_p_all, mp = a.min_p ? ldg(a.min_p + row) : a.min_p_all;
     const int k = a.top_k ? ldg(a.top_k + row) : a.top_k_all;
@@ -213,6 +233,11 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
     const double most = s.z(value_of(low)), span = most < s.z_limit ? most : s.z_limit;
     s.per_z = span > 1e-290 ? kBins / span : 0.0;
     s.by_count = s.k > 0 && s.k <= kMostK;
+    for (double* d : {&s.max, &s.inv_t, &s.z_limit, &s.per_z, &s.min_z, &s.p}) {  // to scalar registers
+        const uint64_t v = __builtin_bit_cast(uint64_t, *d);
+        const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+        *d = __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+    }
     return s;
 }
 
@@ -270,18 +295,22 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
 // Inclusive sums over the workgroup's threads; s_part: one number a wave. Every thread may call it again at once.
 template <class N>
 __device__ __forceinline__ N scan_threads(N v, N* s_part) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const N x = __shfl_up(v, o);
-        v += lane >= o ? x : 0;
-    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v = wave_run(v, [](N a, N b) { return a + b; });
     if (lane == 63) s_part[wave] = v;
     __syncthreads();
-    N base = 0;
-    for (int w = 0; w < kThreads / kWave; ++w) base += w < wave ? s_part[w] : 0;
+    // the waves' sums in the first lanes: their running sum, of which this wave takes its own
+    const N part = wave_run(lane < kThreads / kWave ? s_part[lane] : N(0), [](N a, N b) { return a + b; });
+    N base;
+    if constexpr (sizeof(N) == 8) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(part), wave > 0 ? wave - 1 : 0);
+        const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(part >> 32), wave > 0 ? wave - 1 : 0);
+        base = static_cast<uint64_t>(hi) << 32 | lo;
+    } else {
+        base = __builtin_amdgcn_readlane(static_cast<int>(part), wave > 0 ? wave - 1 : 0);
+    }
     __syncthreads();
-    return v + base;
+    return v + (wave > 0 ? base : N(0));
 }
 
 // The bins' running sums; thread b has bin b.
@@ -477,9 +506,11 @@ struct InRow {
     __device__ __forceinline__ void each(const Segment& g, F f) const {
         each_logit<LT>(a, row, 0, a.V, threadIdx.x, load_piece<LT>(a, row, threadIdx.x * kPiece), [&](float v, int i) {
             const double z = s.z(v);
-            if (!s.counts(z)) return;
-            const int b = s.bin(z);
-            if (b >= g.lo && b <= g.hi) f(place_of(key_of(v), i), z, [&] { return weight_of(z); });
+            if (s.counts(z)) {
+                const int b = s.bin(z);
+                if (b >= g.lo && b <= g.hi) f(place_of(key_of(v), i), z, [&] { return weight_of(z); });
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (eight logits at once would spill)
         });
     }
 };
@@ -501,18 +532,14 @@ struct Search {
             least = c < least ? c : least;
             most = c > most ? c : most;
         });
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const uint64_t l = __shfl_xor(least, o), m = __shfl_xor(most, o);
-            least = l < least ? l : least;
-            most = m > most ? m : most;
-        }
+        least = ~wave_top(~least);
+        most = wave_top(most);
         if (tid == 0) {
             sh.least = ~0ull;
             sh.most = 0;
         }
         __syncthreads();
-        if ((tid & 63) == 0) {
+        if ((tid & 63) == 63) {
             atomicMin(&sh.least, least);
             atomicMax(&sh.most, most);
         }
@@ -582,6 +609,113 @@ struct Search {
         if (threadIdx.x == kThreads - 1) sh.to = w;
         __syncthreads();
         const uint64_t r = g.before + sh.to;
+        __syncthreads();
+        return r;
+    }
+};
+
+// Up to kShort collected tokens: the first wave sorts them in registers, four a lane, and answers from their running sums.
+constexpr int kShort = 4 * kWave;
+
+// The value of lane (l ^ MASK).
+template <int MASK>
+__device__ __forceinline__ uint64_t other_lane(uint64_t v) {
+    const uint32_t lo = __builtin_bit_cast(uint32_t, xor_lanes<MASK>(__builtin_bit_cast(float, static_cast<uint32_t>(v))));
+    const uint32_t hi = __builtin_bit_cast(uint32_t, xor_lanes<MASK>(__builtin_bit_cast(float, static_cast<uint32_t>(v >> 32))));
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// Bitonic steps from (K, J) on, of numbers 4 lane + e.
+template <int K, int J>
+__device__ __forceinline__ void sort_short(uint64_t (&x)[4], int lane) {
+    if constexpr (J >= 4) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint64_t o = other_lane<J / 4>(x[e]);
+            const bool least = ((lane & (J / 4)) == 0) == (((4 * lane + e) & K) == 0);
+            x[e] = (x[e] < o) == least ? x[e] : o;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e & J) continue;
+            const uint64_t a = x[e], b = x[e + J];
+            const bool swap = (a > b) == (((4 * lane + e) & K) == 0);
+            x[e] = swap ? b : a;
+            x[e + J] = swap ? a : b;
+        }
+    }
+    if constexpr (J > 1) sort_short<K, J / 2>(x, lane);
+    else if constexpr (K < kShort) sort_short<2 * K, K>(x, lane);
+}
+
+struct Short {
+    const SamplePlan& s;
+    SampleShared& sh;
+    uint64_t place[4], sum[4];  // (of the first wave; past the last token: the largest place)
+    int bin[4];
+    __device__ __forceinline__ Short(const SamplePlan& s, SampleShared& sh, const uint64_t* list, int n) : s(s), sh(sh) {
+        const int lane = threadIdx.x & 63;
+        if (threadIdx.x >= kWave) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) place[e] = 4 * lane + e < n ? list[4 * lane + e] : ~uint64_t(0);
+        sort_short<2, 1>(place, lane);
+        uint64_t w[4], mine = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool is = 4 * lane + e < n;
+            const double z = s.z(value_of(place_key(place[e])));
+            bin[e] = is ? s.bin(z) : kBins;
+            w[e] = is ? weight_of(z) : 0;
+            mine += w[e];
+        }
+        uint64_t run = wave_run(mine, [](uint64_t a, uint64_t b) { return a + b; }) - mine;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] = run += w[e];
+    }
+    template <class F>
+    __device__ __forceinline__ int how_many(F f) const {
+        int n = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n += __popcll(ballot(f(e)));
+        return n;
+    }
+    static __device__ __forceinline__ uint64_t of_lane(uint64_t v, int lane) {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+        return static_cast<uint64_t>(hi) << 32 | lo;
+    }
+    static __device__ __forceinline__ uint64_t at(const uint64_t (&x)[4], int i) {  // the i-th number
+        const uint64_t a = i & 1 ? x[1] : x[0], b = i & 1 ? x[3] : x[2];
+        return of_lane(i & 2 ? b : a, i >> 2);
+    }
+    __device__ __forceinline__ Found find(const Segment& g, uint64_t x, bool by_count) const {
+        if (threadIdx.x < kWave) {
+            const int first = how_many([&](int e) { return bin[e] < g.lo; });
+            const uint64_t base = first ? at(sum, first - 1) : 0;
+            int i = first + static_cast<int>(x) - 1;
+            if (!by_count) i = how_many([&](int e) { return bin[e] < g.lo || (bin[e] < kBins && sum[e] - base < x); });
+            i = i < kShort ? i : kShort - 1;
+            const uint64_t to = g.before + at(sum, i) - base;
+            const int index = place_index(at(place, i));
+            if (threadIdx.x == 0) {
+                sh.to = to;
+                sh.at = index;
+            }
+        }
+        __syncthreads();
+        const Found r{sh.to, sh.at};
+        __syncthreads();
+        return r;
+    }
+    __device__ __forceinline__ uint64_t within(const Segment& g, double z_max) const {
+        if (threadIdx.x < kWave) {
+            const int first = how_many([&](int e) { return bin[e] < g.lo; });
+            const int end = how_many([&](int e) { return bin[e] < g.lo || (bin[e] <= g.hi && s.z(value_of(place_key(place[e]))) <= z_max); });
+            const uint64_t to = g.before + (end ? at(sum, end - 1) : 0) - (first ? at(sum, first - 1) : 0);
+            if (threadIdx.x == 0) sh.to = to;
+        }
+        __syncthreads();
+        const uint64_t r = sh.to;
         __syncthreads();
         return r;
     }
@@ -670,8 +804,12 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(const SampleArg
             s_weight[i] = weight_of(s.z(value_of(place_key(place))));
         }
         __syncthreads();
-        const Listed q{s, s_place, s_weight, n};
-        token = sample_decide(s, b, u, Search<Listed>{q, sh, s_hist, s_count}, sh);
+        if (n <= kShort) {
+            token = sample_decide(s, b, u, Short(s, sh, s_place, n), sh);
+        } else {
+            const Listed q{s, s_place, s_weight, n};
+            token = sample_decide(s, b, u, Search<Listed>{q, sh, s_hist, s_count}, sh);
+        }
     } else {
         const InRow<LT> q{a, s, row};
         token = sample_decide(s, b, u, Search<InRow<LT>>{q, sh, s_hist, s_count}, sh);
