@@ -12,7 +12,9 @@
 // No sort of the row. Its weights go into kBins bins of equal width in z (a histogram in LDS of each chunk, added up in
 // memory); the running sums over the bins say which bins the k-th token, the p border, the min_p border and the drawn token
 // can lie in; only the tokens of those few bins (a few hundred) are collected, and searched by radix passes in LDS. Rows with a
-// top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole.
+// top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole, and of
+// the other tokens only those are looked at that reach the smallest of the first launch's threads' largest logits (one a thread
+// does, which are at least k).
 // Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
 //
 // Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for few rows and by the three passes
@@ -37,8 +39,8 @@ struct SampleRow {  // of the workspace
 };
 struct SamplePart {  // a chunk's extremes
     uint64_t top;    // key of the largest, ~index
-    uint32_t low;    // key of the smallest number that is not -inf
-    uint32_t pad;
+    uint32_t low;    // key of the smallest number
+    uint32_t bound;  // key of the smallest of the threads' largest: one token a thread reaches it
 };
 
 struct SampleArgs {
@@ -53,6 +55,7 @@ struct SampleArgs {
     SampleRow* rows;
     SamplePart* parts;
     int B, V, chunks, chunk;  // chunks of `chunk` logits a row
+    int threads;              // of a row's that have a logit
 };
 
 // Ascending with the number; NaN on top, both zeros one.
@@ -139,14 +142,15 @@ __device__ __forceinline__ N wave_run(N v, Op op) {
     return v;
 }
 // The largest of the lanes, valid in lane 63.
-__device__ __forceinline__ uint64_t wave_top(uint64_t v) {
-    return wave_run(v, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+template <class N>
+__device__ __forceinline__ N wave_top(N v) {
+    return wave_run(v, [](N a, N b) { return a > b ? a : b; });
 }
 
 template <class LT>
 __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleArgs a) {
     __shared__ uint64_t s_top[kThreads / kWave];
-    __shared__ uint32_t s_low[kThreads / kWave];
+    __shared__ uint32_t s_low[kThreads / kWave], s_bound[kThreads / kWave];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.y, chunk = blockIdx.x;
     if (chunk == 0) {
         SampleRow* w = a.rows + row;
@@ -154,31 +158,75 @@ __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleA
         stg(&w->count[tid], 0u);
         if (tid == 0) stg(&w->listed, 0u);
     }
+    // A thread keeps its largest and smallest number (NaN aside), the piece that the largest came with first, and the largest
+    // pattern without its sign, which tells whether there is a NaN. The index is looked up at the end by those that have the wave's.
     const int lo = chunk * a.chunk, hi = min(a.V, lo + a.chunk);
+    float best = -__builtin_inff(), least = __builtin_inff();
+    uint32_t pattern = 0;
+    int from = lo + tid * kPiece, at = from;
+    Piece x;  // the piece at `at`
+    {
+        Piece next = load_piece<LT>(a, row, from);
+        for (int i = from; i < hi; i += kChunk) {
+            x = next;
+            at = i;
+            if (i + kChunk < hi) next = load_piece<LT>(a, row, i + kChunk);
+            float most = x.v[0];
+#pragma unroll
+            for (int e = 1; e < kPiece; ++e) most = fmaxf(most, x.v[e]);
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) {
+                if (i + e < a.V) least = fminf(least, x.v[e]);
+                const uint32_t m = __builtin_bit_cast(uint32_t, x.v[e]) & 0x7fffffffu;
+                pattern = m > pattern ? m : pattern;
+            }
+            from = most > best ? i : from;
+            best = most > best ? most : best;
+        }
+    }
+    if (pattern > 0x7f800000u) {  // the first NaN is this thread's largest
+        best = __builtin_nanf("");
+        for (int i = lo + tid * kPiece; i < hi; i += kChunk) {
+            x = load_piece<LT>(a, row, i);
+            bool here = false;
+#pragma unroll
+            for (int e = 0; e < kPiece; ++e) here |= x.v[e] != x.v[e];
+            from = at = i;
+            if (here) break;
+        }
+    }
+    const uint32_t best_key = key_of(best);
+    uint32_t low = least == -__builtin_inff() ? kKeyNegInf : key_of(least);
+    const bool any = lo + tid * kPiece < hi;
+    const uint32_t top_key = __builtin_amdgcn_readlane(static_cast<int>(wave_top(any ? best_key : 0u)), 63);
     uint64_t top = 0;
-    uint32_t low = 0xffffffffu;
-    each_logit<LT>(a, row, lo, hi, tid, load_piece<LT>(a, row, lo + tid * kPiece), [&](float v, int i) {
-        if (i >= a.V) return;
-        const uint32_t key = key_of(v);
-        const uint64_t t = static_cast<uint64_t>(key) << 32 | ~static_cast<uint32_t>(i);
-        top = t > top ? t : top;
-        low = key > kKeyNegInf && key < low ? key : low;
-    });
+    if (any && best_key == top_key) {
+        if (from != at) x = load_piece<LT>(a, row, from);
+        int i = a.V;
+#pragma unroll
+        for (int e = kPiece - 1; e >= 0; --e) i = from + e < a.V && key_of(x.v[e]) == top_key ? from + e : i;
+        top = static_cast<uint64_t>(top_key) << 32 | ~static_cast<uint32_t>(i);
+    }
+    uint32_t bound = any ? best_key : 0xffffffffu;
+    bound = ~wave_top(~bound);
     top = wave_top(top);
-    low = ~static_cast<uint32_t>(wave_top(~low));
+    low = ~wave_top(~low);
     if (lane == 63) {
         s_top[wave] = top;
         s_low[wave] = low;
+        s_bound[wave] = bound;
     }
     __syncthreads();
     if (wave == 0) {
-        top = wave_top(lane < kThreads / kWave ? s_top[lane] : 0);
-        low = ~static_cast<uint32_t>(wave_top(lane < kThreads / kWave ? ~s_low[lane] : 0));
+        top = wave_top(lane < kThreads / kWave ? s_top[lane] : uint64_t(0));
+        low = ~wave_top(lane < kThreads / kWave ? ~s_low[lane] : 0u);
+        bound = ~wave_top(lane < kThreads / kWave ? ~s_bound[lane] : 0u);
     }
     if (tid == 63) {
         SamplePart* p = a.parts + static_cast<int64_t>(row) * a.chunks + chunk;
         stg(&p->top, top);
         stg(&p->low, low);
+        stg(&p->bound, bound);
     }
 }
 
@@ -202,19 +250,19 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
     const int lane = threadIdx.x & 63;
     const SamplePart* p = a.parts + static_cast<int64_t>(row) * a.chunks;
     uint64_t top = 0;
-    uint32_t low = 0xffffffffu;
+    uint32_t low = 0xffffffffu, bound = 0xffffffffu;
     for (int c = lane; c < a.chunks; c += kWave) {
         const uint64_t t = ldg(&p[c].top);
-        const uint32_t l = ldg(&p[c].low);
+        const uint32_t l = ldg(&p[c].low), m = ldg(&p[c].bound);
         top = t > top ? t : top;
         low = l < low ? l : low;
+        bound = m < bound ? m : bound;
     }
-    auto last = [](uint64_t v) {
-        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
-        return static_cast<uint64_t>(hi) << 32 | lo;
-    };
-    top = last(wave_top(top));
-    low = ~static_cast<uint32_t>(last(wave_top(~low)));
+    const auto last = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63)); };
+    top = wave_top(top);
+    top = static_cast<uint64_t>(last(static_cast<uint32_t>(top >> 32))) << 32 | last(static_cast<uint32_t>(top));
+    low = ~last(wave_top(~low));
+    bound = ~last(wave_top(~bound));
     const float T = a.temperature ? ldg(a.temperature + row) : a.temperature_all;
     const float tp = a.top_p ? ldg(a.top_p + row) : a.top_p_all, mp = a.min_p ? ldg(a.min_p + row) : a.min_p_all;
     const int k = a.top_k ? ldg(a.top_k + row) : a.top_k_all;
@@ -230,9 +278,13 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
     s.min_z = mp > 0.0f ? (mp < 1.0f ? -log(static_cast<double>(mp)) : 0.0) : __builtin_inf();
     // without top-p, what min-p drops does not count for anything
     s.z_limit = s.p == 1.0 && s.min_z < kZMost ? s.min_z : kZMost;
-    const double most = s.z(value_of(low)), span = most < s.z_limit ? most : s.z_limit;
-    s.per_z = span > 1e-290 ? kBins / span : 0.0;
     s.by_count = s.k > 0 && s.k <= kMostK;
+    if (s.by_count && s.k <= a.threads && bound > kKeyNegInf) {  // as many tokens as threads are at least `bound`
+        const double z = s.z(value_of(bound));
+        s.z_limit = z < s.z_limit ? z : s.z_limit;
+    }
+    const double most = low > kKeyNegInf ? s.z(value_of(low)) : s.z_limit, span = most < s.z_limit ? most : s.z_limit;
+    s.per_z = span > 1e-290 ? kBins / span : 0.0;
     for (double* d : {&s.max, &s.inv_t, &s.z_limit, &s.per_z, &s.min_z, &s.p}) {  // to scalar registers
         const uint64_t v = __builtin_bit_cast(uint64_t, *d);
         const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
@@ -817,9 +869,12 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(const SampleArg
     if (tid == 0) stg(a.tokens + row, token);
 }
 
-// Chunks of a row: as many as give about two workgroups to a CU, each of at least one piece a thread.
+// Chunks of a row: as many as give four workgroups of 1024 threads to a CU, two at a time, each of at least one piece a thread
+// where the row allows it. 200 rows of 151936 fp16 logits, by workgroups to a CU, extremes + bins + collect: 2: 19 + 52 + 35 us
+// (rows differ in how many of their weights count, and one round of them waits for the slowest); 4: 20 + 41 + 33; 8:
+// 27 + 46 + 44; 16: 40 + 53 + 60 (each workgroup's histogram is cleared and added up).
 static int sample_chunks(int64_t B, int64_t V) {
-    const int64_t most = ceil_div64(V, kChunk), want = ceil_div64(512, B);
+    const int64_t most = ceil_div64(V, kChunk), want = B < 1024 ? 1024 / B : 1;
     return static_cast<int>(want < most ? want : most);
 }
 
@@ -854,6 +909,8 @@ extern "C" int soi_sample_tokens(const void* logits, int logits_f32, int64_t str
     a.chunks = sample_chunks(batch, vocab);
     a.chunk = static_cast<int>(ceil_div64(ceil_div64(vocab, a.chunks), kPiece) * kPiece);
     a.chunks = static_cast<int>(ceil_div64(vocab, a.chunk));
+    const auto with_logits = [](int64_t n) { return n < kChunk ? ceil_div64(n, kPiece) : int64_t(kThreads); };
+    a.threads = static_cast<int>((a.chunks - 1) * with_logits(a.chunk) + with_logits(vocab - int64_t(a.chunks - 1) * a.chunk));
     const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(batch)), block(kThreads);
     hipStream_t st = as_stream(stream);
     const bool draws = temperature || temperature_all > 0.0f;  // otherwise every row's token is its largest
