@@ -2317,6 +2317,9 @@ torch::Tensor sample_tokens(torch::Tensor logits, torch::Tensor u, OptTensor tem
     if (out) {
         row_values(out, torch::kInt32, "out");
         no_overlap(o, logits, n, "out and logits");
+        no_overlap(o, u, n, "out and u");
+        for (const OptTensor* t : {&temperature, &top_k, &top_p, &min_p})
+            if (*t) no_overlap(o, **t, n, "out and a row's settings");
     }
     if (B == 0) return o;
     const int64_t bytes = sample_tokens_workspace_bytes(B, V);

@@ -251,3 +251,19 @@ def test_refusals(cuda):
         with pytest.raises(RuntimeError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+def test_outputs_over_an_input_are_refused(cuda):
+    x, u = rows(cuda, 3, 100, 1)
+    k = torch.zeros(3, dtype=torch.int32, device=cuda)
+    f = torch.ones(3, device=cuda)
+    i32 = torch.int32
+    bad = [
+        lambda: ops.sample_tokens(x, u, out=u.view(i32)), lambda: ops.sample_tokens(x, u, 1.0, k, out=k),
+        lambda: ops.sample_tokens(x, u, f, out=f.view(i32)), lambda: ops.sample_tokens(x, u, 1.0, 0, f, out=f.view(i32)),
+        lambda: ops.sample_tokens(x, u, 1.0, 0, 1.0, f, out=f.view(i32)),
+    ]
+    for i, g in enumerate(bad):
+        with pytest.raises(RuntimeError, match="overlap"):
+            g()
+            pytest.fail(f"call {i} was taken")
