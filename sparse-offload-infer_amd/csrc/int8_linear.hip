@@ -130,6 +130,7 @@ __global__ __launch_bounds__(WN * WT * kWave, OCC) void int8_many_kernel(const I
     constexpr int WL = BN / RL / NW, XL = BT / RL / NW;  // 1 KB loads of a wave and stage, RL rows each
     static_assert(BN % (RL * NW) == 0 && BT % (RL * NW) == 0, "whole loads per wave");
     constexpr int SL = 32 / RL;  // loads of a strip
+    static_assert(!GATED || NI % 2 == 0, "a wave has strips of both matrices");
     static_assert(!GATED || SL % WL == 0 || WL % (2 * SL) == 0, "a wave's loads of weights are parts of a strip, or pairs of them");
     __shared__ __attribute__((aligned(1024))) uint8_t s_tile[NBUF * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -439,18 +440,24 @@ static void int8_launch(I8Args a, hipStream_t st) {
                        dim3(kFewWaves * kWave), 0, st, a)
     const int64_t n_all = GATED ? 2 * N : N;
     auto tiles = [&](int64_t n, int64_t t) { return ceil_div64(n_all, n) * ceil_div64(T, t); };
-    // Workgroups that share K among their waves, of the smallest tiles while these fit the CUs once; rows up to 32 are one tile,
-    // and bound by the weights' bytes, however many outputs there are. Larger tiles read less from LDS and the caches: 64 x 64 up
-    // to two rounds of the CUs, then 128 x 128, whose workgroup keeps K to itself, and 256 x 256 where those fill their last
-    // round. us at 2048 -> 4096 (linear, 64 / 128 / 256 / 400 / 1000 rows): 32 x 32 5.5 / 6.1 / 9.7 / 14.8 / -, 64 x 32 5.6 / 5.7 / 9.3 /
-    // 16.1 / -, 64 x 64 7.1 / 7.0 / 7.2 / 12.2 / 23.4, 128 x 128 14.2 / 14.5 / 14.6 / 14.5 / 16.4. 2048 -> 151936, 1 / 32 / 48 rows:
-    // 49 / 68 / 125, 60 / 70 / 130, 66 / 76 / 82, 60 / 66 / 73. 2048 -> 2 x 6144 (gate_up), 2048 / 8192 rows: 128 x 128 57 / 240,
-    // 256 x 256 65 / 227; 6144 -> 8192, 8192 rows: 443, 407.
+    // Where few tiles keep the CUs short of work, workgroups share K among their waves, of the smallest tiles while these fit the
+    // CUs once: 32 x 32, 64 x 32, 64 x 64 weight rows x tokens. Then workgroups keep K to themselves, three stages in LDS: 128 x
+    // 64, two to a CU, where one tile has all rows (bound by the weights' bytes) or those fit the CUs once, then 128 x 128 of eight
+    // waves up to one a CU. More work than that hides its own loads: 128 x 128 of four waves and two stages, two to a CU, and 256 x
+    // 256 where those fill their last round.
+    // us at 2048 -> 4096 (linear, 64 / 128 / 256 / 400 / 1000 rows): 32 x 32 5.5 / 6.1 / 9.7 / 14.8 / -, 64 x 32 5.6 / 5.7 / 9.3 /
+    // 16.1 / -, 64 x 64 5.2 / 5.9 / 7.3 / 12.3 / 23.4, 128 x 64 8.9 / 8.6 / 9.0 / 10.0 / 16.2, 128 x 128 of eight waves 10.5 / 10.6 /
+    // 10.8 / 11.7 / 13.9, of four 14.2 / 14.5 / 14.6 / 14.6 / 16.2. 2048 -> 16384, 1 / 32 / 64 / 128 / 256 rows: 64 x 32 8.0 / 7.7 / - / -
+    // / -, 64 x 64 - / - / 9.1 / 15.2 / 17.3, 128 x 64 8.9 / 9.3 / 10.3 / 10.5 / 15.6, eight waves - / - / 11.4 / 12.1 / 14.4. 2048 ->
+    // 151936, 1 / 32 / 48 rows: 32 x 32 51 / 68 / 125, 128 x 64 51 / 56 / 61, 128 x 128 of four waves 60 / 66 / 73. gate_up, 2048 ->
+    // 2 x 6144, 128 / 256 / 512 / 2048 / 8192 rows: 64 x 64 13.1 / - / - / - / -, 128 x 64 9.2 / 13.0 / 20 / 78 / -, eight waves 10.9 /
+    // 11.6 / 22 / 67 / -, four 14 / 14.6 / 18 / 58 / 240, 256 x 256 26 / 28 / 30 / 65 / 227; linear 6144 -> 8192, 8192 rows: 443, 407.
     const int64_t big = tiles(256, 256), rounds = ceil_div64(big, 256);
     if (tiles(32, 32) <= 256) SOI_F(1, 1);
     else if (tiles(64, 32) <= 256) SOI_F(2, 1);
-    else if (T <= 32) SOI_F(1, 1);
-    else if (tiles(64, 64) <= 512) SOI_F(2, 2);
+    else if (tiles(64, 64) <= 256) SOI_F(2, 2);
+    else if (T <= 64 || tiles(128, 64) <= 256) SOI_M(2, 2, 2, 1, 128, 3, 2);
+    else if (tiles(128, 128) <= 256) SOI_M(2, 4, 2, 1, 128, 3, 2);
     else if (big < 256 || 5 * big < 4 * 256 * rounds) SOI_M(2, 2, 2, 2, 128, 2, 2);
     else if constexpr (GATED) SOI_M(4, 2, 2, 4, 64, 4, 2);
     else SOI_M(2, 4, 4, 2, 64, 4, 2);

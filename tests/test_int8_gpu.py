@@ -278,3 +278,17 @@ def test_streams_and_graphs(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, calls()))
+
+
+# the tiles of three stages: rows of one tile, tiles that fit the CUs once, eight waves; each way of storing
+@pytest.mark.parametrize("T,K,N", [(64, 1040, 9000), (33, 272, 16385), (1, 64, 20004), (130, 400, 6000), (520, 208, 5004),
+                                   (520, 208, 2500), (500, 144, 2051), (250, 2064, 4104), (700, 16, 3000), (511, 6144, 4099)])
+def test_tiles_of_three_stages(cuda, T, K, N):
+    x, xs, ws, ss = problem(cuda, T, K, N, T * K + 3 * N, mats=2)
+    res = torch.randn(T, N, device=cuda).half() * 8
+    check_linear(ops.int8_linear(x, xs, ws[0], ss[0], residual=res), x, xs, ws[0], ss[0], res)
+    check_gate_up(ops.int8_gate_up(x, xs, ws[0], ss[0], ws[1], ss[1]), x, xs, ws, ss)
+    # a row alone, through another tile, has the same bits
+    t = T // 2
+    row = ops.int8_gate_up(x[t:t + 1], xs[t:t + 1], ws[0], ss[0], ws[1], ss[1])
+    assert torch.equal(row, ops.int8_gate_up(x, xs, ws[0], ss[0], ws[1], ss[1])[t:t + 1])
