@@ -10,8 +10,8 @@
 //
 // A unit is taken in stages of 64 tokens. The workgroup's four waves unpack a stage's K and V codes into LDS as binary16
 // integers (exact), the next stage's bytes on their way into registers meanwhile. Then each wave takes 32 columns
-// (v_mfma_f32_32x32x16_f16, lanes n = lane & 31, h = lane >> 5), cw of them side by side, 4 / cw waves sharing the stage's
-// tokens:
+// (v_mfma_f32_32x32x16_f16, lanes n = lane & 31, h = lane >> 5), cw of them side by side, two sharing the stage's tokens where
+// cw < 4 (cw 1 leaves two waves that only unpack):
 //   * S^T = K Q^T: lane (n, h) ends with the scores of column n and tokens 8 (r >> 2) + 4 h + (r & 3), r < 16; a scale group's
 //     sums are multiplied by its scale in binary32;
 //   * O^T = V^T P^T takes these, exponentiated, as its B operand as they lie, times V's scale, rounded to binary16 once: a set
@@ -23,6 +23,12 @@
 //     it, 0 below 2^-37 of it. (K and V rounded to binary16 values in LDS would save a third of the vector work, but their
 //     rounding triples the output's error.)
 // 16-byte chunks are XOR-swizzled so that operand reads and the unpacked rows' writes spread over the banks.
+//
+// 64 sequences behind 8192 shared tokens (up to 512 of their own; 32 / 8 heads of 128): plan 5.8, units 37, states added 5.7 us, where
+// kv4_attention.hip reads 64 times as much. Bound by the launches' latency and, in a unit, by vector instructions: unpacking, and
+// scales, exponentials and conversions of every score, beside 8.9 GFLOP of products (7 us at a library product's rate). Stages of
+// 128 tokens (two workgroups to a CU instead of three) 57 us in all, of 64 45; page table lookups with branches, and addresses
+// kept in registers until they spilled, cost a third of the units' time.
 #include "soi_host.h"
 #include "soi_kv4.h"
 #include "soi_attn.h"

@@ -17,8 +17,10 @@
 // does, which are at least k).
 // Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
 //
-// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for few rows and by the three passes
-// over the logits, the binary64 exponentials of the second and its LDS atomics for many.
+// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.2, 4.7,
+// 6.7 and 8.8 us), for many by the three passes over the logits, the binary64 exponentials and LDS atomics of the second and the
+// search of rows that collect many tokens in the last (200 rows, each with its own settings: 19, 39, 32 and 34 us; one pass at a
+// large copy's rate is 12 us). The collected tokens of a row are sorted by one wave where they are up to 256 (one row 29 -> 23 us).
 #include "soi_host.h"
 #include "soi_device.h"
 
