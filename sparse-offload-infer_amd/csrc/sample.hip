@@ -11,16 +11,17 @@
 //
 // No sort of the row. Its weights go into kBins bins of equal width in z (a histogram in LDS of each chunk, added up in
 // memory); the running sums over the bins say which bins the k-th token, the p border, the min_p border and the drawn token
-// can lie in; only the tokens of those few bins (a few hundred) are collected, and searched by radix passes in LDS. Rows with a
-// top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole, and of
-// the other tokens only those are looked at that reach the smallest of the first launch's threads' largest logits (one a thread
-// does, which are at least k).
+// can lie in; only the tokens of those few bins (a few hundred) are collected, and sorted, or searched by radix passes in LDS.
+// Rows with a top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole,
+// and of the other tokens only those are looked at that reach the smallest of the first launch's threads' largest logits (one a
+// thread does, which are at least k).
 // Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
 //
 // Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.2, 4.7,
-// 6.7 and 8.8 us), for many by the three passes over the logits, the binary64 exponentials and LDS atomics of the second and the
-// search of rows that collect many tokens in the last (200 rows, each with its own settings: 19, 39, 32 and 34 us; one pass at a
-// large copy's rate is 12 us). The collected tokens of a row are sorted by one wave where they are up to 256 (one row 29 -> 23 us).
+// 6.7 and 8.6 us), for many by the three passes over the logits and the binary64 exponentials and LDS atomics of the second (200
+// rows, each with its own settings: 18, 39, 32 and 17 us; one pass at a large copy's rate is 12 us). The collected tokens of a row
+// are sorted, by one wave where they are up to 256 (one row 29 -> 23 us beside radix passes for all), by the workgroup up to 2048
+// (the last launch of the 200 rows 34 -> 17 us).
 #include "soi_host.h"
 #include "soi_device.h"
 
@@ -775,6 +776,91 @@ struct Short {
     }
 };
 
+// Up to E tokens a thread: the workgroup sorts them (in registers and lanes, across waves through LDS), and every wave answers
+// for itself from their running sums in LDS.
+template <int E>
+struct Sorted {
+    static constexpr int kMost = E * kThreads;
+    const SamplePlan& s;
+    const uint64_t *place, *sum;  // [kMost] in LDS, in order; sums with the token
+    int n;
+    // bitonic steps from (K, J) on, of numbers E tid + e; buffer: 2 kMost numbers, of which each exchange takes a half
+    template <int K, int J>
+    static __device__ __forceinline__ void sort(uint64_t (&x)[E], uint64_t* buffer, int half) {
+        const int tid = threadIdx.x;
+        if constexpr (J >= E) {
+            if constexpr (J / E >= kWave) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) buffer[half * kMost + E * tid + e] = x[e];
+                __syncthreads();
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                uint64_t o;
+                if constexpr (J / E >= kWave) o = buffer[half * kMost + ((E * tid + e) ^ J)];
+                else o = other_lane<J / E>(x[e]);
+                const bool least = ((E * tid + e) & J) == 0 ? ((E * tid + e) & K) == 0 : ((E * tid + e) & K) != 0;
+                x[e] = (x[e] < o) == least ? x[e] : o;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                if (e & J) continue;
+                const uint64_t a = x[e], b = x[e + J];
+                const bool swap = (a > b) == (((E * tid + e) & K) == 0);
+                x[e] = swap ? b : a;
+                x[e + J] = swap ? a : b;
+            }
+        }
+        constexpr int kNext = J / E >= kWave ? 1 : 0;  // (the other half: this one may still be read)
+        if constexpr (J > 1) sort<K, J / 2>(x, buffer, half ^ kNext);
+        else if constexpr (K < kMost) sort<2 * K, K>(x, buffer, half ^ kNext);
+    }
+    // list: x[e] of each thread in any order, ~0 past the last; buffer: 2 kMost numbers of LDS, sums: kMost
+    __device__ __forceinline__ Sorted(const SamplePlan& s, SampleShared& sh, uint64_t (&x)[E], uint64_t* buffer, uint64_t* sums, int n)
+        : s(s), place(buffer), sum(sums), n(n) {
+        const int tid = threadIdx.x;
+        sort<2, 1>(x, buffer, 0);
+        uint64_t w[E], mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            w[e] = E * tid + e < n ? weight_of(s.z(value_of(place_key(x[e])))) : 0;
+            mine += w[e];
+        }
+        uint64_t run = scan_threads(mine, sh.part) - mine;  // (its barriers are behind the last reads of the buffer)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            buffer[E * tid + e] = x[e];
+            sums[E * tid + e] = run += w[e];
+        }
+        __syncthreads();
+    }
+    __device__ __forceinline__ double z(int i) const { return s.z(value_of(place_key(place[i]))); }
+    // how many tokens f(i) is true of; it is for the first ones and no other
+    template <class F>
+    __device__ __forceinline__ int how_many(F f) const {
+        constexpr int kPart = kMost / kWave;
+        const int lane = threadIdx.x & 63;
+        const int i = kPart * lane + kPart - 1;
+        const int part = __popcll(ballot(i < n && f(i)));
+        const int j = kPart * part + lane;
+        return kPart * part + __popcll(ballot(lane < kPart && j < n && f(j)));
+    }
+    __device__ __forceinline__ Found find(const Segment& g, uint64_t x, bool by_count) const {
+        const int first = how_many([&](int i) { return s.bin(z(i)) < g.lo; });
+        const uint64_t base = first ? sum[first - 1] : 0;
+        int i = first + static_cast<int>(x) - 1;
+        if (!by_count) i = how_many([&](int i) { return i < first || sum[i] - base < x; });
+        i = i < n ? i : n - 1;
+        return Found{g.before + sum[i] - base, place_index(place[i])};
+    }
+    __device__ __forceinline__ uint64_t within(const Segment& g, double z_max) const {
+        const int first = how_many([&](int i) { return s.bin(z(i)) < g.lo; });
+        const int end = how_many([&](int i) { return i < first || (s.bin(z(i)) <= g.hi && z(i) <= z_max); });
+        return g.before + (end ? sum[end - 1] : 0) - (first ? sum[first - 1] : 0);
+    }
+};
+
 template <class Q>
 __device__ __forceinline__ int sample_decide(const SamplePlan& s, const SampleBins& b, float u, const Q& q, SampleShared& sh) {
     if (threadIdx.x == kBins - 1) {
@@ -852,17 +938,25 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(const SampleArg
     int token;
     if (listed <= kList) {
         const int n = static_cast<int>(listed);
-        for (int i = tid; i < n; i += kThreads) {
-            if (i >= kThreads) place = ldg(&w->list[i]);
-            s_place[i] = place;
-            s_weight[i] = weight_of(s.z(value_of(place_key(place))));
-        }
-        __syncthreads();
-        if (n <= kShort) {
-            token = sample_decide(s, b, u, Short(s, sh, s_place, n), sh);
+        if (n > kShort && n <= kThreads) {
+            uint64_t x[1] = {tid < n ? place : ~uint64_t(0)};
+            token = sample_decide(s, b, u, Sorted<1>(s, sh, x, s_place, s_weight, n), sh);
+        } else if (n > kThreads && n <= 2 * kThreads) {
+            uint64_t x[2] = {place, tid + kThreads < n ? ldg(&w->list[tid + kThreads]) : ~uint64_t(0)};
+            token = sample_decide(s, b, u, Sorted<2>(s, sh, x, s_place, s_weight, n), sh);
         } else {
-            const Listed q{s, s_place, s_weight, n};
-            token = sample_decide(s, b, u, Search<Listed>{q, sh, s_hist, s_count}, sh);
+            for (int i = tid; i < n; i += kThreads) {
+                if (i >= kThreads) place = ldg(&w->list[i]);
+                s_place[i] = place;
+                s_weight[i] = weight_of(s.z(value_of(place_key(place))));
+            }
+            __syncthreads();
+            if (n <= kShort) {
+                token = sample_decide(s, b, u, Short(s, sh, s_place, n), sh);
+            } else {
+                const Listed q{s, s_place, s_weight, n};
+                token = sample_decide(s, b, u, Search<Listed>{q, sh, s_hist, s_count}, sh);
+            }
         }
     } else {
         const InRow<LT> q{a, s, row};

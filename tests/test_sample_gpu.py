@@ -267,3 +267,19 @@ def test_outputs_over_an_input_are_refused(cuda):
         with pytest.raises(RuntimeError, match="overlap"):
             g()
             pytest.fail(f"call {i} was taken")
+
+
+@pytest.mark.parametrize("half", [True, False])
+def test_numbers_of_collected_tokens(cuda, half):
+    """Top-k up to 2048 collects about k tokens: numbers about the sizes that one wave, the workgroup with one or two tokens a
+    thread, and the search take. Row b of the last logits has so many equal ones, which top-k cuts in their middle."""
+    ks = [1, 2, 255, 256, 257, 300, 700, 1000, 1023, 1024, 1025, 1400, 1999, 2047, 2048]
+    k = torch.tensor(ks, dtype=torch.int32, device=cuda)
+    for i, (T, p, m) in enumerate([(1.0, 1.0, 0.0), (1.4, 0.9, 0.0), (0.9, 1.0, 0.01), (2.0, 0.97, 0.03), (5.0, 0.5, 1e-3)]):
+        x, u = rows(cuda, len(ks), 30011, 40 + i, half=half)
+        check(x, u, T, k, p, m)
+    for n in (200, 256, 257, 1000, 1024, 1025, 2000, 2048, 2049, 4000, 4096, 4097):
+        x, u = rows(cuda, len(ks), 9001, n, spread=0.5, half=half)
+        x[:, 17:17 + n] = 30.0
+        check(x, u, 1.0, k, 0.7, 0.0, close_allowed=1)
+        check(x, u, 0.5, 0, 0.35, 0.5, close_allowed=1)
