@@ -17,9 +17,9 @@
 // thread does, which are at least k).
 // Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
 //
-// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.2, 4.7,
+// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.3, 4.0,
 // 6.7 and 8.6 us), for many by the three passes over the logits and the binary64 exponentials and LDS atomics of the second (200
-// rows, each with its own settings: 18, 39, 32 and 17 us; one pass at a large copy's rate is 12 us). The collected tokens of a row
+// rows, each with its own settings: 18, 37, 32 and 17 us; one pass at a large copy's rate is 12 us). The collected tokens of a row
 // are sorted, by one wave where they are up to 256 (one row 29 -> 23 us beside radix passes for all), by the workgroup up to 2048
 // (the last launch of the 200 rows 34 -> 17 us).
 #include "soi_host.h"
@@ -30,6 +30,7 @@
 namespace soi {
 
 constexpr int kBins = 1024, kThreads = 1024, kList = 4096, kMostK = 2048, kPiece = 8, kChunk = kThreads * kPiece;
+constexpr int kBinThreads = 512;                  // of the bins' workgroups: rows differ in work, and half as much each evens out (40 -> 37 us)
 constexpr int kIdxBits = 20;                      // of a token's index in its place in the order (the vocabulary: 2^19)
 constexpr double kZMost = 45 * 0.6931471805599453;  // 2^44 exp(-z) rounds to 0 from here on
 constexpr uint32_t kKeyInf = 0xff800000u, kKeyNegInf = 0x007fffffu;
@@ -58,6 +59,7 @@ struct SampleArgs {
     SampleRow* rows;
     SamplePart* parts;
     int B, V, chunks, chunk;  // chunks of `chunk` logits a row
+    int bin_chunk;            // logits of a workgroup of the bins
     int threads;              // of a row's that have a logit
 };
 
@@ -111,13 +113,13 @@ __device__ __forceinline__ Piece load_piece(const SampleArgs& a, int row, int i)
     return x;
 }
 
-// Calls f(logit, index) for the logits of [lo, hi) that thread `tid` of kThreads has (and for -infinity past the row's end);
+// Calls f(logit, index) for the logits of [lo, hi) that thread `tid` of NT has (and for -infinity past the row's end);
 // first: its first piece, requested before.
-template <class LT, class F>
+template <class LT, int NT = kThreads, class F>
 __device__ __forceinline__ void each_logit(const SampleArgs& a, int row, int lo, int hi, int tid, Piece first, F f) {
-    for (int i = lo + tid * kPiece; i < hi; i += kChunk) {
+    for (int i = lo + tid * kPiece; i < hi; i += NT * kPiece) {
         const Piece x = first;
-        if (i + kChunk < hi) first = load_piece<LT>(a, row, i + kChunk);
+        if (i + NT * kPiece < hi) first = load_piece<LT>(a, row, i + NT * kPiece);
 #pragma unroll
         for (int e = 0; e < kPiece; ++e) f(x.v[e], i + e);
     }
@@ -319,18 +321,21 @@ __device__ __forceinline__ uint64_t weight_of(double z) {
 }
 
 template <class LT>
-__global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(kBinThreads) void sample_bins_kernel(const SampleArgs a) {
     __shared__ uint64_t s_weight[kBins];
     __shared__ uint32_t s_count[kBins];
-    const int tid = threadIdx.x, row = blockIdx.y, chunk = blockIdx.x, lo = chunk * a.chunk, hi = min(a.V, lo + a.chunk);
+    const int tid = threadIdx.x, row = blockIdx.y, lo = static_cast<int>(blockIdx.x) * a.bin_chunk, hi = min(a.V, lo + a.bin_chunk);
     const Piece first = load_piece<LT>(a, row, lo + tid * kPiece);
-    s_weight[tid] = 0;
-    s_count[tid] = 0;
+#pragma unroll
+    for (int i = tid; i < kBins; i += kBinThreads) {
+        s_weight[i] = 0;
+        s_count[i] = 0;
+    }
     const SamplePlan s = sample_plan(a, row);
     if (s.greedy) return;
     __syncthreads();
     auto pass = [&](auto WEIGHTS, auto COUNTS) {
-        each_logit<LT>(a, row, lo, hi, tid, first, [&](float v, int) {
+        each_logit<LT, kBinThreads>(a, row, lo, hi, tid, first, [&](float v, int) {
             const double z = s.z(v);
             if (!s.counts(z)) return;
             const int b = s.bin(z);
@@ -343,8 +348,11 @@ __global__ __launch_bounds__(kThreads) void sample_bins_kernel(const SampleArgs 
     else pass(std::true_type{}, std::false_type{});
     __syncthreads();
     SampleRow* w = a.rows + row;
-    if (s_weight[tid]) atomicAdd(reinterpret_cast<unsigned long long*>(&w->weight[tid]), s_weight[tid]);
-    if (s_count[tid]) atomicAdd(&w->count[tid], s_count[tid]);
+#pragma unroll
+    for (int i = tid; i < kBins; i += kBinThreads) {
+        if (s_weight[i]) atomicAdd(reinterpret_cast<unsigned long long*>(&w->weight[i]), s_weight[i]);
+        if (s_count[i]) atomicAdd(&w->count[i], s_count[i]);
+    }
 }
 
 // Inclusive sums over the workgroup's threads; s_part: one number a wave. Every thread may call it again at once.
@@ -1000,11 +1008,12 @@ extern "C" int soi_sample_tokens(const void* logits, int logits_f32, int64_t str
         return SOI_ERR_WORKSPACE;
     }
     SampleArgs a{logits, stride, u, temperature, top_p, min_p, top_k, temperature_all, top_p_all, min_p_all, top_k_all, tokens,
-                 static_cast<SampleRow*>(workspace), nullptr, static_cast<int>(batch), static_cast<int>(vocab), 0, 0};
+                 static_cast<SampleRow*>(workspace), nullptr, static_cast<int>(batch), static_cast<int>(vocab), 0, 0, 0, 0};
     a.parts = reinterpret_cast<SamplePart*>(a.rows + batch);
     a.chunks = sample_chunks(batch, vocab);
     a.chunk = static_cast<int>(ceil_div64(ceil_div64(vocab, a.chunks), kPiece) * kPiece);
     a.chunks = static_cast<int>(ceil_div64(vocab, a.chunk));
+    a.bin_chunk = static_cast<int>(ceil_div64(a.chunk, 2 * kPiece) * kPiece);
     const auto with_logits = [](int64_t n) { return n < kChunk ? ceil_div64(n, kPiece) : int64_t(kThreads); };
     a.threads = static_cast<int>((a.chunks - 1) * with_logits(a.chunk) + with_logits(vocab - int64_t(a.chunks - 1) * a.chunk));
     const dim3 grid(static_cast<unsigned>(a.chunks), static_cast<unsigned>(batch)), block(kThreads);
@@ -1014,7 +1023,8 @@ extern "C" int soi_sample_tokens(const void* logits, int logits_f32, int64_t str
         using LT = decltype(type);
         hipLaunchKernelGGL(sample_extremes_kernel<LT>, grid, block, 0, st, a);
         if (draws) {
-            hipLaunchKernelGGL(sample_bins_kernel<LT>, grid, block, 0, st, a);
+            hipLaunchKernelGGL(sample_bins_kernel<LT>, dim3(static_cast<unsigned>(ceil_div64(vocab, a.bin_chunk)), grid.y),
+                               dim3(kBinThreads), 0, st, a);
             hipLaunchKernelGGL(sample_collect_kernel<LT>, grid, block, 0, st, a);
         }
         hipLaunchKernelGGL(sample_decide_kernel<LT>, dim3(static_cast<unsigned>(batch)), block, 0, st, a);
