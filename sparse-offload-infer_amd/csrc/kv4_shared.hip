@@ -14,14 +14,16 @@
 // cw < 4 (cw 1 leaves two waves that only unpack):
 //   * S^T = K Q^T: lane (n, h) ends with the scores of column n and tokens 8 (r >> 2) + 4 h + (r & 3), r < 16; a scale group's
 //     sums are multiplied by its scale in binary32;
-//   * O^T = V^T P^T takes these, exponentiated, as its B operand as they lie, times V's scale, rounded to binary16 once: a set
-//     of weights for each scale group. V is kept as V^T [dimension][token], tokens in the order that this operand's k slots
-//     want (16 j + 4 h + 0 .. 3, + 8 .. 11 side by side: one 16-byte read). The cache's V units hold four tokens of one
-//     dimension, so unpacking writes such rows without a transposition;
+//   * O^T = V^T P^T takes these, exponentiated, as its B operand as they lie, times V's scale: a set of weights for each scale
+//     group, each in two binary16 numbers, the product rounded and what that left, with a matrix instruction for either. V is
+//     kept as V^T [dimension][token], tokens in the order that this operand's k slots want (16 j + 4 h + 0 .. 3, + 8 .. 11 side by
+//     side: one 16-byte read). The cache's V units hold four tokens of one dimension, so unpacking writes such rows without a
+//     transposition;
 //   * the base of the exponents follows weight times the stage's largest V scale, so the products fill binary16's range
-//     whatever V's size: rounded by 2^-11 of themselves down to 2^-26 of the largest weight times the largest scale that meets
-//     it, 0 below 2^-37 of it. (K and V rounded to binary16 values in LDS would save a third of the vector work, but their
-//     rounding triples the output's error.)
+//     whatever V's size: off by 2^-22 of themselves, or by 2^-25 where the unit's largest product so far is at least 2^11: 2^-36
+//     of it. (One binary16 number a weight is off by 2^-11: 45 instead of 49 us for the 64 sequences below, and outputs that
+//     differ by 2e-4 from the formula's in 32 bits, where those of two numbers differ by 3e-5. K and V rounded to binary16
+//     values in LDS would save a third of the vector work, with such a rounding each.)
 // 16-byte chunks are XOR-swizzled so that operand reads and the unpacked rows' writes spread over the banks.
 //
 // 64 sequences behind 8192 shared tokens (up to 512 of their own; 32 / 8 heads of 128): plan 5.8, units 37, states added 5.7 us, where
@@ -227,11 +229,11 @@ __device__ __forceinline__ void sh_meet() {
     asm volatile("" ::: "memory");
 }
 
-// (a lo(s), b hi(s)) as binary16, each product rounded once
-__device__ __forceinline__ uint32_t times_f16(float a, float b, uint32_t s) {
-    const f16x2 w = as_f16x2(s);  // (fma, not a product: one mixed-precision instruction)
-    return __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(fmaf(a, static_cast<float>(w.x), 0.0f)),
-                                              static_cast<f16>(fmaf(b, static_cast<float>(w.y), 0.0f))});
+// (a lo(s), b hi(s)) as binary16, each product rounded once; less the same products in `from`
+__device__ __forceinline__ uint32_t times_f16(float a, float b, uint32_t s, uint32_t from = 0) {
+    const f16x2 w = as_f16x2(s), f = as_f16x2(from);  // (fma, not a product: one mixed-precision instruction)
+    return __builtin_bit_cast(uint32_t, f16x2{static_cast<f16>(fmaf(a, static_cast<float>(w.x), -static_cast<float>(f.x))),
+                                              static_cast<f16>(fmaf(b, static_cast<float>(w.y), -static_cast<float>(f.y)))});
 }
 
 // physical 16-byte chunk of chunk c: c ^ swizzle, of a K row (HD / 8 chunks) and of a V row (8 chunks: the stage's tokens)
@@ -487,13 +489,20 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD, GS)) void kv4_shared_kern
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            u32x4 pb[2];
+            u32x4 pb[2], rest[2];  // the products rounded, and what the rounding left
             const int v_at = sh_here(n * VROWB + (((4 * sub + hh) ^ sh_swz_v(n)) << 4));
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const u32x2 sc = *reinterpret_cast<const u32x2*>(&s_vs[g][at + 8 * x]);
-                pb[x >> 1][2 * (x & 1)] = times_f16(z[4 * x], z[4 * x + 1], sc.x);
-                pb[x >> 1][2 * (x & 1) + 1] = times_f16(z[4 * x + 2], z[4 * x + 3], sc.y);
+                const uint32_t w[2] = {sc.x, sc.y};
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float p0 = z[4 * x + 2 * y], p1 = z[4 * x + 2 * y + 1];
+                    uint32_t top = times_f16(p0, p1, w[y]);
+                    asm("" : "+v"(top));  // (one value: it came in two roundings where the compiler made it twice)
+                    pb[x >> 1][2 * (x & 1) + y] = top;
+                    rest[x >> 1][2 * (x & 1) + y] = times_f16(p0, p1, w[y], top);
+                }
             }
 #pragma unroll
             for (int d = g * (GS / 32); d < (g + 1) * (GS / 32); ++d) {
@@ -501,6 +510,7 @@ __global__ __launch_bounds__(kShThreads, sh_per_cu(HD, GS)) void kv4_shared_kern
                 for (int x = 0; x < 2; ++x) {
                     const f16x8 vf = *reinterpret_cast<const f16x8*>(s_v + (v_at ^ (x << 5)) + 32 * d * VROWB);
                     acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, __builtin_bit_cast(f16x8, pb[x]), acc[d], 0, 0, 0);
+                    acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, __builtin_bit_cast(f16x8, rest[x]), acc[d], 0, 0, 0);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
