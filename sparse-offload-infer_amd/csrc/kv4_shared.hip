@@ -33,6 +33,7 @@
 // kept in registers until they spilled, cost a third of the units' time.
 #include "soi_host.h"
 #include "soi_kv4.h"
+#include "soi_kv4_shared_plan.h"
 #include "soi_attn.h"
 
 #include <type_traits>
@@ -43,7 +44,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kShWaves = 4, kShThreads = kShWaves * kWave, kShKeys = 64;
+constexpr int kShWaves = 4, kShThreads = kShWaves * kWave;
 constexpr int kShRound = 64;                     // shared tokens end on a multiple of this
 constexpr int kShMost = 2048;                    // sequences of a call
 constexpr float kShLow = 12.0f, kShHigh = 15.0f;  // a column's largest weight times V scale is between 2^kShLow and 2^kShHigh
@@ -76,9 +77,6 @@ struct ShArgs {
     int cw, want, most_units, states;
     float scale_log2;
 };
-
-// What a stage costs a wave, roughly (in units of ten cycles): unpacking its part, and cw rounds of 32 tokens.
-__device__ __forceinline__ int sh_cost(int cw) { return 60 + 90 * (cw == 4 ? 2 : 1); }
 
 template <int NT>
 __device__ __forceinline__ int64_t sh_scan(int64_t v, int64_t* s_part, int64_t& all) {  // exclusive over the threads, and the sum
@@ -152,26 +150,19 @@ __global__ __launch_bounds__(NT) void kv4_shared_plan_kernel(const ShArgs a, con
     }
     __syncthreads();
     const int width = 32 * a.cw, own_tiles = (rep + 31) / 32;
-    auto stages = [](int keys) { return (keys + kShKeys - 1) / kShKeys; };
     auto keys_of = [&](int g) { return s_row[g] == 0x7fffffff ? 0 : s_keys[g]; };
     auto columns = [&](int g) { return (s_cu[g + 1] - s_cu[g]) * rep; };
     auto tiles = [&](int g) { return (columns(g) + width - 1) / width; };
     auto start_of = [&](int b) { return s_group[b] == kNone ? 0 : keys_of(s_group[b]); };
     int64_t cost = 0, total;
-    for (int g = tid; g < G; g += NT) cost += static_cast<int64_t>(tiles(g)) * stages(keys_of(g)) * sh_cost(a.cw);
-    for (int b = tid; b < B; b += NT) cost += static_cast<int64_t>(own_tiles) * stages(s_len[b] - start_of(b)) * sh_cost(1);
+    for (int g = tid; g < G; g += NT) cost += static_cast<int64_t>(tiles(g)) * sh_stages(keys_of(g)) * sh_cost(a.cw);
+    for (int b = tid; b < B; b += NT) cost += static_cast<int64_t>(own_tiles) * sh_stages(s_len[b] - start_of(b)) * sh_cost(1);
     sh_scan<NT>(cost, s_part, total);
-    auto per_unit = [&](int of) {  // stages of a unit, each of cost `of`
-        const uint64_t d = static_cast<uint64_t>(a.want) * of, t = static_cast<uint64_t>(total);
-        const uint64_t n = (t | d) >> 32 ? (t + d - 1) / d : (static_cast<uint32_t>(t) + static_cast<uint32_t>(d) - 1) / static_cast<uint32_t>(d);
-        return static_cast<int>(n < 1 ? 1 : n);
-    };
-    const int pre_per = per_unit(sh_cost(a.cw)), own_per = per_unit(sh_cost(1));
-    auto splits = [&](int keys, int per) { return (stages(keys) + per - 1) / per; };
+    const int pre_per = sh_per_unit(total, a.want, sh_cost(a.cw)), own_per = sh_per_unit(total, a.want, sh_cost(1));
     auto both = [](int units, int64_t states) { return states << 24 | units; };  // (at most 65535 units, 2^31 states)
     int64_t at = 0;
     for (int g0 = 0; g0 < G; g0 += NT) {
-        const int g = g0 + tid, ns = g < G ? splits(keys_of(g), pre_per) : 0;
+        const int g = g0 + tid, ns = g < G ? sh_splits(keys_of(g), pre_per) : 0;
         int64_t all;
         const int64_t x = at + sh_scan<NT>(ns ? both(tiles(g) * ns, static_cast<int64_t>(columns(g)) * ns) : 0, s_part, all);
         if (g < G) {
@@ -182,7 +173,7 @@ __global__ __launch_bounds__(NT) void kv4_shared_plan_kernel(const ShArgs a, con
     }
     __syncthreads();
     for (int g = wave; g < G; g += NT / kWave) {  // a wave lists a group's units
-        const int keys = keys_of(g), ns = splits(keys, pre_per), cols = columns(g), n = ns ? tiles(g) * ns : 0;
+        const int keys = keys_of(g), ns = sh_splits(keys, pre_per), cols = columns(g), n = ns ? tiles(g) * ns : 0;
         for (int i = lane; i < n; i += kWave) {
             const int t = i / ns, k = i - t * ns, k0 = k * pre_per * kShKeys, k1 = k0 + pre_per * kShKeys;
             const int left = cols - t * width;
@@ -192,7 +183,7 @@ __global__ __launch_bounds__(NT) void kv4_shared_plan_kernel(const ShArgs a, con
         }
     }
     for (int b0 = 0; b0 < B; b0 += NT) {
-        const int b = b0 + tid, L = b < B ? s_len[b] : 0, start = b < B ? start_of(b) : 0, ns = splits(L - start, own_per);
+        const int b = b0 + tid, L = b < B ? s_len[b] : 0, start = b < B ? start_of(b) : 0, ns = sh_splits(L - start, own_per);
         int64_t all;
         const int64_t x = at + sh_scan<NT>(both(ns * own_tiles, static_cast<int64_t>(ns) * rep), s_part, all);
         at += all;
@@ -205,8 +196,11 @@ __global__ __launch_bounds__(NT) void kv4_shared_plan_kernel(const ShArgs a, con
                 if (u < a.most_units)
                     a.units[u] = ShUnit{b, k0, k1 < L ? k1 : L, b, 32 * t, left < 32 ? left : 32, s + k * rep + 32 * t, 1};
             }
-        const int g = start ? s_group[b] : 0, cols = start ? columns(g) : 0;
-        a.seqs[b] = ShSeq{start ? s_state[g] + (b - s_cu[g]) * rep : 0, cols, start ? splits(start, pre_per) : 0, s, ns, {0, 0, 0}};
+        const int g = start ? s_group[b] : 0, cols = start ? columns(g) : 0, ps = start ? s_state[g] : 0;
+        const int pn = start ? sh_splits(start, pre_per) : 0;
+        // (none where states would lie past the workspace, which ShSizes says they do not)
+        const bool pre_fits = ps + static_cast<int64_t>(pn) * cols <= a.states, own_fits = s + static_cast<int64_t>(ns) * rep <= a.states;
+        a.seqs[b] = ShSeq{start ? ps + (b - s_cu[g]) * rep : 0, cols, pre_fits ? pn : 0, s, own_fits ? ns : 0, {0, 0, 0}};
     }
     if (tid == 0) {
         const int units = static_cast<int>(at & 0xffffff);
@@ -638,29 +632,9 @@ __global__ __launch_bounds__(256) void kv4_shared_combine_kernel(const ShArgs a)
         stg(a.out + (static_cast<int64_t>(b) * a.NQ + h) * HD + 64 * e + lane, f32_to_f16_bits(l == 0.0f ? 0.0f : v[e] / l));
 }
 
-// Units aimed at: two workgroups to a CU (one for heads of 256). 64 sequences of up to 512 tokens behind 8192 shared ones, 32 /
-// 8 heads of 128, with 1 / 2 / 4 / 8: 55 / 37 / 45 / 45 us for the units and 6 / 8 / 14 / 26 us to add up their states.
-// The most units and states there can be. Each of the plan's splits but a tile's last costs at least a unit's share, so there
-// are at most `want` units more than tiles.
-struct ShSizes {
-    int64_t cw, want, units, states;
-    ShSizes(int64_t B, int64_t G, int64_t NQ, int64_t NKV, int64_t hd, int64_t max_len, int64_t max_shared) {
-        const int64_t rep = NQ / NKV, per_group = ceil_div64(B * rep, G < 1 ? 1 : G);
-        cw = per_group > 64 ? 4 : per_group > 32 ? 2 : 1;
-        want = ceil_div64(256 * (hd == 256 ? 1 : 2), NKV);
-        const int64_t pre_tiles = B * rep / (32 * cw) + G, own_tiles = B * ceil_div64(rep, 32);
-        auto units_of = [&](int64_t tiles, int64_t keys) {
-            const int64_t most = tiles * ceil_div64(keys, kShKeys);
-            return want + tiles < most ? want + tiles : most;
-        };
-        const int64_t pre = units_of(pre_tiles, max_shared), own = units_of(own_tiles, max_len);
-        units = pre + own;
-        states = pre * 32 * cw + own * (rep < 32 ? rep : 32);
-    }
-    size_t bytes(int64_t B, int64_t NKV, int64_t hd) const {
-        return sizeof(ShHead) + units * sizeof(ShUnit) + B * sizeof(ShSeq) + static_cast<size_t>(NKV) * states * (hd + 4) * 4;
-    }
-};
+static size_t sh_bytes(const ShSizes& sz, int64_t B, int64_t NKV, int64_t hd) {
+    return sizeof(ShHead) + sz.units * sizeof(ShUnit) + B * sizeof(ShSeq) + static_cast<size_t>(NKV) * sz.states * (hd + 4) * 4;
+}
 
 static bool sh_sizes_fit(int64_t B, int64_t G, int64_t NQ, int64_t NKV, int64_t hd, int64_t max_len, int64_t max_shared) {
     return B >= 1 && B <= kShMost && G >= 0 && G <= kShMost && NKV >= 1 && NQ >= NKV && NQ <= 65535 && NQ % NKV == 0 && hd >= 1 && max_len >= 0 &&
@@ -675,7 +649,7 @@ extern "C" size_t soi_kv4_shared_attention_workspace_bytes(int64_t batch, int64_
                                                            int64_t num_kv_heads, int64_t head_dim, int64_t max_len,
                                                            int64_t max_shared) {
     if (!sh_sizes_fit(batch, groups, num_q_heads, num_kv_heads, head_dim, max_len, max_shared)) return 0;
-    return ShSizes(batch, groups, num_q_heads, num_kv_heads, head_dim, max_len, max_shared).bytes(batch, num_kv_heads, head_dim);
+    return sh_bytes(ShSizes(batch, groups, num_q_heads, num_kv_heads, head_dim, max_len, max_shared), batch, num_kv_heads, head_dim);
 }
 
 extern "C" int soi_kv4_shared_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,
@@ -700,7 +674,7 @@ extern "C" int soi_kv4_shared_attention(const soi_kv4_cache* cache, const uint16
     SOI_REQUIRE(q && out && q != out && cu_groups && shared_lens, "%s: null pointer or out = q", what);
     const ShSizes sz(B, groups, num_q_heads, NKV, hd, max_len, max_shared);
     SOI_REQUIRE(sz.units <= 65535 && sz.states < (int64_t(1) << 31), "%s: too many sequences and heads", what);
-    const size_t need = sz.bytes(B, NKV, hd);
+    const size_t need = sh_bytes(sz, B, NKV, hd);
     if (!workspace || workspace_bytes < need || !aligned16(workspace)) {
         set_last_error("%s: workspace of %zu bytes (16-byte aligned) needed, got %zu", what, need, workspace_bytes);
         return SOI_ERR_WORKSPACE;
