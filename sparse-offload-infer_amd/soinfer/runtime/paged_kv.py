@@ -14,7 +14,8 @@ a fixed length per layer (python/soinfer/runtime/generate.py:276-310).
     out = cache.attend(layer, step, cache.append(layer, step, qkv, qn, kn, cos, sin, NQ))
     c = cache.fork(a)                                        # begins with a's whole pages, which it does not copy
 
-Sequences next to each other in a decode step that share pages are attended to together: their common pages are read once.
+Sequences next to each other in a decode step that share pages are attended to together, their common pages read once, where
+that is faster.
 
 One page number stands for the same page in every layer, so a step's tables serve them all.
 """
@@ -43,6 +44,7 @@ class Step:
     cu_groups: torch.Tensor | None = None    # int32 [groups + 1]: sequences next to each other that share pages,
     shared_lens: torch.Tensor | None = None  # int32 [B]: and the tokens these hold (None, None: no sequences do)
     max_shared: int = 0
+    groups: tuple[tuple[int, int], ...] = ()  # of each group: its sequences, the tokens that they share
 
 
 class PagedKV4:
@@ -169,6 +171,7 @@ class PagedKV4:
         step = Step(seqs, tuple(new.values()), lens, t.view(table.shape), ln, c, int(cu[-1]), max(new.values()), max(lens))
         if groups:
             step.cu_groups, step.shared_lens, step.max_shared = gr, sh, max(shared)
+            step.groups = tuple((end - first, shared[first]) for first, end in zip(groups, groups[1:]))
         return step
 
     # ---- the operators --------------------------------------------------------------------------
@@ -205,10 +208,31 @@ class PagedKV4:
         k, v = ops.kv4_read(*self._layer(layer), step.block_table, step.seq_lens, cu_k, int(cu[-1]))
         return k, v, cu_k
 
+    def _together(self, step: Step, num_q_heads: int) -> bool:
+        """Whether ops.kv4_shared_attention is the faster one. Counted in tokens of ops.kv4_decode_attention: a token behind the
+        shared ones costs four (it fills a tile of 32 columns with one sequence's heads), a shared one eight for every 128
+        columns (sequence, head) of its group, five for every 64 or 32 where groups are small; its two more launches are
+        400000 (token, KV head). Of 8607 random steps with heads of 64 and 128 the choice is 0.4 % slower than the better one
+        on average, 1.37 times at worst; decode alone would be 15 % and 5.8 times, the shared form alone 35 to 51 %. 48 contexts
+        of 8192 tokens, 32 / 8 heads of 128, 768 / 4096 / 6144 / 7360 of them shared: decode 84 / 66 / 66 / 66 us, shared
+        290 / 244 / 143 / 61. With heads of 256, one workgroup to a CU, it lost 1384 of 1387 (2.1 times the time on average)."""
+        B, G, rep = len(step.sequences), len(step.groups), num_q_heads // self.num_kv_heads
+        if not G or B > 2048 or self.head_dim > 128:  # (2048: sequences that it takes)
+            return False
+        columns = -(-B * rep // G)
+        width, price = (128, 8) if columns > 64 else (64, 5) if columns > 32 else (32, 5)
+        tokens = own = sum(step.lens)
+        cost = 0
+        for n, shared in step.groups:
+            shared -= shared % 64  # (it shares whole 64 tokens)
+            own -= n * shared
+            cost += price * -(-n * rep // width) * shared
+        return (tokens - 4 * own - cost) * self.num_kv_heads >= 400_000
+
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float | None = None) -> torch.Tensor:
         """ops.kv4_decode_attention: one query token of each sequence, q [B, NQ, hd], over its cached tokens. Where sequences
-        next to each other share pages, ops.kv4_shared_attention (up to its 2048 sequences)."""
-        if step.cu_groups is not None and len(step.sequences) <= 2048:
+        next to each other share pages and it is faster, ops.kv4_shared_attention."""
+        if q.dim() == 3 and self._together(step, q.shape[1]):
             return ops.kv4_shared_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.cu_groups,
                                             step.shared_lens, step.max_len, min(step.max_shared, step.max_len), scale)
         return ops.kv4_decode_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.max_len, scale)
