@@ -35,7 +35,8 @@ HIP_SOURCES = ["decoder.hip", "capi.hip", "gemv_int4.hip", "gemv_int8.hip", "top
                "prompt_attention.hip", "int8_rows.hip", "int8_linear.hip", "sample.hip", "kv4_shared.hip"]
 # Kernels of these may not spill: a version of the decode attention that did came back with a register of Q lost, for a
 # reason that was never found.
-NO_SPILLS = ["kv4_cache.hip", "kv4_attention.hip", "prompt_attention.hip", "int8_linear.hip", "kv4_shared.hip"]
+NO_SPILLS = ["kv4_cache.hip", "kv4_attention.hip", "prompt_attention.hip", "int8_linear.hip", "kv4_shared.hip",
+             "sample.hip"]
 HIP_LIB = SOINFER / "libsoinfer_hip.so"
 EXT_LIB = SOINFER / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 

@@ -937,12 +937,17 @@ __global__ __launch_bounds__(kThreads) void sample_decide_kernel(const SampleArg
     uint64_t place = ldg(&w->list[tid]);
     const uint32_t listed = ldg(&w->listed);
     const float u = ldg(a.u + row);
-    const SamplePlan s = sample_plan(a, row);
-    if (s.greedy) {
-        if (tid == 0) stg(a.tokens + row, s.first);
-        return;
+    __shared__ SamplePlan s_plan;  // (in scalar registers it spilled some)
+    {
+        const SamplePlan p = sample_plan(a, row);
+        if (p.greedy) {
+            if (tid == 0) stg(a.tokens + row, p.first);
+            return;
+        }
+        if (tid == 0) s_plan = p;
     }
-    sum_bins(b, sh);
+    sum_bins(b, sh);  // (its barriers are behind the plan's writes)
+    const SamplePlan& s = s_plan;
     int token;
     if (listed <= kList) {
         const int n = static_cast<int>(listed);
