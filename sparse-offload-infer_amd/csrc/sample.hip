@@ -11,11 +11,15 @@
 //
 // No sort of the row. Its weights go into kBins bins of equal width in z (a histogram in LDS of each chunk, added up in
 // memory); the running sums over the bins say which bins the k-th token, the p border, the min_p border and the drawn token
-// can lie in; only the tokens of those few bins (a few hundred) are collected, and sorted, or searched by radix passes in LDS.
+// can lie in; only the tokens of those few bins are collected (a few hundred, in flat rows a thousand or two), and sorted, or
+// searched by radix passes in LDS. The bins' width follows from the row's lowest logits, a few far below the others left aside:
+// with the smallest logit, one of -1e4 or -infinity in a row of 151936 of deviation 0.35 spread its tokens over a tenth of the
+// bins, and it took 200 to 505 us instead of 26 to 28.
 // Rows with a top-k of up to kMostK need no weights before that: the bins down to the k-th token are counted and collected whole,
 // and of the other tokens only those are looked at that reach the smallest of the first launch's threads' largest logits (one a
 // thread does, which are at least k).
-// Bins that hold more than kList tokens (many equal logits) are searched by the same passes over the row.
+// Bins that hold more than kList tokens (many equal logits, or nearly so beside others far below) are searched by the same passes
+// over the row, by one workgroup.
 //
 // Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.3, 4.0,
 // 6.7 and 8.6 us), for many by the three passes over the logits and the binary64 exponentials and LDS atomics of the second (200
@@ -43,7 +47,7 @@ struct SampleRow {  // of the workspace
 };
 struct SamplePart {  // a chunk's extremes
     uint64_t top;    // key of the largest, ~index
-    uint32_t low;    // key of the smallest number
+    uint32_t low;    // key that stands for its smallest numbers: the median of its waves' smallest
     uint32_t bound;  // key of the smallest of the threads' largest: one token a thread reaches it
 };
 
@@ -152,6 +156,18 @@ __device__ __forceinline__ N wave_top(N v) {
     return wave_run(v, [](N a, N b) { return a > b ? a : b; });
 }
 
+// The median (of an even number: the lower one) of the first n lanes' keys, 1 <= n <= 16, but for their last four bits.
+__device__ __forceinline__ uint32_t median_key(uint32_t key, int n) {
+    constexpr int kMost = 16;
+    const int lane = threadIdx.x & 63;
+    const uint32_t mine = lane < n ? (key & ~(kMost - 1u)) | static_cast<uint32_t>(lane) : 0xffffffffu;
+    int rank = 0;
+#pragma unroll
+    for (int j = 0; j < kMost; ++j) rank += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) < mine;
+    const int at = __builtin_ctzll(ballot(rank == (n - 1) / 2));
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), at)) & ~(kMost - 1u);
+}
+
 template <class LT>
 __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleArgs a) {
     __shared__ uint64_t s_top[kThreads / kWave];
@@ -224,7 +240,7 @@ __global__ __launch_bounds__(kThreads) void sample_extremes_kernel(const SampleA
     __syncthreads();
     if (wave == 0) {
         top = wave_top(lane < kThreads / kWave ? s_top[lane] : uint64_t(0));
-        low = ~wave_top(lane < kThreads / kWave ? ~s_low[lane] : 0u);
+        low = median_key(s_low[lane & (kThreads / kWave - 1)], min(kThreads / kWave, (hi - lo + kWave * kPiece - 1) / (kWave * kPiece)));
         bound = ~wave_top(lane < kThreads / kWave ? ~s_bound[lane] : 0u);
     }
     if (tid == 63) {
@@ -253,20 +269,18 @@ struct SamplePlan {
 
 __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) {
     const int lane = threadIdx.x & 63;
-    const SamplePart* p = a.parts + static_cast<int64_t>(row) * a.chunks;
+    const SamplePart* p = a.parts + static_cast<int64_t>(row) * a.chunks;  // (the lanes' chunks)
     uint64_t top = 0;
     uint32_t low = 0xffffffffu, bound = 0xffffffffu;
-    for (int c = lane; c < a.chunks; c += kWave) {
-        const uint64_t t = ldg(&p[c].top);
-        const uint32_t l = ldg(&p[c].low), m = ldg(&p[c].bound);
-        top = t > top ? t : top;
-        low = l < low ? l : low;
-        bound = m < bound ? m : bound;
+    static_assert((1 << 19) <= kChunk * kWave, "a lane for each chunk");
+    if (lane < a.chunks) {
+        top = ldg(&p[lane].top);
+        low = ldg(&p[lane].low);
+        bound = ldg(&p[lane].bound);
     }
     const auto last = [](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63)); };
     top = wave_top(top);
     top = static_cast<uint64_t>(last(static_cast<uint32_t>(top >> 32))) << 32 | last(static_cast<uint32_t>(top));
-    low = ~last(wave_top(~low));
     bound = ~last(wave_top(~bound));
     const float T = a.temperature ? ldg(a.temperature + row) : a.temperature_all;
     const float tp = a.top_p ? ldg(a.top_p + row) : a.top_p_all, mp = a.min_p ? ldg(a.min_p + row) : a.min_p_all;
@@ -288,7 +302,20 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
         const double z = s.z(value_of(bound));
         s.z_limit = z < s.z_limit ? z : s.z_limit;
     }
-    const double most = low > kKeyNegInf ? s.z(value_of(low)) : s.z_limit, span = most < s.z_limit ? most : s.z_limit;
+    // The bins reach to the lowest of the chunks' numbers that is at most four times as far from the largest as is usual among
+    // them (their mean on the float's pattern, which is one of logarithms): a few logits far below the rest (masks of -1e4 or
+    // -infinity) leave the others their bins.
+    const double far = lane < a.chunks && low > kKeyNegInf ? s.z(value_of(low)) : 1e300;
+    const uint32_t base = __builtin_bit_cast(uint32_t, 0.01f);
+    const uint32_t log_far = __builtin_bit_cast(uint32_t, fminf(fmaxf(static_cast<float>(far), 0.01f), 128.0f)) - base;
+    const uint32_t logs = last(wave_run(lane < a.chunks ? log_far >> 3 : 0u, [](uint32_t v, uint32_t w) { return v + w; }));
+    const float usual = __builtin_bit_cast(float, base + (logs / static_cast<uint32_t>(a.chunks) << 3));
+    const uint32_t lowest = ~last(wave_top(static_cast<float>(far) <= 4.0f * usual ? ~low : 0u));
+    double span = s.z_limit;
+    if (lowest < kKeyInf) {
+        const double most = s.z(value_of(lowest));
+        span = most < span ? most : span;
+    }
     s.per_z = span > 1e-290 ? kBins / span : 0.0;
     for (double* d : {&s.max, &s.inv_t, &s.z_limit, &s.per_z, &s.min_z, &s.p}) {  // to scalar registers
         const uint64_t v = __builtin_bit_cast(uint64_t, *d);
