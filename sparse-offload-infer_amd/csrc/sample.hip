@@ -292,7 +292,7 @@ __device__ __forceinline__ SamplePlan sample_plan(const SampleArgs& a, int row) 
     if (s.greedy) return s;
     s.max = static_cast<double>(value_of(key));
     s.inv_t = 1.0 / static_cast<double>(T);
-    s.p = tp < 1.0f ? static_cast<double>(tp) : 1.0;  // (NaN: 1)
+    s.p = tp < 1.0f ? static_cast<double>(fmaxf(tp, 0.0f)) : 1.0;  // (NaN: 1; a negative sum is no whole number of p_border's)
     s.k = k > 0 ? k : 0;
     s.min_z = mp > 0.0f ? (mp < 1.0f ? -log(static_cast<double>(mp)) : 0.0) : __builtin_inf();
     // without top-p, what min-p drops does not count for anything
