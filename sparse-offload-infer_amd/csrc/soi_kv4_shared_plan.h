@@ -29,7 +29,8 @@ __host__ __device__ __forceinline__ int sh_splits(int keys, int per) { return (s
 // Units aimed at: two workgroups to a CU (one for heads of 256). 64 sequences of up to 512 tokens behind 8192 shared ones, 32 /
 // 8 heads of 128, with 1 / 2 / 4 / 8: 55 / 37 / 45 / 45 us for the units and 6 / 8 / 14 / 26 us to add up their states.
 // The most units and states there can be. Each of the plan's splits but a tile's last costs at least a unit's share, so there
-// are at most `want` units more than tiles.
+// are at most `want` units more than tiles, and as many states as columns and those units' (full tiles for all of the units: 217
+// MB instead of 79 for 2048 sequences in 1024 groups, 32 / 8 heads of 128).
 struct ShSizes {
     int64_t cw, want, units, states;
     ShSizes(int64_t B, int64_t G, int64_t NQ, int64_t NKV, int64_t hd, int64_t max_len, int64_t max_shared) {
@@ -44,7 +45,11 @@ struct ShSizes {
         };
         const int64_t pre = units_of(pre_tiles, max_shared), own = units_of(own_tiles, max_len);
         units = pre + own;
-        states = pre * 32 * cw + own * (rep < 32 ? rep : 32);
+        auto states_of = [&](int64_t all, int64_t wide) {
+            const int64_t most = B * rep + want * wide;
+            return all * wide < most ? all * wide : most;
+        };
+        states = states_of(pre, 32 * cw) + states_of(own, rep < 32 ? rep : 32);
     }
 };
 
