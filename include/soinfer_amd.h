@@ -807,11 +807,12 @@ int soi_kv4_decode_attention(const soi_kv4_cache* cache, const uint16_t* q, int6
  * first shared_lens[b] tokens (int32 [batch]; at most max_shared) are the same in every table row of the group. They are
  * read and multiplied once for the group, through the row of one of its sequences; the tokens behind them through each
  * sequence's own row. What counts as shared is the least of min(shared_lens[b], seq_lens[b]) over the group's sequences where
- * that is at least 64, rounded down to a multiple of 64; the others, and sequences in no group, share nothing. The product of
- * a token's weight and a V scale is off by 2^-22 of itself, or where that is more by 2^-36 of the largest weight times the
- * largest V scale (of any group) in the context. How contexts are split follows from all lengths, as there. batch and groups
- * at most 2048, max_shared at most max_len. The workspace is 16-byte aligned, needs no initial value and may be reused by the
- * next call on the stream; calls that overlap need one each. */
+ * that is at least 64, rounded down to a multiple of 64; the others, and sequences in no group, share nothing. Faster than
+ * soi_kv4_decode_attention where many sequences share most of what they hold; a token behind the shared ones costs some four
+ * of that operator's. The product of a token's weight and a V scale is off by 2^-22 of itself, or where that is more by 2^-36 of
+ * the largest weight times the largest V scale (of any group) in the context. How contexts are split follows from all lengths,
+ * as there. batch and groups at most 2048, max_shared at most max_len. The workspace is 16-byte aligned, needs no initial
+ * value and may be reused by the next call on the stream; calls that overlap need one each. */
 size_t soi_kv4_shared_attention_workspace_bytes(int64_t batch, int64_t groups, int64_t num_q_heads, int64_t num_kv_heads,
                                                 int64_t head_dim, int64_t max_len, int64_t max_shared);
 int soi_kv4_shared_attention(const soi_kv4_cache* cache, const uint16_t* q, int64_t q_stride, int64_t num_q_heads,

@@ -11,7 +11,7 @@
 //
 // Few rows are bound by the weights' bytes, or by latency: 5 rows 2048 -> 4096 3.8 us, 48 rows 2048 -> 151936 62 us (5.2 TB/s).
 // Many are bound by the operands' way through LDS, the power limit and gate_up's epilogue: 4096 rows 6144 -> 2048 with residual
-// 55 us (1.88 POP/s; a library product without the epilogue 61 us), 8192 rows 2048 -> 2 x 6144 215 us (1.92 POP/s; library 244).
+// 56 us (1.84 POP/s; a library product without the epilogue 61 us), 8192 rows 2048 -> 2 x 6144 225 us (1.83 POP/s; library 244).
 #include "soi_host.h"
 #include "soi_device.h"
 

@@ -22,15 +22,17 @@
 //   * the base of the exponents follows weight times the stage's largest V scale, so the products fill binary16's range
 //     whatever V's size: off by 2^-22 of themselves, or by 2^-25 where the unit's largest product so far is at least 2^11: 2^-36
 //     of it. (One binary16 number a weight is off by 2^-11: 45 instead of 49 us for the 64 sequences below, and outputs that
-//     differ by 2e-4 from the formula's in 32 bits, where those of two numbers differ by 3e-5. K and V rounded to binary16
+//     differ by 2e-4 from the formula's in 32 bits, where those of two numbers differ by 1e-5 to 4e-5. K and V rounded to binary16
 //     values in LDS would save a third of the vector work, with such a rounding each.)
 // 16-byte chunks are XOR-swizzled so that operand reads and the unpacked rows' writes spread over the banks.
 //
-// 64 sequences behind 8192 shared tokens (up to 512 of their own; 32 / 8 heads of 128): plan 5.8, units 37, states added 5.7 us, where
-// kv4_attention.hip reads 64 times as much. Bound by the launches' latency and, in a unit, by vector instructions: unpacking, and
-// scales, exponentials and conversions of every score, beside 8.9 GFLOP of products (7 us at a library product's rate). Stages of
-// 128 tokens (two workgroups to a CU instead of three) 57 us in all, of 64 45; page table lookups with branches, and addresses
-// kept in registers until they spilled, cost a third of the units' time.
+// 64 sequences behind 8192 shared tokens (up to 512 of their own; 32 / 8 heads of 128): plan 5.8, units 42, states added 5.8 us;
+// kv4_attention.hip, which reads the prompt 64 times, takes 113 us, but is faster where less is shared: a token behind the shared
+// ones costs it a quarter. Bound by the launches' latency and, in a unit, by vector instructions: unpacking, and scales,
+// exponentials and conversions of every score, beside 8.9 GFLOP of products (7 us at a library product's rate; half as much
+// again for the weights' second numbers). With one number a weight, stages of 128 tokens (two workgroups to a CU instead of three)
+// took 57 us in all and those of 64 took 45; page table lookups with branches, and addresses kept in registers until they spilled,
+// cost a third of the units' time.
 #include "soi_host.h"
 #include "soi_kv4.h"
 #include "soi_kv4_shared_plan.h"

@@ -21,9 +21,9 @@
 // Bins that hold more than kList tokens (many equal logits, or nearly so beside others far below) are searched by the same passes
 // over the row, by one workgroup.
 //
-// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.3, 4.0,
-// 6.7 and 8.6 us), for many by the three passes over the logits and the binary64 exponentials and LDS atomics of the second (200
-// rows, each with its own settings: 18, 37, 32 and 17 us; one pass at a large copy's rate is 12 us). The collected tokens of a row
+// Four launches: largest and smallest logit, bins, collect, decide. Bound by latency for one row (151936 binary16 logits: 4.6, 4.3,
+// 7.0 and 9.9 us), for many by the three passes over the logits and the binary64 exponentials and LDS atomics of the second (200
+// rows, each with its own settings: 18, 37, 32 and 20 us; one pass at a large copy's rate is 12 us). The collected tokens of a row
 // are sorted, by one wave where they are up to 256 (one row 29 -> 23 us beside radix passes for all), by the workgroup up to 2048
 // (the last launch of the 200 rows 34 -> 17 us).
 #include "soi_host.h"

@@ -27,7 +27,8 @@ __host__ __device__ __forceinline__ int sh_per_unit(uint64_t total, int want, in
 __host__ __device__ __forceinline__ int sh_splits(int keys, int per) { return (sh_stages(keys) + per - 1) / per; }
 
 // Units aimed at: two workgroups to a CU (one for heads of 256). 64 sequences of up to 512 tokens behind 8192 shared ones, 32 /
-// 8 heads of 128, with 1 / 2 / 4 / 8: 55 / 37 / 45 / 45 us for the units and 6 / 8 / 14 / 26 us to add up their states.
+// 8 heads of 128, with 1 / 2 / 4 / 8: 55 / 37 / 45 / 45 us for the units and 6 / 8 / 14 / 26 us to add up their states
+// (weights in one binary16 number then; 42 us now at 2).
 // The most units and states there can be. Each of the plan's splits but a tile's last costs at least a unit's share, so there
 // are at most `want` units more than tiles, and as many states as columns and those units' (full tiles for all of the units: 217
 // MB instead of 79 for 2048 sequences in 1024 groups, 32 / 8 heads of 128).
