@@ -21,7 +21,7 @@ One page number stands for the same page in every layer, so a step's tables serv
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -45,6 +45,7 @@ class Step:
     shared_lens: torch.Tensor | None = None  # int32 [B]: and the tokens these hold (None, None: no sequences do)
     max_shared: int = 0
     groups: tuple[tuple[int, int], ...] = ()  # of each group: its sequences, the tokens that they share
+    together: dict[int, bool] = field(default_factory=dict)  # by query heads: whether attend takes the groups together
 
 
 class PagedKV4:
@@ -232,7 +233,10 @@ class PagedKV4:
     def attend(self, layer: int, step: Step, q: torch.Tensor, scale: float | None = None) -> torch.Tensor:
         """ops.kv4_decode_attention: one query token of each sequence, q [B, NQ, hd], over its cached tokens. Where sequences
         next to each other share pages and it is faster, ops.kv4_shared_attention."""
-        if q.dim() == 3 and self._together(step, q.shape[1]):
+        heads = q.shape[1] if step.groups and q.dim() == 3 else 0
+        if heads and heads not in step.together:  # (once for all layers)
+            step.together[heads] = self._together(step, heads)
+        if step.together.get(heads):
             return ops.kv4_shared_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.cu_groups,
                                             step.shared_lens, step.max_len, min(step.max_shared, step.max_len), scale)
         return ops.kv4_decode_attention(q, *self._layer(layer), step.block_table, step.seq_lens, step.max_len, scale)

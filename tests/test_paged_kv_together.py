@@ -85,3 +85,19 @@ def test_the_same_either_way(cuda, n, prompt, together):
         wide = bound + (2 * d + 2 * R.U) * vb.abs().amax()
         R.assert_within(got[b:b + 1], ref, wide, f"sequence {b}")
         R.assert_within(other[b:b + 1], ref, wide, f"sequence {b}, decode")
+
+
+def test_the_choice_is_made_once_a_step(monkeypatch):
+    """Every layer of a step attends alike, and the rule's loop over the groups runs for the first of them."""
+    from soinfer import ops
+
+    c = make(layers=3, num_pages=60, num_kv_heads=2, head_dim=64, max_len=400)
+    step = forks(c, 5, 64, 1)
+    made = []
+    monkeypatch.setattr(c, "_together", lambda s, n: made.append(n) or n == 4)
+    calls = []
+    for name in ("kv4_shared_attention", "kv4_decode_attention"):
+        monkeypatch.setattr(ops, name, lambda *a, name=name, **k: calls.append(name))
+    for heads in (4, 4, 8, 4):
+        c.attend(0, step, torch.zeros(5, heads, 64, dtype=torch.float16))
+    assert made == [4, 8] and calls == ["kv4_shared_attention"] * 2 + ["kv4_decode_attention", "kv4_shared_attention"]
